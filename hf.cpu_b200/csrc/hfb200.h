@@ -194,6 +194,28 @@ int hfb_attention_tc2_opt(const void *q, const void *k_cache, const void *v_cach
                           void *out, int T, int H, int G, int d, const float *sinks, int zero_sink, const float *slopes,
                           const float *head_scales, float softcap, hfb_stream s);
 
+/* The key/value cache in 8 bits (kv8.cuh): `cache` is [num_pages, G] records of hfb_kv8_record_bytes(block_size, d) bytes (0: sizes
+ * that are not served), 16-byte aligned: per page and head the block's key codes, value codes, key scales and value scales.  Head
+ * sizes are multiples of 16 up to 256, pages of 1 to 1,024 tokens.
+ *
+ * write: rows q [T, H d], k and v [T, G d] (the next token's `*_stride` elements further) of type `dt`.  q and k are rotated (n_rot
+ * leading numbers of a head, cos_sin float32 [n_positions, n_rot/2, 2]; pairs (i, i + n_rot/2), or (2i, 2i + 1) with `interleaved`);
+ * q goes to q_out [T, H d], k and v into the cache at slots[t] (page * block_size + row; < 0 or slots == NULL: not written).
+ * Two tokens of one call must not have the same slot.  H = 0: keys and values only.
+ * read: the rows r < used[n] of page pages[n] (< 0: none) as values, out [N, block_size, G, d]; the other rows as zeros. */
+int hfb_kv8_record_bytes(int block_size, int d);
+int hfb_kv8_write(const void *q, int64_t q_stride, const void *k, int64_t k_stride, const void *v, int64_t v_stride, int dt,
+                  const float *cos_sin, int n_rot, int n_positions, int interleaved, const int32_t *positions, const int32_t *slots,
+                  void *q_out, void *cache, int64_t num_pages, int block_size, int T, int H, int G, int d, hfb_stream s);
+int hfb_kv8_read(const void *cache, int64_t num_pages, const int32_t *pages, const int32_t *used, void *k_out, void *v_out,
+                 int out_dt, int64_t N, int block_size, int G, int d, hfb_stream s);
+
+/* Attention over it, plain kernel: one block per (token, head), as hfb_attention_plain. */
+int hfb_kv8_attention_plain(const void *q, const void *cache, int dt, const int32_t *block_table, int max_blocks,
+                            const int32_t *token_seq, const int32_t *positions, int block_size, int64_t num_pages, int window,
+                            float scale, void *out, int T, int H, int G, int d, const float *sinks, int zero_sink, const float *slopes,
+                            const float *head_scales, float softcap, hfb_stream s);
+
 /* Launches may overlap with the kernel in front (programmatic dependent launch): on by default, off with HFB_PDL=0. */
 void hfb_set_launch_overlap(int on);
 

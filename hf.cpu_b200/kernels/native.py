@@ -377,6 +377,46 @@ class NativeBackend:
                                                  c_float(scale), _p(out), c_int(T), c_int(H), c_int(G), c_int(d), c_int(dv),
                                                  c_int(v_row), *opt_args, self._stream()), "attention")
 
+    # ---- the key/value cache in 8 bits ----------------------------------------------------------------------
+    @staticmethod
+    def _here(*ts):
+        """Tensors of the current device, whose current stream the launches go to."""
+        dev = _current_device()
+        for t in ts:
+            if t is not None and (not t.is_cuda or t.device.index != dev):
+                raise KernelError(f"kernel arguments must be tensors of the current CUDA device ({dev})")
+
+    def kv8_write(self, q, k, v, cos_sin, n_rot, pairing, positions, slots, q_out, cache, H, G, d, block_size):
+        self._here(q, k, v, cos_sin, positions, slots, q_out, cache)
+        self._on_gpu(cos_sin, positions, slots, q_out, cache)
+        if slots is None:
+            G = 0                                         # (nothing is cached: only the queries are turned)
+        if H + G == 0:
+            return
+        stride = lambda x: c_int64(x.stride(0) if x is not None else 0)
+        self._check(self.lib.hfb_kv8_write(
+            _p(q), stride(q), _p(k), stride(k), _p(v), stride(v), c_int(_dt(k)), _p(cos_sin), c_int(n_rot),
+            c_int(cos_sin.shape[0] if cos_sin is not None else 0), c_int(1 if pairing == "interleaved" else 0), _p(positions), _p(slots),
+            _p(q_out), _p(cache), c_int64(cache.shape[0]), c_int(block_size), c_int(k.shape[0]), c_int(H), c_int(G), c_int(d),
+            self._stream()), "kv8_write")
+
+    def kv8_read(self, cache, pages, rows, k_out, v_out):
+        self._here(cache, pages, rows, k_out, v_out)
+        self._on_gpu(cache, pages, rows, k_out, v_out)
+        N, block_size, G, d = k_out.shape
+        self._check(self.lib.hfb_kv8_read(_p(cache), c_int64(cache.shape[0]), _p(pages), _p(rows), _p(k_out), _p(v_out), c_int(_dt(k_out)),
+                                          c_int64(N), c_int(block_size), c_int(G), c_int(d), self._stream()), "kv8_read")
+
+    def paged_attention_kv8(self, q, cache, meta, ctx, H, G, d, window, scale, out, tiles, settled=False, sinks=None, zero_sink=False,
+                            slopes=None, head_scales=None, softcap=0.0):
+        self._here(q, cache, meta.block_table, ctx.token_seq, ctx.positions, out, sinks, slopes, head_scales)
+        self._on_gpu(q, cache, meta.block_table, ctx.token_seq, ctx.positions, out, sinks, slopes, head_scales)
+        opt_args = (_p(sinks), c_int(1 if zero_sink else 0), _p(slopes), _p(head_scales), c_float(softcap))
+        self._check(self.lib.hfb_kv8_attention_plain(
+            _p(q), _p(cache), c_int(_dt(q)), _p(meta.block_table), c_int(meta.max_blocks), _p(ctx.token_seq), _p(ctx.positions),
+            c_int(meta.block_size), c_int64(cache.shape[0]), c_int(window), c_float(scale), _p(out), c_int(q.shape[0]), c_int(H), c_int(G),
+            c_int(d), *opt_args, self._stream()), "kv8_attention_plain")
+
     def swiglu(self, gu, out, interleaved):
         self._on_gpu(gu, out)
         T, F = out.shape
