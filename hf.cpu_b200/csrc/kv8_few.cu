@@ -1,0 +1,504 @@
+// Attention of few queries over the key/value cache in 8 bits (kv8.cuh): bfloat16, head sizes 64 and 128, pages of 8..64 tokens.
+//
+// What bounds it is reading the cache: d + 4 bytes a key, and as many a value.  A fifth warp keeps the copies going, one bulk copy per page
+// and head (codes and scales of keys and values are one record), several tiles of 64 keys ahead of the four warps that compute,
+// 16 keys of each tile a warp.
+//
+// Between the copy and the tensor core every byte has to become a 16-bit number, so that is what the layout serves:
+// * A code is a whole number below 2^11, which float16 holds as it is: 0x6400 | byte is 1024 + byte, minus 1152 gives the code; a
+//   permutation of bytes and half a subtraction per number.  The scales stay out of the operands: a key's multiplies its score in
+//   float32, a value's its weight.
+// * Scores are computed as S^T = K Q^T and outputs as O^T = V^T P^T: the cache fills the 16 rows of mma.m16n8k16, the (token, head)
+//   pairs that share it the 8 columns, so that up to eight of them cost one product and not half an empty one.  The numbers of
+//   a K word (four neighbours of a row) go to places k = 2c, 2c+1, 2c+8, 2c+9 of one product, and the queries are loaded
+//   in that order.  A transposing ldmatrix of value bytes gives two neighbouring numbers of two keys; the even ones make the product's
+//   rows 0..7, the odd ones 8..15, so that a thread ends up with neighbours of the output.
+// * A query row is multiplied by the power of two that brings its largest number to 2^14..2^15: float16 then holds every number
+//   of it that matters exactly (eight bits, down to 2^-31 of the largest).
+// * A weight goes into the second product as p * (scale of the value / largest scale the warp has seen) * 2^15, at most 2^15,
+//   rounded once to float16 (11 bits; down to 2^-29 of the largest at full precision, 2^-39 at all).  When a larger scale arrives the sums
+//   so far are rescaled, as they are when the running maximum grows.
+//
+// The keys of a request are cut into ranges that are merged, in the order of the ranges whoever comes last, by the CTA that
+// stores its range last.  A range has `per` tiles at least whatever the request's length, so that long requests beside short ones
+// get more CTAs instead of longer ones.
+#include "attention_common.cuh"
+#include "kv8.cuh"
+#include "tc_ptx.cuh"
+
+static thread_local cudaError_t g_launch_err = cudaSuccess;      // what the last launch_pdl returned
+
+namespace hfb {
+int *error_word();
+
+constexpr int KF_THREADS = 160, KF_MAX_SPLITS = 64;
+
+struct Kv8FewParams {
+    Kv8Params a;
+    float *part_o, *part_ml;             // several ranges: [T, H, splits, D] and [T, H, splits, 2]
+    int *counters;                       // ... one per (tile, group of heads), zero between launches
+    int splits, per;                     // most ranges of a request, fewest tiles of a range
+    int kv_share;                        // neighbouring groups of heads that read the same key/value head (a.G counts the groups)
+    int settled;                         // rows before the step's positions need no wait
+};
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+// Two bytes of a word of codes (named by the selector) as two float16 numbers.
+__device__ __forceinline__ uint32_t codes_f16(uint32_t w, uint32_t selector)
+{
+    uint32_t r;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(w), "r"(0x64646464u), "r"(selector));
+    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(r) : "r"(0x64806480u));                // 1152
+    return r;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t v)
+{
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ void mma_f16(float *c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// D: head size; NT: columns (token, head) of a tile in eights; STAGES: tiles of 64 keys in flight
+template <int D, int NT, int STAGES>
+__global__ void __launch_bounds__(KF_THREADS)
+kv8_few_kernel(Kv8FewParams f, int *err)
+{
+    const Kv8Params &p = f.a;
+    constexpr int COLS = 8 * NT, CH = D / 16;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 127u) & ~127u;
+    uint8_t *gen = smem_raw + (base - smem_u32(smem_raw));
+    const int bs = p.block_size, pages = ABN / bs;
+    const uint32_t stage_bytes = (uint32_t)pages * p.record;
+    // barriers and page masks in front of the tiles
+    const uint32_t full0 = base, empty0 = base + 8 * STAGES, tiles0 = base + 128;
+    volatile uint32_t *page_mask = (volatile uint32_t *)(gen + 16 * STAGES);
+    volatile int *abort_flag = (volatile int *)(gen + 16 * STAGES + 4 * STAGES);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (!f.settled) pdl_wait();                               // nothing is read that the kernels in front may still write
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; s++) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 4); }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncthreads();
+
+    const int tile = blockIdx.x, g = blockIdx.y, split = blockIdx.z, r = p.H / p.G;
+    const int seq = p.tile_seq[tile], t0 = p.tile_t0[tile], nt = p.tile_nt[tile];
+    const int pos_first = p.positions[t0], pos_last = p.positions[t0 + nt - 1];
+    const int lo_first = mask_lo(pos_first, p.window), lo_last = mask_lo(pos_last, p.window);
+    int kt_lo = lo_first / ABN, kt_hi = pos_last < 0 ? kt_lo : pos_last / ABN + 1;
+    const int per = max(f.per, (kt_hi - kt_lo + f.splits - 1) / f.splits);
+    const int used = max(1, (kt_hi - kt_lo + per - 1) / per);   // ranges of this request
+    if (split >= used) return;
+    kt_lo += split * per;
+    kt_hi = min(kt_hi, kt_lo + per);
+
+    float o[CH][NT][4], m[NT][2], l[NT][2], vm = 0.f;
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        m[n][0] = m[n][1] = -INFINITY;
+        l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+        for (int c = 0; c < CH; c++) o[c][n][0] = o[c][n][1] = o[c][n][2] = o[c][n][3] = 0.f;
+    }
+    const int c4 = lane & 3, row8 = lane >> 2;
+
+    if (warp == 4) {
+        // ---- the copying warp: the lanes look up 32 pages at a time, and each asks for its page -------------------------------
+        const int32_t *table = p.block_table + (size_t)seq * p.max_blocks;
+        const int tiles_per_round = 32 / pages, kv_g = g / f.kv_share, kv_heads = p.G / f.kv_share;
+        bool waited = !f.settled, ok = true;
+        for (int kt0 = kt_lo; kt0 < kt_hi && ok; kt0 += tiles_per_round) {
+            const int key0 = kt0 * ABN + lane * bs, blk = key0 / bs;
+            const bool wanted = lane < tiles_per_round * pages && kt0 + lane / pages < kt_hi && key0 <= pos_last && key0 + bs > lo_first;
+            const long long page = wanted && blk < p.max_blocks ? table[blk] : -1;
+            const bool there = page >= 0 && page < p.num_pages;
+            if (wanted && !there) atomicOr(err, HFB_ERR_PAGE);
+            const uint32_t have = __ballot_sync(0xffffffffu, there);
+            const uint8_t *src = p.cache + ((size_t)(there ? page : 0) * kv_heads + kv_g) * p.record;
+            for (int t = 0; t < tiles_per_round && kt0 + t < kt_hi && ok; t++) {
+                const int j = kt0 + t - kt_lo, s = j % STAGES;
+                if (!waited && (kt0 + t) * ABN + ABN - 1 >= pos_first) {
+                    pdl_wait();                               // this tile holds rows that the kernel in front writes
+                    waited = true;
+                }
+                const uint32_t mine = pages == 32 ? have : (have >> (t * pages)) & ((1u << pages) - 1u);
+                if (lane == 0) {
+                    ok = mbar_wait(empty0 + 8 * s, ((j / STAGES) & 1) ^ 1, abort_flag, err);
+                    if (ok) {
+                        page_mask[s] = mine;
+                        mbar_arrive_expect_tx(full0 + 8 * s, __popc(mine) * p.record);
+                    }
+                }
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+                if (ok && there && lane / pages == t)
+                    bulk_load(tiles0 + s * stage_bytes + (lane % pages) * p.record, src, p.record, full0 + 8 * s);
+            }
+        }
+    } else {
+        // ---- the computing warps --------------------------------------------------------------------------------------------
+        if (f.settled) pdl_wait();                            // the queries come from the kernel in front
+        pdl_trigger();
+        const float log2e = 1.4426950408889634f;
+        uint32_t qf[CH][NT][2];
+        float fac[NT][2], slope[NT][2];
+        int pos[NT][2];
+        const bool capped = p.softcap > 0.f;
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            // this lane's share of column 8 n + lane / 4: numbers 16 c + 4 (lane % 4) + 0..3
+            const int col = 8 * n + row8, tl = col / r, hl = col % r;
+            const bool valid = tl < nt;
+            const __nv_bfloat16 *src = (const __nv_bfloat16 *)p.q + ((size_t)(t0 + (valid ? tl : 0)) * p.H + g * r + (valid ? hl : 0)) * D + 4 * c4;
+            uint2 raw[CH];
+            unsigned top = 0;
+#pragma unroll
+            for (int c = 0; c < CH; c++) {
+                raw[c] = valid ? *(const uint2 *)(src + 16 * c) : make_uint2(0, 0);
+                top = max(top, max(max(raw[c].x & 0x7fffu, (raw[c].x >> 16) & 0x7fffu), max(raw[c].y & 0x7fffu, (raw[c].y >> 16) & 0x7fffu)));
+            }
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const unsigned field = min(268u - (top >> 7), 253u);                  // exponent field of the power of two
+            const float up = __uint_as_float(field << 23), down = __uint_as_float((254u - field) << 23);
+#pragma unroll
+            for (int c = 0; c < CH; c++) {
+                qf[c][n][0] = pack_f16(__uint_as_float(raw[c].x << 16) * up, __uint_as_float(raw[c].x & 0xffff0000u) * up);
+                qf[c][n][1] = pack_f16(__uint_as_float(raw[c].y << 16) * up, __uint_as_float(raw[c].y & 0xffff0000u) * up);
+            }
+            const float hs = p.head_scales && valid ? p.head_scales[g * r + hl] : 1.f;
+            const float own = (capped ? p.scale * hs / p.softcap : p.scale * hs * log2e) * down;
+            const float sl = p.slopes && valid ? p.slopes[g * r + hl] * log2e : 0.f;
+            const int ps = valid ? p.positions[t0 + tl] : -1;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {                     // ... and of the columns whose scores it will hold
+                fac[n][i] = __shfl_sync(0xffffffffu, own, 4 * (2 * c4 + i));
+                slope[n][i] = __shfl_sync(0xffffffffu, sl, 4 * (2 * c4 + i));
+                pos[n][i] = __shfl_sync(0xffffffffu, ps, 4 * (2 * c4 + i));
+            }
+        }
+        const float cap2 = p.softcap * log2e;
+        const int kbase = warp * 16;
+        // ldmatrix: lanes 0..7 and 8..15 name the rows of the warp's two eights of keys, the upper lanes the same rows one piece further
+        const int kk = kbase + (lane & 7) + ((lane >> 3) & 1) * 8;
+        const uint32_t row_at = (uint32_t)(kk / bs) * p.record + (uint32_t)(kk % bs) * D;
+        const int turn = D == 128 ? lane & 7 : (lane & 7) >> 1;
+        uint32_t piece[CH / 2];
+#pragma unroll
+        for (int c = 0; c < CH / 2; c++) piece[c] = row_at + (uint32_t)((2 * c + (lane >> 4)) ^ turn) * 16u;
+        // the scales of the two keys whose scores this lane holds
+        const int k0 = kbase + row8, k1 = k0 + 8;
+        const uint32_t s_at0 = (uint32_t)(k0 / bs) * p.record + 2u * bs * D + 4u * (k0 % bs);
+        const uint32_t s_at1 = (uint32_t)(k1 / bs) * p.record + 2u * bs * D + 4u * (k1 % bs);
+        const uint32_t v_codes = (uint32_t)bs * D, v_scales = 4u * bs;
+        float rv = 0.f;                                       // 1 / vm
+
+        for (int kt = kt_lo; kt < kt_hi; kt++) {
+            const int j = kt - kt_lo, s = j % STAGES;
+            if (!mbar_wait(full0 + 8 * s, (j / STAGES) & 1, abort_flag, err)) break;
+            const uint32_t st = tiles0 + s * stage_bytes;
+            const uint8_t *sg = gen + 128 + s * stage_bytes;
+            const uint32_t mask = page_mask[s];
+            float sc[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; n++) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+#pragma unroll
+            for (int c = 0; c < CH / 2; c++) {
+                uint32_t w0, w1, w2, w3;
+                ldsm_x4(st + piece[c], w0, w1, w2, w3);
+                const uint32_t a0 = codes_f16(w0, 0x4140), a1 = codes_f16(w1, 0x4140), a2 = codes_f16(w0, 0x4342), a3 = codes_f16(w1, 0x4342);
+                const uint32_t b0 = codes_f16(w2, 0x4140), b1 = codes_f16(w3, 0x4140), b2 = codes_f16(w2, 0x4342), b3 = codes_f16(w3, 0x4342);
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    mma_f16(sc[n], a0, a1, a2, a3, qf[2 * c][n][0], qf[2 * c][n][1]);
+                    mma_f16(sc[n], b0, b1, b2, b3, qf[2 * c + 1][n][0], qf[2 * c + 1][n][1]);
+                }
+            }
+            // a tile wholly inside every row's range, with all of its pages, needs no mask
+            const int key0 = kt * ABN + k0, key1 = kt * ABN + k1;
+            const bool edge = kt * ABN + ABN - 1 > pos_first || kt * ABN < lo_last || mask != (1u << pages) - 1u;
+            float ks0 = *(const float *)(sg + s_at0), ks1 = *(const float *)(sg + s_at1);
+            float vs0 = *(const float *)(sg + s_at0 + v_scales), vs1 = *(const float *)(sg + s_at1 + v_scales);
+            bool in0 = true, in1 = true;
+            if (edge) {
+                // (rows behind the request's last and missing pages hold anything)
+                in0 = key0 <= pos_last && (mask >> (k0 / bs) & 1u);
+                in1 = key1 <= pos_last && (mask >> (k1 / bs) & 1u);
+                if (!in0) ks0 = vs0 = 0.f;
+                if (!in1) ks1 = vs1 = 0.f;
+            }
+            if (__any_sync(0xffffffffu, fmaxf(vs0, vs1) > vm)) {
+                float v = fmaxf(vm, fmaxf(vs0, vs1));
+                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+                const float shrink = vm / v;
+#pragma unroll
+                for (int c = 0; c < CH; c++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++) { o[c][n][0] *= shrink; o[c][n][1] *= shrink; o[c][n][2] *= shrink; o[c][n][3] *= shrink; }
+                vm = v;
+                rv = 1.0f / v;
+            }
+            const float vn0 = vs0 * rv * 32768.f, vn1 = vs1 * rv * 32768.f;
+            bool grew = false;
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int i = e & 1;
+                    float x = sc[n][e] * (e < 2 ? ks0 : ks1) * fac[n][i];
+                    if (capped) x = cap2 * tanh_fast(x);
+                    const int key = e < 2 ? key0 : key1;
+                    if (p.slopes) x = fmaf(slope[n][i], (float)(key - pos[n][i]), x);
+                    if (edge) x = (e < 2 ? in0 : in1) && key <= pos[n][i] && key >= mask_lo(pos[n][i], p.window) ? x : -INFINITY;
+                    sc[n][e] = x;
+                    grew |= x > m[n][i];
+                }
+            if (__any_sync(0xffffffffu, grew)) {
+                // a maximum grew somewhere in the warp: rescale what has been summed so far
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        float v = fmaxf(m[n][i], fmaxf(sc[n][i], sc[n][2 + i]));
+                        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+                        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+                        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+                        const float corr = fast_exp2(m[n][i] - (v == -INFINITY ? 0.f : v));
+                        l[n][i] *= corr;
+#pragma unroll
+                        for (int c = 0; c < CH; c++) { o[c][n][i] *= corr; o[c][n][2 + i] *= corr; }
+                        m[n][i] = v;
+                    }
+            }
+            uint32_t pf[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                float w[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int i = e & 1;
+                    const float q = fast_exp2(sc[n][e] - (m[n][i] == -INFINITY ? 0.f : m[n][i]));
+                    l[n][i] += q;
+                    w[e] = q * (e < 2 ? vn0 : vn1);
+                    if (edge && sc[n][e] == -INFINITY) w[e] = 0.f;       // (a value that is no number, for a row that does not see it)
+                }
+                pf[n][0] = transpose8(pack_f16(w[0], w[1]));
+                pf[n][1] = transpose8(pack_f16(w[2], w[3]));
+            }
+#pragma unroll
+            for (int c = 0; c < CH / 2; c++) {
+                uint32_t w0, w1, w2, w3;
+                ldsm_x4_t(st + piece[c] + v_codes, w0, w1, w2, w3);
+                const uint32_t a0 = codes_f16(w0, 0x4240), a1 = codes_f16(w0, 0x4341), a2 = codes_f16(w1, 0x4240), a3 = codes_f16(w1, 0x4341);
+                const uint32_t b0 = codes_f16(w2, 0x4240), b1 = codes_f16(w2, 0x4341), b2 = codes_f16(w3, 0x4240), b3 = codes_f16(w3, 0x4341);
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    mma_f16(o[2 * c][n], a0, a1, a2, a3, pf[n][0], pf[n][1]);
+                    mma_f16(o[2 * c + 1][n], b0, b1, b2, b3, pf[n][0], pf[n][1]);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty0 + 8 * s);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], 4);
+                l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], 8);
+                l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], 16);
+            }
+    }
+
+    // ---- merge the four warps (they saw disjoint keys) in warp order ------------------------------------------------------------
+    __syncthreads();                                          // every tile has been used: its buffers are free
+    if (*abort_flag != 0) {
+        // a wait ran out: give copies that are still in flight time to land before the shared memory goes away
+        if (threadIdx.x == 0)
+            for (int i = 0; i < 2000; i++) __nanosleep(1000);
+        __syncthreads();
+        return;
+    }
+    constexpr int OROW = D + 4;                               // (rows of the buffer in different banks)
+    float *mo = (float *)(gen + 128);                         // [4][COLS][OROW]
+    float *ml = mo + 4 * COLS * OROW;                         // [4][COLS][2]
+    float *mv = ml + 4 * COLS * 2;                            // [4]
+    if (warp < 4) {
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int col = 8 * n + 2 * c4 + i;
+#pragma unroll
+                for (int c = 0; c < CH; c++)
+                    *(float2 *)(mo + (warp * COLS + col) * OROW + 16 * c + 2 * row8) = make_float2(o[c][n][i], o[c][n][2 + i]);
+                if (row8 == 0) *(float2 *)(ml + (warp * COLS + col) * 2) = make_float2(m[n][i], l[n][i]);
+            }
+        if (lane == 0) mv[warp] = vm;
+    }
+    __syncthreads();
+    const int rows = nt * r;
+    float top_v = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; w++) top_v = fmaxf(top_v, mv[w]);
+    for (int idx = threadIdx.x; idx < rows * (D / 4); idx += KF_THREADS) {
+        const int row = idx / (D / 4), q4 = idx % (D / 4);
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < 4; w++) top = fmaxf(top, ml[(w * COLS + row) * 2]);
+        float denom = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < 4; w++) {                         // in warp order
+            const float mw = ml[(w * COLS + row) * 2];
+            const float e = mw == -INFINITY ? 0.f : fast_exp2(mw - top);
+            denom += ml[(w * COLS + row) * 2 + 1] * (mw == -INFINITY ? 1.f : e);       // (zero, or no number)
+            const float fo = mv[w] == 0.f ? 0.f : e * (mv[w] / top_v);
+            const float4 v = *(const float4 *)(mo + (w * COLS + row) * OROW + 4 * q4);
+            acc.x += v.x * fo; acc.y += v.y * fo; acc.z += v.z * fo; acc.w += v.w * fo;
+        }
+        const float unit = top_v * (1.f / 32768.f);
+        acc.x *= unit; acc.y *= unit; acc.z *= unit; acc.w *= unit;
+        const int tok = t0 + row / r, head = g * r + row % r;
+        const size_t th = (size_t)tok * p.H + head;
+        if ((p.sinks || p.zero_sink) && split == 0) {
+            // the sink joins the first range's sum as one more score; the merge of the ranges carries it like any other
+            const float sk = p.sinks ? p.sinks[head] * 1.4426950408889634f : 0.f;
+            const float t = fmaxf(top, sk);
+            const float e = top == -INFINITY ? 0.f : exp2f(top - t);
+            denom = denom * e + exp2f(sk - t);
+            acc.x *= e; acc.y *= e; acc.z *= e; acc.w *= e;
+            top = t;
+        }
+        if (used > 1) {
+            *(float4 *)(f.part_o + (th * f.splits + split) * D + 4 * q4) = acc;
+            if (q4 == 0) *(float2 *)(f.part_ml + (th * f.splits + split) * 2) = make_float2(top, denom);
+        } else {
+            const float inv = denom == 0.f ? 0.f : 1.0f / denom;
+            *(uint2 *)((__nv_bfloat16 *)p.out + th * D + 4 * q4) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+        }
+    }
+    if (used == 1) return;
+
+    // ---- merge the ranges: whoever stored its range last, in the order of the ranges ------------------------------------------
+    volatile int *last_flag = abort_flag + 1;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        __threadfence();                                      // (after the barrier: it covers every thread's stores)
+        int *cnt = f.counters + (size_t)tile * p.G + g;
+        const int last = atomicAdd(cnt, 1) == used - 1;
+        if (last) *cnt = 0;
+        *last_flag = last;
+    }
+    __syncthreads();
+    if (!*last_flag) return;
+    __threadfence();
+    for (int idx = threadIdx.x; idx < rows * (D / 4); idx += KF_THREADS) {
+        const int row = idx / (D / 4), q4 = idx % (D / 4);
+        const size_t th = (size_t)(t0 + row / r) * p.H + g * r + row % r;
+        const float2 *src_ml = (const float2 *)(f.part_ml + th * f.splits * 2);
+        const float4 *src = (const float4 *)(f.part_o + th * f.splits * D) + q4;
+        float top = -INFINITY, denom = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c = 0; c < used; c += 8) {                   // eight reads in flight
+            float2 w[8];
+            float4 v[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                w[i] = c + i < used ? __ldcg(src_ml + c + i) : make_float2(-INFINITY, 0.f);
+                v[i] = c + i < used ? __ldcg(src + (size_t)(c + i) * (D / 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            float t = top;
+#pragma unroll
+            for (int i = 0; i < 8; i++) t = fmaxf(t, w[i].x);
+            const float e = top == -INFINITY ? 0.f : exp2f(top - t);
+            if (top != -INFINITY) { denom *= e; acc.x *= e; acc.y *= e; acc.z *= e; acc.w *= e; }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float x = w[i].x == -INFINITY ? 0.f : exp2f(w[i].x - t);
+                denom += w[i].y * (w[i].x == -INFINITY ? 1.f : x);
+                acc.x += v[i].x * x; acc.y += v[i].y * x; acc.z += v[i].z * x; acc.w += v[i].w * x;
+            }
+            top = t;
+        }
+        const float inv = denom == 0.f ? 0.f : 1.0f / denom;
+        *(uint2 *)((__nv_bfloat16 *)p.out + th * D + 4 * q4) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+    }
+}
+
+template <int D, int NT, int STAGES>
+static int launch_kv8_few(const Kv8FewParams &f, int n_tiles, cudaStream_t st)
+{
+    const int tiles = STAGES * (ABN / f.a.block_size) * f.a.record;
+    constexpr int merge = (4 * 8 * NT * (D + 4) + 4 * 8 * NT * 2 + 4) * 4;
+    const int smem = 256 + (tiles > merge ? tiles : merge);
+    static bool configured[64] = {false};                     // (the opt-in is a property of the function on one device)
+    if (!configured[current_device()]) {
+        cudaError_t e = cudaFuncSetAttribute(kv8_few_kernel<D, NT, STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, 256 + STAGES * ABN * (2 * D + 16));
+        if (e != cudaSuccess) return fail(HFB_ECUDA, "kv8_attention_few: cannot opt in to shared memory: %s", cudaGetErrorString(e));
+        configured[current_device()] = true;
+    }
+    g_launch_err = launch_pdl(kv8_few_kernel<D, NT, STAGES>, dim3(n_tiles, f.a.G, f.splits), dim3(KF_THREADS), smem, st, f, error_word());
+    return check_pdl_launch(g_launch_err, "kv8_attention_few");
+}
+
+}  // namespace hfb
+
+using namespace hfb;
+
+extern "C" size_t hfb_kv8_attention_few_scratch(int T, int H, int d, int splits)
+{
+    return splits > 1 ? (size_t)T * H * splits * (d + 2) * sizeof(float) : 0;
+}
+
+extern "C" int hfb_kv8_attention_few(const void *q, const void *cache, const int32_t *block_table, int max_blocks, const int32_t *positions,
+                                     const int32_t *tile_seq, const int32_t *tile_t0, const int32_t *tile_nt, int n_tiles, int tile_tokens,
+                                     int splits, int min_tiles, int settled, int block_size, int64_t num_pages, int window, float scale, void *out,
+                                     void *scratch, size_t scratch_bytes, int *counters, int counters_len, int T, int H, int G, int d,
+                                     const float *sinks, int zero_sink, const float *slopes, const float *head_scales, float softcap, hfb_stream s)
+{
+    if (n_tiles <= 0) return HFB_OK;
+    if (d != 64 && d != 128) return fail(HFB_ENOTSUP, "kv8_attention_few: head size %d (64 and 128 only)", d);
+    if (H <= 0 || G <= 0 || H % G || max_blocks <= 0 || num_pages < 0 || tile_tokens < 1)
+        return fail(HFB_EINVAL, "kv8_attention_few: bad arguments (H=%d G=%d)", H, G);
+    if (block_size < 8 || block_size > ABN || ABN % block_size) return fail(HFB_ENOTSUP, "kv8_attention_few: pages of %d tokens (8, 16, 32 and 64)", block_size);
+    // more heads on a key/value head than a tile has columns: as several groups that read the same keys and values
+    int share = 1;
+    while (H / G > 16 * share || (H / G) % share) share++;
+    const int groups = G * share, cols = tile_tokens * (H / groups);
+    if (cols > 16 || (tile_tokens > 1 && share > 1)) return fail(HFB_EINVAL, "kv8_attention_few: tiles of %d tokens of %d heads", tile_tokens, H / groups);
+    if (groups > 65535 || splits < 1 || splits > KF_MAX_SPLITS || min_tiles < 1) return fail(HFB_EINVAL, "kv8_attention_few: bad split or group count");
+    if (((uintptr_t)q & 7) || ((uintptr_t)out & 7) || ((uintptr_t)cache & 15) || ((uintptr_t)scratch & 15))
+        return fail(HFB_EINVAL, "kv8_attention_few: misaligned arrays");
+    if (splits > 1 && (!scratch || scratch_bytes < hfb_kv8_attention_few_scratch(T, H, d, splits) || !counters || (long long)counters_len < (long long)n_tiles * groups))
+        return fail(HFB_EINVAL, "kv8_attention_few: %d ranges need scratch and counters", splits);
+    Kv8FewParams f = {};
+    f.a.q = q; f.a.cache = (const uint8_t *)cache; f.a.out = out; f.a.block_table = block_table; f.a.positions = positions;
+    f.a.tile_seq = tile_seq; f.a.tile_t0 = tile_t0; f.a.tile_nt = tile_nt; f.a.max_blocks = max_blocks; f.a.block_size = block_size;
+    f.a.record = kv8_record_bytes(block_size, d); f.a.window = window; f.a.H = H; f.a.G = groups; f.a.num_pages = num_pages; f.a.scale = scale;
+    f.a.sinks = sinks; f.a.slopes = slopes; f.a.head_scales = head_scales; f.a.zero_sink = zero_sink; f.a.softcap = softcap > 0.f ? softcap : 0.f;
+    f.part_o = (float *)scratch; f.part_ml = splits > 1 ? (float *)scratch + (size_t)T * H * splits * d : nullptr;
+    f.counters = counters; f.splits = splits; f.per = min_tiles; f.kv_share = share; f.settled = settled;
+    cudaStream_t st = (cudaStream_t)s;
+    if (d == 128) return cols <= 8 ? launch_kv8_few<128, 1, 3>(f, n_tiles, st) : launch_kv8_few<128, 2, 3>(f, n_tiles, st);
+    return cols <= 8 ? launch_kv8_few<64, 1, 4>(f, n_tiles, st) : launch_kv8_few<64, 2, 4>(f, n_tiles, st);
+}

@@ -397,9 +397,25 @@ def kv8_read(cache, pages, rows, k_out, v_out) -> None:
     backend().kv8_read(cache, pages, rows, k_out, v_out)
 
 
+def kv8_head_groups(heads_per_group: int) -> int:
+    """Into how many groups the heads on one key/value head are cut for the tiles of few queries, which have 16 places."""
+    return next(s for s in range(1, heads_per_group + 1) if heads_per_group <= 16 * s and heads_per_group % s == 0)
+
+
 def kv8_step_arrays(q_lens, heads_per_group: int):
-    """Tile lists of a step's tokens for :func:`paged_attention_kv8`, as named int32 arrays."""
-    return {}
+    """Tile lists of a step's tokens for :func:`paged_attention_kv8`, as named int32 arrays: a tile is up to ``few.nt`` consecutive tokens of
+    request ``few.seq`` from token ``few.t0`` of the step on, with their heads at most 16 places."""
+    import numpy as np
+    q = np.asarray(q_lens, dtype=np.int32)
+    share = kv8_head_groups(heads_per_group)
+    per = 1 if share > 1 else max(1, 16 // heads_per_group)
+    if int(q.max()) == 1:
+        return {"few.seq": np.arange(len(q), dtype=np.int32), "few.t0": np.arange(len(q), dtype=np.int32), "few.nt": np.ones(len(q), dtype=np.int32)}
+    tiles = -(-q // per)
+    seq = np.repeat(np.arange(len(q), dtype=np.int32), tiles)
+    number = np.arange(len(seq), dtype=np.int32) - np.repeat(np.cumsum(tiles) - tiles, tiles).astype(np.int32)
+    first = (np.cumsum(q) - q).astype(np.int32)
+    return {"few.seq": seq, "few.t0": first[seq] + number * per, "few.nt": np.minimum(per, q[seq] - number * per).astype(np.int32)}
 
 
 def paged_attention_kv8(q, cache, meta, ctx, H, G, d, window, scale, out, tiles=None, settled: bool = False, sinks=None, zero_sink=False,

@@ -115,6 +115,7 @@ class NativeBackend:
         self.lib.hfb_last_error.restype = ctypes.c_char_p
         self.lib.hfb_linear_tc_workspace.restype = ctypes.c_size_t
         self.lib.hfb_attention_fast_scratch.restype = ctypes.c_size_t
+        self.lib.hfb_kv8_attention_few_scratch.restype = ctypes.c_size_t
         # "fast": tiled tensor-core attention where the sizes allow; "plain": one block per (token, head) always
         self.attention = os.environ.get("HFB_ATTENTION", "fast")
         self.attention_tc = os.environ.get("HFB_ATTN_TC", "1") != "0"     # tcgen05 attention for prompt portions
@@ -143,6 +144,8 @@ class NativeBackend:
         if self.lib.hfb_decay_chunk_tokens() != DECAY_CHUNK:
             raise KernelError("the library's chunks and the binding's are not of one length")
         self.decay_chunks = os.environ.get("HFB_DECAY_CHUNKS", "1") != "0"     # portions of a recurrence with scalar decays in chunks
+        self._kv8_counters = {}
+        self.kv8_ctas_per_sm, self.kv8_most_tiles = 6, 16
         self.path = path
         self.launches = 0          # kernels launched through this binding (one per successful call)
 
@@ -412,10 +415,56 @@ class NativeBackend:
         self._here(q, cache, meta.block_table, ctx.token_seq, ctx.positions, out, sinks, slopes, head_scales)
         self._on_gpu(q, cache, meta.block_table, ctx.token_seq, ctx.positions, out, sinks, slopes, head_scales)
         opt_args = (_p(sinks), c_int(1 if zero_sink else 0), _p(slopes), _p(head_scales), c_float(softcap))
+        if (self.attention == "fast" and "few.seq" in tiles and q.dtype == torch.bfloat16 and d in (64, 128) and meta.block_size in (8, 16, 32, 64)):
+            self._kv8_few(q, cache, meta, ctx, H, G, d, window, scale, out, tiles, settled, opt_args)
+            return
         self._check(self.lib.hfb_kv8_attention_plain(
             _p(q), _p(cache), c_int(_dt(q)), _p(meta.block_table), c_int(meta.max_blocks), _p(ctx.token_seq), _p(ctx.positions),
             c_int(meta.block_size), c_int64(cache.shape[0]), c_int(window), c_float(scale), _p(out), c_int(q.shape[0]), c_int(H), c_int(G),
             c_int(d), *opt_args, self._stream()), "kv8_attention_plain")
+
+    def _kv8_zeros(self, device, n):
+        """``n`` counters that are zero and that no launch uses which may run beside the one they are for: one set a stream, and for
+        a launch that is being captured a set of its own, since its graph may be replayed beside anything."""
+        if torch.cuda.is_current_stream_capturing():
+            pool = self._kv8_counters.get(device)
+            if pool is None or pool[1] + n > pool[0].numel():
+                return torch.zeros(n, dtype=torch.int32, device=device)       # (a part of the graph then)
+            pool[1] += n
+            return pool[0][pool[1] - n:pool[1]]
+        if device not in self._kv8_counters:
+            self._kv8_counters[device] = [torch.zeros(1 << 20, dtype=torch.int32, device=device), 0]
+        key = device, _raw_stream(device.index)
+        have = self._kv8_counters.get(key)
+        if have is None or have.numel() < n:
+            have = self._kv8_counters[key] = torch.zeros(max(n, 4096), dtype=torch.int32, device=device)
+        return have
+
+    def _kv8_few(self, q, cache, meta, ctx, H, G, d, window, scale, out, tiles, settled, opt_args):
+        from . import decode_split_hint, kv8_head_groups
+        seq, t0, nt = tiles["few.seq"], tiles["few.t0"], tiles["few.nt"]
+        r, n_tiles, T = H // G, seq.shape[0], q.shape[0]
+        share = kv8_head_groups(r)
+        tile_tokens = 1 if share > 1 or ctx.max_q_len == 1 else max(1, 16 // r)
+        # The most tiles of 64 keys a request may have when this launch runs: a captured one is replayed while the requests grow within
+        # the range that the split hint stands for.
+        longest = max(1, (ctx.max_kv_len + 63) // 64)
+        if torch.cuda.is_current_stream_capturing():
+            hint = getattr(ctx, "decode_split_hint", None) or decode_split_hint(ctx.max_kv_len)
+            longest = max(longest, {1: 6, 4: 7, 8: 15, 16: 63, 32: 127}.get(hint, 512))
+        if window:
+            longest = min(longest, abs(window) // 64 + 2)
+        ctas = n_tiles * G * share
+        per = max(1, min(self.kv8_most_tiles, ctas * longest // (self.kv8_ctas_per_sm * self.sm_count)))
+        splits = max(1, min(64, -(-longest // per)))
+        need = 0 if splits == 1 else 4 * T * H * splits * (d + 2)
+        scratch = ctx.buf("kv8_scratch", (need,), torch.uint8) if need else None
+        counters = self._kv8_zeros(q.device, ctas) if need else None
+        self._check(self.lib.hfb_kv8_attention_few(
+            _p(q), _p(cache), _p(meta.block_table), c_int(meta.max_blocks), _p(ctx.positions), _p(seq), _p(t0), _p(nt), c_int(n_tiles),
+            c_int(tile_tokens), c_int(splits), c_int(per), c_int(1 if settled else 0), c_int(meta.block_size), c_int64(cache.shape[0]),
+            c_int(window), c_float(scale), _p(out), _p(scratch), ctypes.c_size_t(need), _p(counters),
+            c_int(counters.numel() if need else 0), c_int(T), c_int(H), c_int(G), c_int(d), *opt_args, self._stream()), "kv8_attention_few")
 
     def swiglu(self, gu, out, interleaved):
         self._on_gpu(gu, out)
