@@ -2,7 +2,7 @@
 //
 // What bounds it is reading the cache: d + 4 bytes a key, and as many a value.  A fifth warp keeps the copies going, one bulk copy per page
 // and head (codes and scales of keys and values are one record), several tiles of 64 keys ahead of the four warps that compute,
-// 16 keys of each tile a warp.
+// two of them a tile.
 //
 // Between the copy and the tensor core every byte has to become a 16-bit number, so that is what the layout serves:
 // * A code is a whole number below 2^11, which float16 holds as it is: 0x6400 | byte is 1024 + byte, minus 1152 gives the code; a
@@ -73,12 +73,14 @@ __device__ __forceinline__ void mma_f16(float *c, uint32_t a0, uint32_t a1, uint
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// D: head size; NT: columns (token, head) of a tile in eights; STAGES: tiles of 64 keys in flight
-template <int D, int NT, int STAGES>
-__global__ void __launch_bounds__(KF_THREADS)
+// D: head size; NT: columns (token, head) of a tile in eights; STAGES: tiles of 64 keys in flight; OPTS: a cap or slopes
+template <int D, int NT, int STAGES, bool OPTS>
+__global__ void __launch_bounds__(KF_THREADS, D == 128 ? (NT == 1 ? 3 : 2) : (NT == 1 ? 4 : 3))
 kv8_few_kernel(Kv8FewParams f, int *err)
 {
     const Kv8Params &p = f.a;
+    // (a stage belongs to one of the two pairs of warps: one that took turns on it could find the phase before its own complete)
+    static_assert(STAGES % 2 == 0, "the pairs of warps have stages of their own");
     constexpr int COLS = 8 * NT, CH = D / 16;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 127u) & ~127u;
@@ -92,7 +94,7 @@ kv8_few_kernel(Kv8FewParams f, int *err)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (!f.settled) pdl_wait();                               // nothing is read that the kernels in front may still write
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; s++) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 4); }
+        for (int s = 0; s < STAGES; s++) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 2); }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -159,7 +161,7 @@ kv8_few_kernel(Kv8FewParams f, int *err)
         const float log2e = 1.4426950408889634f;
         uint32_t qf[CH][NT][2];
         float fac[NT][2], slope[NT][2];
-        int pos[NT][2];
+        int pos[NT][2], lo[NT][2];
         const bool capped = p.softcap > 0.f;
 #pragma unroll
         for (int n = 0; n < NT; n++) {
@@ -192,60 +194,80 @@ kv8_few_kernel(Kv8FewParams f, int *err)
                 fac[n][i] = __shfl_sync(0xffffffffu, own, 4 * (2 * c4 + i));
                 slope[n][i] = __shfl_sync(0xffffffffu, sl, 4 * (2 * c4 + i));
                 pos[n][i] = __shfl_sync(0xffffffffu, ps, 4 * (2 * c4 + i));
+                lo[n][i] = mask_lo(pos[n][i], p.window);
             }
         }
         const float cap2 = p.softcap * log2e;
-        const int kbase = warp * 16;
-        // ldmatrix: lanes 0..7 and 8..15 name the rows of the warp's two eights of keys, the upper lanes the same rows one piece further
-        const int kk = kbase + (lane & 7) + ((lane >> 3) & 1) * 8;
-        const uint32_t row_at = (uint32_t)(kk / bs) * p.record + (uint32_t)(kk % bs) * D;
+        // warps 0 and 1 take every other tile, 32 keys each, warps 2 and 3 the others
+        const int kbase = (warp & 1) * 32;
+        // ldmatrix: lanes 0..7 and 8..15 name the rows of two eights of keys, the upper lanes the same rows one piece further; this lane
+        // holds the scores of the keys `row8` and `row8 + 8` of each sixteen
         const int turn = D == 128 ? lane & 7 : (lane & 7) >> 1;
+        uint32_t row_at[2], s_at[2][2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int kk = kbase + 16 * h + (lane & 7) + ((lane >> 3) & 1) * 8;
+            row_at[h] = (uint32_t)(kk / bs) * p.record + (uint32_t)(kk % bs) * D;
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int k = kbase + 16 * h + 8 * u + row8;
+                s_at[h][u] = (uint32_t)(k / bs) * p.record + 2u * bs * D + 4u * (k % bs);
+            }
+        }
         uint32_t piece[CH / 2];
 #pragma unroll
-        for (int c = 0; c < CH / 2; c++) piece[c] = row_at + (uint32_t)((2 * c + (lane >> 4)) ^ turn) * 16u;
-        // the scales of the two keys whose scores this lane holds
-        const int k0 = kbase + row8, k1 = k0 + 8;
-        const uint32_t s_at0 = (uint32_t)(k0 / bs) * p.record + 2u * bs * D + 4u * (k0 % bs);
-        const uint32_t s_at1 = (uint32_t)(k1 / bs) * p.record + 2u * bs * D + 4u * (k1 % bs);
+        for (int c = 0; c < CH / 2; c++) piece[c] = (uint32_t)((2 * c + (lane >> 4)) ^ turn) * 16u;
         const uint32_t v_codes = (uint32_t)bs * D, v_scales = 4u * bs;
+        const uint32_t all_pages = (1u << pages) - 1u;
         float rv = 0.f;                                       // 1 / vm
 
-        for (int kt = kt_lo; kt < kt_hi; kt++) {
-            const int j = kt - kt_lo, s = j % STAGES;
-            if (!mbar_wait(full0 + 8 * s, (j / STAGES) & 1, abort_flag, err)) break;
+        int s = (warp >> 1) % STAGES, phase = 0;
+        for (int kt = kt_lo + (warp >> 1); kt < kt_hi; kt += 2) {
+            if (!mbar_wait(full0 + 8 * s, phase, abort_flag, err)) break;
             const uint32_t st = tiles0 + s * stage_bytes;
             const uint8_t *sg = gen + 128 + s * stage_bytes;
             const uint32_t mask = page_mask[s];
-            float sc[NT][4];
+            float sc[2][NT][4];
 #pragma unroll
-            for (int n = 0; n < NT; n++) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+            for (int h = 0; h < 2; h++) {
 #pragma unroll
-            for (int c = 0; c < CH / 2; c++) {
-                uint32_t w0, w1, w2, w3;
-                ldsm_x4(st + piece[c], w0, w1, w2, w3);
-                const uint32_t a0 = codes_f16(w0, 0x4140), a1 = codes_f16(w1, 0x4140), a2 = codes_f16(w0, 0x4342), a3 = codes_f16(w1, 0x4342);
-                const uint32_t b0 = codes_f16(w2, 0x4140), b1 = codes_f16(w3, 0x4140), b2 = codes_f16(w2, 0x4342), b3 = codes_f16(w3, 0x4342);
+                for (int n = 0; n < NT; n++) sc[h][n][0] = sc[h][n][1] = sc[h][n][2] = sc[h][n][3] = 0.f;
 #pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    mma_f16(sc[n], a0, a1, a2, a3, qf[2 * c][n][0], qf[2 * c][n][1]);
-                    mma_f16(sc[n], b0, b1, b2, b3, qf[2 * c + 1][n][0], qf[2 * c + 1][n][1]);
+                for (int c = 0; c < CH / 2; c++) {
+                    uint32_t w0, w1, w2, w3;
+                    ldsm_x4(st + row_at[h] + piece[c], w0, w1, w2, w3);
+                    const uint32_t a0 = codes_f16(w0, 0x4140), a1 = codes_f16(w1, 0x4140), a2 = codes_f16(w0, 0x4342), a3 = codes_f16(w1, 0x4342);
+                    const uint32_t b0 = codes_f16(w2, 0x4140), b1 = codes_f16(w3, 0x4140), b2 = codes_f16(w2, 0x4342), b3 = codes_f16(w3, 0x4342);
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        mma_f16(sc[h][n], a0, a1, a2, a3, qf[2 * c][n][0], qf[2 * c][n][1]);
+                        mma_f16(sc[h][n], b0, b1, b2, b3, qf[2 * c + 1][n][0], qf[2 * c + 1][n][1]);
+                    }
                 }
             }
+            float ks[2][2], vs[2][2];
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    ks[h][u] = *(const float *)(sg + s_at[h][u]);
+                    vs[h][u] = *(const float *)(sg + s_at[h][u] + v_scales);
+                }
             // a tile wholly inside every row's range, with all of its pages, needs no mask
-            const int key0 = kt * ABN + k0, key1 = kt * ABN + k1;
-            const bool edge = kt * ABN + ABN - 1 > pos_first || kt * ABN < lo_last || mask != (1u << pages) - 1u;
-            float ks0 = *(const float *)(sg + s_at0), ks1 = *(const float *)(sg + s_at1);
-            float vs0 = *(const float *)(sg + s_at0 + v_scales), vs1 = *(const float *)(sg + s_at1 + v_scales);
-            bool in0 = true, in1 = true;
+            const bool edge = kt * ABN + ABN - 1 > pos_first || kt * ABN < lo_last || mask != all_pages;
             if (edge) {
                 // (rows behind the request's last and missing pages hold anything)
-                in0 = key0 <= pos_last && (mask >> (k0 / bs) & 1u);
-                in1 = key1 <= pos_last && (mask >> (k1 / bs) & 1u);
-                if (!in0) ks0 = vs0 = 0.f;
-                if (!in1) ks1 = vs1 = 0.f;
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        const int k = kbase + 16 * h + 8 * u + row8;
+                        if (kt * ABN + k > pos_last || !(mask >> (k / bs) & 1u)) ks[h][u] = vs[h][u] = 0.f;
+                    }
             }
-            if (__any_sync(0xffffffffu, fmaxf(vs0, vs1) > vm)) {
-                float v = fmaxf(vm, fmaxf(vs0, vs1));
+            const float vs_top = fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[1][0], vs[1][1]));
+            if (__any_sync(0xffffffffu, vs_top > vm)) {
+                float v = fmaxf(vm, vs_top);
                 v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
                 v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
                 v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
@@ -257,28 +279,49 @@ kv8_few_kernel(Kv8FewParams f, int *err)
                 vm = v;
                 rv = 1.0f / v;
             }
-            const float vn0 = vs0 * rv * 32768.f, vn1 = vs1 * rv * 32768.f;
             bool grew = false;
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+            for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int i = e & 1;
-                    float x = sc[n][e] * (e < 2 ? ks0 : ks1) * fac[n][i];
-                    if (capped) x = cap2 * tanh_fast(x);
-                    const int key = e < 2 ? key0 : key1;
-                    if (p.slopes) x = fmaf(slope[n][i], (float)(key - pos[n][i]), x);
-                    if (edge) x = (e < 2 ? in0 : in1) && key <= pos[n][i] && key >= mask_lo(pos[n][i], p.window) ? x : -INFINITY;
-                    sc[n][e] = x;
-                    grew |= x > m[n][i];
-                }
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sc[h][n][e] *= ks[h][e >> 1] * fac[n][e & 1];
+            if (OPTS) {
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int key = kt * ABN + kbase + 16 * h + 8 * (e >> 1) + row8;
+                            if (capped) sc[h][n][e] = cap2 * tanh_fast(sc[h][n][e]);
+                            sc[h][n][e] = fmaf(slope[n][e & 1], (float)(key - pos[n][e & 1]), sc[h][n][e]);
+                        }
+            }
+            if (edge) {
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int k = kbase + 16 * h + 8 * (e >> 1) + row8, key = kt * ABN + k;
+                            if (key > pos[n][e & 1] || key < lo[n][e & 1] || !(mask >> (k / bs) & 1u)) sc[h][n][e] = -INFINITY;
+                        }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) grew |= sc[h][n][e] > m[n][e & 1];
             if (__any_sync(0xffffffffu, grew)) {
                 // a maximum grew somewhere in the warp: rescale what has been summed so far
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
-                        float v = fmaxf(m[n][i], fmaxf(sc[n][i], sc[n][2 + i]));
+                        float v = fmaxf(fmaxf(m[n][i], fmaxf(sc[0][n][i], sc[0][n][2 + i])), fmaxf(sc[1][n][i], sc[1][n][2 + i]));
                         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
                         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
                         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
@@ -289,35 +332,41 @@ kv8_few_kernel(Kv8FewParams f, int *err)
                         m[n][i] = v;
                     }
             }
-            uint32_t pf[NT][2];
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
-                float w[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int i = e & 1;
-                    const float q = fast_exp2(sc[n][e] - (m[n][i] == -INFINITY ? 0.f : m[n][i]));
-                    l[n][i] += q;
-                    w[e] = q * (e < 2 ? vn0 : vn1);
-                    if (edge && sc[n][e] == -INFINITY) w[e] = 0.f;       // (a value that is no number, for a row that does not see it)
-                }
-                pf[n][0] = transpose8(pack_f16(w[0], w[1]));
-                pf[n][1] = transpose8(pack_f16(w[2], w[3]));
-            }
-#pragma unroll
-            for (int c = 0; c < CH / 2; c++) {
-                uint32_t w0, w1, w2, w3;
-                ldsm_x4_t(st + piece[c] + v_codes, w0, w1, w2, w3);
-                const uint32_t a0 = codes_f16(w0, 0x4240), a1 = codes_f16(w0, 0x4341), a2 = codes_f16(w1, 0x4240), a3 = codes_f16(w1, 0x4341);
-                const uint32_t b0 = codes_f16(w2, 0x4240), b1 = codes_f16(w2, 0x4341), b2 = codes_f16(w3, 0x4240), b3 = codes_f16(w3, 0x4341);
+            for (int h = 0; h < 2; h++) {
+                const float vn0 = vs[h][0] * rv * 32768.f, vn1 = vs[h][1] * rv * 32768.f;
+                uint32_t pf[NT][2];
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                    mma_f16(o[2 * c][n], a0, a1, a2, a3, pf[n][0], pf[n][1]);
-                    mma_f16(o[2 * c + 1][n], b0, b1, b2, b3, pf[n][0], pf[n][1]);
+                    float w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int i = e & 1;
+                        const float q = fast_exp2(sc[h][n][e] - (m[n][i] == -INFINITY ? 0.f : m[n][i]));
+                        l[n][i] += q;
+                        w[e] = q * (e < 2 ? vn0 : vn1);
+                        if (edge && sc[h][n][e] == -INFINITY) w[e] = 0.f;    // (a value that is no number, for a row that does not see it)
+                    }
+                    pf[n][0] = transpose8(pack_f16(w[0], w[1]));
+                    pf[n][1] = transpose8(pack_f16(w[2], w[3]));
+                }
+#pragma unroll
+                for (int c = 0; c < CH / 2; c++) {
+                    uint32_t w0, w1, w2, w3;
+                    ldsm_x4_t(st + row_at[h] + piece[c] + v_codes, w0, w1, w2, w3);
+                    const uint32_t a0 = codes_f16(w0, 0x4240), a1 = codes_f16(w0, 0x4341), a2 = codes_f16(w1, 0x4240), a3 = codes_f16(w1, 0x4341);
+                    const uint32_t b0 = codes_f16(w2, 0x4240), b1 = codes_f16(w2, 0x4341), b2 = codes_f16(w3, 0x4240), b3 = codes_f16(w3, 0x4341);
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        mma_f16(o[2 * c][n], a0, a1, a2, a3, pf[n][0], pf[n][1]);
+                        mma_f16(o[2 * c + 1][n], b0, b1, b2, b3, pf[n][0], pf[n][1]);
+                    }
                 }
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(empty0 + 8 * s);
+            s += 2;
+            if (s >= STAGES) { s -= STAGES; phase ^= 1; }
         }
 #pragma unroll
         for (int n = 0; n < NT; n++)
@@ -445,20 +494,26 @@ kv8_few_kernel(Kv8FewParams f, int *err)
     }
 }
 
-template <int D, int NT, int STAGES>
-static int launch_kv8_few(const Kv8FewParams &f, int n_tiles, cudaStream_t st)
+template <int D, int NT, int STAGES, bool OPTS>
+static int launch_kv8_few_opts(const Kv8FewParams &f, int n_tiles, cudaStream_t st)
 {
     const int tiles = STAGES * (ABN / f.a.block_size) * f.a.record;
     constexpr int merge = (4 * 8 * NT * (D + 4) + 4 * 8 * NT * 2 + 4) * 4;
     const int smem = 256 + (tiles > merge ? tiles : merge);
     static bool configured[64] = {false};                     // (the opt-in is a property of the function on one device)
     if (!configured[current_device()]) {
-        cudaError_t e = cudaFuncSetAttribute(kv8_few_kernel<D, NT, STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, 256 + STAGES * ABN * (2 * D + 16));
+        cudaError_t e = cudaFuncSetAttribute(kv8_few_kernel<D, NT, STAGES, OPTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 256 + STAGES * ABN * (2 * D + 16));
         if (e != cudaSuccess) return fail(HFB_ECUDA, "kv8_attention_few: cannot opt in to shared memory: %s", cudaGetErrorString(e));
         configured[current_device()] = true;
     }
-    g_launch_err = launch_pdl(kv8_few_kernel<D, NT, STAGES>, dim3(n_tiles, f.a.G, f.splits), dim3(KF_THREADS), smem, st, f, error_word());
+    g_launch_err = launch_pdl(kv8_few_kernel<D, NT, STAGES, OPTS>, dim3(n_tiles, f.a.G, f.splits), dim3(KF_THREADS), smem, st, f, error_word());
     return check_pdl_launch(g_launch_err, "kv8_attention_few");
+}
+
+template <int D, int NT, int STAGES>
+static int launch_kv8_few(const Kv8FewParams &f, int n_tiles, cudaStream_t st)
+{
+    return f.a.slopes || f.a.softcap > 0.f ? launch_kv8_few_opts<D, NT, STAGES, true>(f, n_tiles, st) : launch_kv8_few_opts<D, NT, STAGES, false>(f, n_tiles, st);
 }
 
 }  // namespace hfb
@@ -499,6 +554,6 @@ extern "C" int hfb_kv8_attention_few(const void *q, const void *cache, const int
     f.part_o = (float *)scratch; f.part_ml = splits > 1 ? (float *)scratch + (size_t)T * H * splits * d : nullptr;
     f.counters = counters; f.splits = splits; f.per = min_tiles; f.kv_share = share; f.settled = settled;
     cudaStream_t st = (cudaStream_t)s;
-    if (d == 128) return cols <= 8 ? launch_kv8_few<128, 1, 3>(f, n_tiles, st) : launch_kv8_few<128, 2, 3>(f, n_tiles, st);
+    if (d == 128) return cols <= 8 ? launch_kv8_few<128, 1, 4>(f, n_tiles, st) : launch_kv8_few<128, 2, 4>(f, n_tiles, st);
     return cols <= 8 ? launch_kv8_few<64, 1, 4>(f, n_tiles, st) : launch_kv8_few<64, 2, 4>(f, n_tiles, st);
 }
