@@ -216,16 +216,18 @@ int hfb_kv8_attention_plain(const void *q, const void *cache, int dt, const int3
                             float scale, void *out, int T, int H, int G, int d, const float *sinks, int zero_sink, const float *slopes,
                             const float *head_scales, float softcap, hfb_stream s);
 
-/* ... of few queries, tiled: bfloat16, head sizes 64 and 128, pages of 8, 16, 32 or 64 tokens.  A tile is up to `tile_tokens`
- * consecutive tokens of one request, at most 16 (token, head) pairs of a key/value head (with more than 16 heads on one: single tokens,
- * in groups of heads).  A request's keys are cut into up to `splits` (64 at most) ranges of `min_tiles` tiles of 64 keys or more, which
- * needs hfb_kv8_attention_few_scratch bytes of scratch and n_tiles * groups counters, zero before the launch and after it.
- * `settled`: the rows before the tokens' positions may be read before the kernel in front has finished. */
-size_t hfb_kv8_attention_few_scratch(int T, int H, int d, int splits);
+/* ... of few queries, tiled: bfloat16, head sizes 64 and 128, pages of 8, 16, 32 or 64 tokens, hfb_kv8_attention_few_tiles() tiles at
+ * most.  A tile is up to `tile_tokens` consecutive tokens of one request, at most 16 (token, head) pairs of a key/value head (with
+ * more than 16 heads on one: single tokens, in groups of heads).  The work is cut evenly over `ctas` CTAs, or over fewer so that each
+ * has `min_steps` steps of 64 keys (a tile's start and end reckoned as `tile_cost` steps); that needs hfb_kv8_attention_few_scratch bytes of scratch and n_tiles * groups counters, zero
+ * before the launch and after it.  `settled`: the rows before the tokens' positions may be read before the kernel in front has
+ * finished. */
+size_t hfb_kv8_attention_few_scratch(int ctas, int d);
+int hfb_kv8_attention_few_tiles(void);
 int hfb_kv8_attention_few(const void *q, const void *cache, const int32_t *block_table, int max_blocks, const int32_t *positions,
-                          const int32_t *tile_seq, const int32_t *tile_t0, const int32_t *tile_nt, int n_tiles, int tile_tokens, int splits,
-                          int min_tiles, int settled, int block_size, int64_t num_pages, int window, float scale, void *out, void *scratch,
-                          size_t scratch_bytes, int *counters, int counters_len, int T, int H, int G, int d, const float *sinks,
+                          const int32_t *tile_seq, const int32_t *tile_t0, const int32_t *tile_nt, int n_tiles, int tile_tokens, int ctas,
+                          int min_steps, int tile_cost, int settled, int block_size, int64_t num_pages, int window, float scale, void *out, void *scratch,
+                          size_t scratch_bytes, int *counters, int counters_len, int H, int G, int d, const float *sinks,
                           int zero_sink, const float *slopes, const float *head_scales, float softcap, hfb_stream s);
 
 /* Launches may overlap with the kernel in front (programmatic dependent launch): on by default, off with HFB_PDL=0. */

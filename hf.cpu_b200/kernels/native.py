@@ -145,7 +145,9 @@ class NativeBackend:
             raise KernelError("the library's chunks and the binding's are not of one length")
         self.decay_chunks = os.environ.get("HFB_DECAY_CHUNKS", "1") != "0"     # portions of a recurrence with scalar decays in chunks
         self._kv8_counters = {}
-        self.kv8_ctas_per_sm, self.kv8_most_tiles = 6, 16
+        # attention of few queries over the 8-bit cache: CTAs per SM by (heads of 128, more than 8 places a tile), fewest steps of a CTA
+        self.kv8_ctas_per_sm, self.kv8_min_steps = {(False, False): 4, (False, True): 3, (True, False): 2, (True, True): 2}, 1
+        self.kv8_tile_cost = 2                    # ... and what a tile's start and end are reckoned as, in steps
         self.path = path
         self.launches = 0          # kernels launched through this binding (one per successful call)
 
@@ -441,30 +443,23 @@ class NativeBackend:
         return have
 
     def _kv8_few(self, q, cache, meta, ctx, H, G, d, window, scale, out, tiles, settled, opt_args):
-        from . import decode_split_hint, kv8_head_groups
+        from . import kv8_head_groups
         seq, t0, nt = tiles["few.seq"], tiles["few.t0"], tiles["few.nt"]
-        r, n_tiles, T = H // G, seq.shape[0], q.shape[0]
+        r, most = H // G, self.lib.hfb_kv8_attention_few_tiles()
         share = kv8_head_groups(r)
         tile_tokens = 1 if share > 1 or ctx.max_q_len == 1 else max(1, 16 // r)
-        # The most tiles of 64 keys a request may have when this launch runs: a captured one is replayed while the requests grow within
-        # the range that the split hint stands for.
-        longest = max(1, (ctx.max_kv_len + 63) // 64)
-        if torch.cuda.is_current_stream_capturing():
-            hint = getattr(ctx, "decode_split_hint", None) or decode_split_hint(ctx.max_kv_len)
-            longest = max(longest, {1: 6, 4: 7, 8: 15, 16: 63, 32: 127}.get(hint, 512))
-        if window:
-            longest = min(longest, abs(window) // 64 + 2)
-        ctas = n_tiles * G * share
-        per = max(1, min(self.kv8_most_tiles, ctas * longest // (self.kv8_ctas_per_sm * self.sm_count)))
-        splits = max(1, min(64, -(-longest // per)))
-        need = 0 if splits == 1 else 4 * T * H * splits * (d + 2)
-        scratch = ctx.buf("kv8_scratch", (need,), torch.uint8) if need else None
-        counters = self._kv8_zeros(q.device, ctas) if need else None
-        self._check(self.lib.hfb_kv8_attention_few(
-            _p(q), _p(cache), _p(meta.block_table), c_int(meta.max_blocks), _p(ctx.positions), _p(seq), _p(t0), _p(nt), c_int(n_tiles),
-            c_int(tile_tokens), c_int(splits), c_int(per), c_int(1 if settled else 0), c_int(meta.block_size), c_int64(cache.shape[0]),
-            c_int(window), c_float(scale), _p(out), _p(scratch), ctypes.c_size_t(need), _p(counters),
-            c_int(counters.numel() if need else 0), c_int(T), c_int(H), c_int(G), c_int(d), *opt_args, self._stream()), "kv8_attention_few")
+        ctas = self.kv8_ctas_per_sm[d == 128, tile_tokens * (r // share) > 8] * self.sm_count
+        need = self.lib.hfb_kv8_attention_few_scratch(c_int(ctas), c_int(d))
+        scratch = ctx.buf("kv8_scratch", (need,), torch.uint8)
+        for i in range(0, seq.shape[0], most):
+            n = min(most, seq.shape[0] - i)
+            counters = self._kv8_zeros(q.device, n * G * share)
+            at = lambda x: c_void_p(x.data_ptr() + 4 * i)
+            self._check(self.lib.hfb_kv8_attention_few(
+                _p(q), _p(cache), _p(meta.block_table), c_int(meta.max_blocks), _p(ctx.positions), at(seq), at(t0), at(nt), c_int(n),
+                c_int(tile_tokens), c_int(ctas), c_int(self.kv8_min_steps), c_int(self.kv8_tile_cost), c_int(1 if settled else 0), c_int(meta.block_size),
+                c_int64(cache.shape[0]), c_int(window), c_float(scale), _p(out), _p(scratch), ctypes.c_size_t(need), _p(counters),
+                c_int(counters.numel()), c_int(H), c_int(G), c_int(d), *opt_args, self._stream()), "kv8_attention_few")
 
     def swiglu(self, gu, out, interleaved):
         self._on_gpu(gu, out)
