@@ -1,8 +1,7 @@
 // Attention of few queries over the key/value cache in 8 bits (kv8.cuh): bfloat16, head sizes 64 and 128, pages of 8..64 tokens.
 //
-// What bounds it is reading the cache: d + 4 bytes a key, and as many a value.  A fifth warp keeps the copies going, one bulk copy per page
-// and head (codes and scales of keys and values are one record), several tiles of 64 keys ahead of the four warps that compute,
-// two of them a tile.
+// What bounds it is reading the cache: d + 4 bytes a key, and as many a value.  A warp of its own keeps the copies going, one bulk copy per page
+// and head (codes and scales of keys and values are one record), several tiles of 64 keys ahead of the warps that compute.
 //
 // Between the copy and the tensor core every byte has to become a 16-bit number, so that is what the layout serves:
 // * A code's byte, code + 128, is a float16 number as it stands: with a zero byte above it the subnormal (code + 128) 2^-24.  A key
@@ -18,9 +17,10 @@
 //   rows 0..7, the odd ones 8..15, so that a thread ends up with neighbours of the output.
 // * A query row is multiplied by the power of two that brings its largest number to 2^14..2^15: float16 then holds every number
 //   of it that matters exactly (eight bits, down to 2^-31 of the largest).
-// * A weight goes into the second product as p * (scale of the value / largest scale the warp has seen) * 2^15, at most 2^15,
-//   rounded once to float16 (11 bits; down to 2^-29 of the largest at full precision, 2^-39 at all).  When a larger scale arrives the sums
-//   so far are rescaled, as they are when the running maximum grows.
+// * A weight goes into the second product as p * (scale of the value / reference scale) * 2^10, p relative to a reference maximum.  The
+//   references are raised, and the sums so far rescaled, only when a score exceeds its by more than 2^4 or a scale by more than a
+//   factor of two: the product is 2^15 at most, and is rounded once to float16 (11 bits; weights down to 2^-24 of the largest at
+//   full precision, 2^-34 at all).  (Raised whenever a maximum grows, one of eight columns' did in more than half of the steps.)
 //
 // Work is cut evenly: all steps (64 keys of one tile and key/value head) stand in one row, a tile's behind `tile_cost` empty ones
 // for its queries and its merge, and CTA c of C walks steps c N / C to (c + 1) N / C.  The copies run ahead from one tile's keys into the next
@@ -37,7 +37,7 @@ static thread_local cudaError_t g_launch_err = cudaSuccess;      // what the las
 namespace hfb {
 int *error_word();
 
-constexpr int KF_THREADS = 160, KF_MAX_TILES = 2048;
+constexpr int KF_MAX_TILES = 2048;
 
 struct Kv8FewParams {
     Kv8Params a;
@@ -84,20 +84,28 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v)
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
+// (the first product of a sum)
+__device__ __forceinline__ void mma_f16_first(float *c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ void mma_f16(float *c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// D: head size; NT: columns (token, head) of a tile in eights; STAGES: tiles of 64 keys in flight; OPTS: a cap or slopes
-template <int D, int NT, int STAGES, bool OPTS>
-__global__ void __launch_bounds__(KF_THREADS, D == 128 ? 2 : (NT == 1 ? 4 : 3))
+// D: head size; NT: columns (token, head) of a tile in eights; STAGES: tiles of 64 keys in flight; OPTS: a cap or slopes; KH: sixteens of
+// keys a warp and step.  Two groups of 4 / KH computing warps take the tiles in turn.
+template <int D, int NT, int STAGES, bool OPTS, int KH, int CTAS>
+__global__ void __launch_bounds__(32 * (8 / KH + 1), CTAS)
 kv8_few_kernel(Kv8FewParams f, int *err)
 {
     const Kv8Params &p = f.a;
-    // (a stage belongs to one of the two pairs of warps: one that took turns on it could find the phase before its own complete)
-    static_assert(STAGES % 2 == 0, "the pairs of warps have stages of their own");
+    // (a stage belongs to one of the two groups of warps: one that took turns on it could find the phase before its own complete)
+    static_assert(STAGES % 2 == 0, "the groups of warps have stages of their own");
+    constexpr int WARPS = 8 / KH, GROUP = WARPS / 2, THREADS = 32 * (WARPS + 1);
     constexpr int COLS = 8 * NT, CH = D / 16, OROW = D + 4;  // (rows of the merge buffer in different banks)
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 127u) & ~127u;
@@ -108,18 +116,19 @@ kv8_few_kernel(Kv8FewParams f, int *err)
     const uint32_t full0 = base, empty0 = base + 8 * STAGES;
     volatile uint32_t *page_mask = (volatile uint32_t *)(gen + 16 * STAGES);
     volatile int *abort_flag = (volatile int *)(gen + 20 * STAGES), *last_flag = abort_flag + 1;
-    int *scan = (int *)(gen + 128);                           // [8]
+    int *scan = (int *)(gen + 128);                           // [WARPS + 1], 9 at most
     // two slots for coming pieces: a barrier each for their queries' arrival and release, the tile's numbers, the queries
-    const uint32_t q_full = base + 160, q_empty = base + 176;
+    const uint32_t q_full = base + 192, q_empty = base + 208;
     constexpr uint32_t Q_BYTES = COLS * D * 2, SLOT = 128 + Q_BYTES;
-    float *mo = (float *)(gen + 256 + 2 * SLOT), *ml = mo + 4 * COLS * OROW, *mv = ml + 4 * COLS * 2;
-    int *first_step = (int *)(mv + 4);                        // [n_tiles + 1]
-    const uint32_t tiles0 = (base + 256 + 2 * SLOT + (4 * COLS * (OROW + 2) + 4) * 4 + 4 * (f.n_tiles + 1) + 127u) & ~127u;
+    float *mo = (float *)(gen + 256 + 2 * SLOT), *ml = mo + WARPS * COLS * OROW, *mv = ml + WARPS * COLS * 2;
+    enum { I_T0, I_NT, I_POS_FIRST, I_POS_LAST, I_KT, I_LEN, I_HEADS, I_BEGINS, I_COUNTER, I_PIECES, I_PLACE, I_FIRST, I_FIRST_PLACE, I_POSITIONS = 16 };
+    int *first_step = (int *)(mv + WARPS);                        // [n_tiles + 1]
+    const uint32_t tiles0 = (base + 256 + 2 * SLOT + WARPS * (COLS * (OROW + 2) + 1) * 4 + 4 * (f.n_tiles + 1) + 127u) & ~127u;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (!f.settled) pdl_wait();                               // nothing is read that the kernels in front may still write
     if (threadIdx.x == 0) {
-        for (int s = 0; s < 2; s++) { mbar_init(q_full + 8 * s, 1); mbar_init(q_empty + 8 * s, 4); }
-        for (int s = 0; s < STAGES; s++) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 2); }
+        for (int s = 0; s < 2; s++) { mbar_init(q_full + 8 * s, 1); mbar_init(q_empty + 8 * s, WARPS); }
+        for (int s = 0; s < STAGES; s++) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, GROUP); }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -138,7 +147,7 @@ kv8_few_kernel(Kv8FewParams f, int *err)
         return x;
     };
     {
-        const int each = (f.n_tiles + KF_THREADS - 1) / KF_THREADS, i0 = min((int)threadIdx.x * each, f.n_tiles), i1 = min(i0 + each, f.n_tiles);
+        const int each = (f.n_tiles + THREADS - 1) / THREADS, i0 = min((int)threadIdx.x * each, f.n_tiles), i1 = min(i0 + each, f.n_tiles);
         int sum = 0;
         for (int i = i0; i < i1; i++) { first_step[i] = sum; sum += tile_of(i).n + f.tile_cost; }
         int up = sum;
@@ -149,7 +158,7 @@ kv8_few_kernel(Kv8FewParams f, int *err)
         int before = up - sum;
         for (int w = 0; w < warp; w++) before += scan[w];
         for (int i = i0; i < i1; i++) first_step[i] += before;
-        if (threadIdx.x == KF_THREADS - 1) first_step[f.n_tiles] = before + sum;
+        if (threadIdx.x == THREADS - 1) first_step[f.n_tiles] = before + sum;
     }
     __syncthreads();
     const int groups = p.G, r = p.H / groups;
@@ -185,7 +194,7 @@ kv8_few_kernel(Kv8FewParams f, int *err)
         it.len = (int)max(0ll, x - begin);
     };
 
-    if (warp == 4) {
+    if (warp == WARPS) {
         // ---- the copying warp: the lanes look up 32 pages at a time, and each asks for its page -------------------------------
         const int tiles_per_round = 32 / pages, kv_heads = groups / f.kv_share;
         bool ok = true;
@@ -214,8 +223,18 @@ kv8_few_kernel(Kv8FewParams f, int *err)
                 if (lane == 0) ok = mbar_wait(q_empty + 8 * slot, ((number >> 1) & 1) ^ 1, abort_flag, err);
                 ok = __shfl_sync(0xffffffffu, ok, 0);
                 if (!ok) break;
-                if (lane == 0) { info[0] = tl.t0; info[1] = tl.nt; info[2] = tl.pos_first; info[3] = tl.pos_last; info[4] = tl.kt_lo; }
-                if (lane < 16) info[8 + lane] = lane < tl.nt ? p.positions[tl.t0 + lane] : -1;
+                if (lane == 0) {
+                    // the piece for the computing warps; of a tile's pieces only the first can be its CTA's last
+                    const int c_first = (int)(((it.first + 1) * ctas - 1) / total);
+                    info[I_T0] = tl.t0; info[I_NT] = tl.nt; info[I_POS_FIRST] = tl.pos_first; info[I_POS_LAST] = tl.pos_last;
+                    info[I_KT] = tl.kt_lo + it.off; info[I_LEN] = it.len; info[I_HEADS] = it.g * r; info[I_BEGINS] = it.off == 0;
+                    info[I_COUNTER] = it.tile * groups + it.g;
+                    info[I_PIECES] = (int)(((it.first + it.n) * ctas - 1) / total) - c_first + 1;
+                    info[I_PLACE] = cta * 2 + (start_of(cta) >= it.first ? 0 : 1);
+                    info[I_FIRST] = c_first;
+                    info[I_FIRST_PLACE] = c_first * 2 + (start_of(c_first) >= it.first ? 0 : 1);
+                }
+                if (lane < 16) info[I_POSITIONS + lane] = lane < tl.nt ? p.positions[tl.t0 + lane] : -1;
                 __syncwarp();
                 const uint32_t bytes = (uint32_t)r * D * 2;
                 if (lane == 0) mbar_arrive_expect_tx(q_full + 8 * slot, tl.nt * bytes);
@@ -251,6 +270,11 @@ kv8_few_kernel(Kv8FewParams f, int *err)
                 }
             }
         }
+        // the end of the row
+        if (lane == 0 && ok && mbar_wait(q_empty + 8 * (number & 1), ((number >> 1) & 1) ^ 1, abort_flag, err)) {
+            ((int *)(gen + 256 + (number & 1) * SLOT))[I_LEN] = 0;
+            mbar_arrive(q_full + 8 * (number & 1));
+        }
     } else {
         // ---- the computing warps --------------------------------------------------------------------------------------------
         if (f.settled) pdl_wait();                            // the queries come from the kernel in front
@@ -258,40 +282,41 @@ kv8_few_kernel(Kv8FewParams f, int *err)
         const float log2e = 1.4426950408889634f, cap2 = p.softcap * log2e;
         const bool capped = p.softcap > 0.f;
         const int c4 = lane & 3, row8 = lane >> 2;
-        // warps 0 and 1 take every other tile, 32 keys each, warps 2 and 3 the others
-        const int kbase = (warp & 1) * 32;
+        const int kbase = (warp % GROUP) * 16 * KH, group = warp / GROUP;
         // ldmatrix: lanes 0..7 and 8..15 name the rows of two eights of keys, the upper lanes the same rows one piece further; this lane
         // holds the scores of the keys `row8` and `row8 + 8` of each sixteen
         const int turn = D == 128 ? lane & 7 : (lane & 7) >> 1;
-        uint32_t row_at[2], s_at[2][2];
+        uint32_t piece[KH][CH / 2], s_at[KH][2];
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
+        for (int h = 0; h < KH; h++) {
             const int kk = kbase + 16 * h + (lane & 7) + ((lane >> 3) & 1) * 8;
-            row_at[h] = (uint32_t)(kk / bs) * p.record + (uint32_t)(kk % bs) * D;
+#pragma unroll
+            for (int c = 0; c < CH / 2; c++)
+                piece[h][c] = (uint32_t)(kk / bs) * p.record + (uint32_t)(kk % bs) * D + (uint32_t)((2 * c + (lane >> 4)) ^ turn) * 16u;
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 const int k = kbase + 16 * h + 8 * u + row8;
                 s_at[h][u] = (uint32_t)(k / bs) * p.record + 2u * bs * D + 4u * (k % bs);
             }
         }
-        uint32_t piece[CH / 2];
-#pragma unroll
-        for (int c = 0; c < CH / 2; c++) piece[c] = (uint32_t)((2 * c + (lane >> 4)) ^ turn) * 16u;
         const uint32_t v_codes = (uint32_t)bs * D, v_scales = 4u * bs;
         const uint32_t all_pages = (1u << pages) - 1u;
-        bool ok = true;                                       // (a wait that ran out: the walk goes on without waiting, for the barriers' sake)
-        int js = 0, number = 0;
+        int js = 0;
 
-        for (long long x = start_of(cta); x < x_end;) {
-            Piece it;
-            piece_at(x, it);
-            if (it.len == 0) continue;
-            const int slot = number & 1, g = it.g;
-            const int *info = (const int *)(gen + 256 + slot * SLOT);
-            ok = mbar_wait(q_full + 8 * slot, (number >> 1) & 1, abort_flag, err) && ok;
-            number++;
-            const int t0 = info[0], nt = ok ? info[1] : 0, pos_first = info[2], pos_last = info[3];
-            const int lo_last = mask_lo(pos_last, p.window), kt_first = info[4] + it.off;
+        for (int number = 0;; number++) {
+            const int *info = (const int *)(gen + 256 + (number & 1) * SLOT);
+            bool ok = mbar_wait(q_full + 8 * (number & 1), (number >> 1) & 1, abort_flag, err);
+            {
+                // (a wait that ran out ends the walk of all warps together: none may be left at a barrier)
+                int all;
+                asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.and.pred q, 1, %2, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+                             : "=r"(all) : "r"((int)ok), "n"(32 * WARPS) : "memory");
+                if (!all) break;
+            }
+            const int len = info[I_LEN], nt = info[I_NT], heads = info[I_HEADS];
+            if (len == 0) break;
+            const int pos_first = info[I_POS_FIRST], pos_last = info[I_POS_LAST], kt_first = info[I_KT];
+            const int lo_last = mask_lo(pos_last, p.window);
             uint32_t qf[CH][NT][2];
             float fac[NT][2], off[NT][2], slope[NT][2];
             int pos[NT][2], lo[NT][2];
@@ -300,7 +325,7 @@ kv8_few_kernel(Kv8FewParams f, int *err)
                 // this lane's share of column 8 n + lane / 4: numbers 16 c + 4 (lane % 4) + 0..3
                 const int col = 8 * n + row8, tok = col / r, hl = col % r;
                 const bool valid = tok < nt;
-                const uint8_t *src = gen + 256 + slot * SLOT + 128 + (size_t)(valid ? col : 0) * D * 2 + 8 * c4;
+                const uint8_t *src = (const uint8_t *)(info + 32) + (valid ? col : 0) * D * 2 + 8 * c4;
                 uint2 raw[CH];
                 unsigned top = 0;
 #pragma unroll
@@ -325,11 +350,11 @@ kv8_few_kernel(Kv8FewParams f, int *err)
                 }
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                const float hs = p.head_scales && valid ? p.head_scales[g * r + hl] : 1.f;
+                const float hs = p.head_scales && valid ? p.head_scales[heads + hl] : 1.f;
                 const float unit = (capped ? p.scale * hs / p.softcap : p.scale * hs * log2e) * back, own_off = -128.f * sum * unit;
                 const float own = unit * 16777216.f;
-                const float sl = p.slopes && valid ? p.slopes[g * r + hl] * log2e : 0.f;
-                const int ps = valid ? info[8 + tok] : -1;
+                const float sl = p.slopes && valid ? p.slopes[heads + hl] * log2e : 0.f;
+                const int ps = valid ? info[I_POSITIONS + tok] : -1;
 #pragma unroll
                 for (int i = 0; i < 2; i++) {                 // ... and of the columns whose scores it will hold
                     fac[n][i] = __shfl_sync(0xffffffffu, own, 4 * (2 * c4 + i));
@@ -339,8 +364,6 @@ kv8_few_kernel(Kv8FewParams f, int *err)
                     lo[n][i] = mask_lo(pos[n][i], p.window);
                 }
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(q_empty + 8 * slot);
             float o[CH][NT][4], m[NT][2], l[NT][2], vm = 0.f, rv = 0.f;           // rv = 1 / vm
 #pragma unroll
             for (int n = 0; n < NT; n++) {
@@ -349,35 +372,38 @@ kv8_few_kernel(Kv8FewParams f, int *err)
 #pragma unroll
                 for (int c = 0; c < CH; c++) o[c][n][0] = o[c][n][1] = o[c][n][2] = o[c][n][3] = 0.f;
             }
-            const int skip = (js ^ (warp >> 1)) & 1;
-            for (int j = skip; j < it.len; j += 2) {
+            const int skip = (js ^ group) & 1;
+            for (int j = skip; j < len; j += 2) {
                 const int kt = kt_first + j, s = (js + j) % STAGES;
                 ok = mbar_wait(full0 + 8 * s, ((js + j) / STAGES) & 1, abort_flag, err) && ok;
                 if (!ok) continue;
-                const uint32_t st = tiles0 + s * stage_bytes;
+                const uint32_t st = tiles0 + s * stage_bytes, sv = st + v_codes;
                 const uint8_t *sg = gen + (tiles0 - base) + s * stage_bytes;
                 const uint32_t mask = page_mask[s];
-                float sc[2][NT][4];
+                // (two sums a score, of the even and the odd pieces of a row: a chain of products half as long)
+                float sc[KH][NT][4], sd[KH][NT][4];
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
+                for (int c = 0; c < CH / 2; c++)
 #pragma unroll
-                    for (int n = 0; n < NT; n++) sc[h][n][0] = sc[h][n][1] = sc[h][n][2] = sc[h][n][3] = 0.f;
-#pragma unroll
-                    for (int c = 0; c < CH / 2; c++) {
+                    for (int h = 0; h < KH; h++) {
                         uint32_t w0, w1, w2, w3;
-                        ldsm_x4(st + row_at[h] + piece[c], w0, w1, w2, w3);
+                        ldsm_x4(st + piece[h][c], w0, w1, w2, w3);
                         const uint32_t a0 = bytes_f16(w0, 0x4140), a1 = bytes_f16(w1, 0x4140), a2 = bytes_f16(w0, 0x4342), a3 = bytes_f16(w1, 0x4342);
                         const uint32_t b0 = bytes_f16(w2, 0x4140), b1 = bytes_f16(w3, 0x4140), b2 = bytes_f16(w2, 0x4342), b3 = bytes_f16(w3, 0x4342);
 #pragma unroll
                         for (int n = 0; n < NT; n++) {
-                            mma_f16(sc[h][n], a0, a1, a2, a3, qf[2 * c][n][0], qf[2 * c][n][1]);
-                            mma_f16(sc[h][n], b0, b1, b2, b3, qf[2 * c + 1][n][0], qf[2 * c + 1][n][1]);
+                            if (c == 0) {
+                                mma_f16_first(sc[h][n], a0, a1, a2, a3, qf[0][n][0], qf[0][n][1]);
+                                mma_f16_first(sd[h][n], b0, b1, b2, b3, qf[1][n][0], qf[1][n][1]);
+                            } else {
+                                mma_f16(sc[h][n], a0, a1, a2, a3, qf[2 * c][n][0], qf[2 * c][n][1]);
+                                mma_f16(sd[h][n], b0, b1, b2, b3, qf[2 * c + 1][n][0], qf[2 * c + 1][n][1]);
+                            }
                         }
                     }
-                }
-                float ks[2][2], vs[2][2];
+                float ks[KH][2], vs[KH][2];
 #pragma unroll
-                for (int h = 0; h < 2; h++)
+                for (int h = 0; h < KH; h++)
 #pragma unroll
                     for (int u = 0; u < 2; u++) {
                         ks[h][u] = *(const float *)(sg + s_at[h][u]);
@@ -388,15 +414,15 @@ kv8_few_kernel(Kv8FewParams f, int *err)
                 if (edge) {
                     // (rows behind the request's last and missing pages hold anything)
 #pragma unroll
-                    for (int h = 0; h < 2; h++)
+                    for (int h = 0; h < KH; h++)
 #pragma unroll
                         for (int u = 0; u < 2; u++) {
                             const int k = kbase + 16 * h + 8 * u + row8;
                             if (kt * ABN + k > pos_last || !(mask >> (k / bs) & 1u)) ks[h][u] = vs[h][u] = 0.f;
                         }
                 }
-                const float vs_top = fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[1][0], vs[1][1]));
-                if (__any_sync(0xffffffffu, vs_top > vm)) {
+                const float vs_top = fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[KH - 1][0], vs[KH - 1][1]));
+                if (__any_sync(0xffffffffu, vs_top > 2.f * vm)) {
                     float v = fmaxf(vm, vs_top);
                     v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
                     v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
@@ -409,16 +435,15 @@ kv8_few_kernel(Kv8FewParams f, int *err)
                     vm = v;
                     rv = 1.0f / v;
                 }
-                bool grew = false;
 #pragma unroll
-                for (int h = 0; h < 2; h++)
+                for (int h = 0; h < KH; h++)
 #pragma unroll
                     for (int n = 0; n < NT; n++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) sc[h][n][e] = fmaf(sc[h][n][e], fac[n][e & 1], off[n][e & 1]) * ks[h][e >> 1];
+                        for (int e = 0; e < 4; e++) sc[h][n][e] = fmaf(sc[h][n][e] + sd[h][n][e], fac[n][e & 1], off[n][e & 1]) * ks[h][e >> 1];
                 if (OPTS) {
 #pragma unroll
-                    for (int h = 0; h < 2; h++)
+                    for (int h = 0; h < KH; h++)
 #pragma unroll
                         for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -430,7 +455,7 @@ kv8_few_kernel(Kv8FewParams f, int *err)
                 }
                 if (edge) {
 #pragma unroll
-                    for (int h = 0; h < 2; h++)
+                    for (int h = 0; h < KH; h++)
 #pragma unroll
                         for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -439,19 +464,22 @@ kv8_few_kernel(Kv8FewParams f, int *err)
                                 if (key > pos[n][e & 1] || key < lo[n][e & 1] || !(mask >> (k / bs) & 1u)) sc[h][n][e] = -INFINITY;
                             }
                 }
+                float top[NT][2];
+                bool grew = false;
 #pragma unroll
-                for (int h = 0; h < 2; h++)
+                for (int n = 0; n < NT; n++)
 #pragma unroll
-                    for (int n = 0; n < NT; n++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) grew |= sc[h][n][e] > m[n][e & 1];
+                    for (int i = 0; i < 2; i++) {
+                        top[n][i] = fmaxf(fmaxf(sc[0][n][i], sc[0][n][2 + i]), fmaxf(sc[KH - 1][n][i], sc[KH - 1][n][2 + i]));
+                        grew |= top[n][i] > m[n][i] + 4.f;
+                    }
                 if (__any_sync(0xffffffffu, grew)) {
-                    // a maximum grew somewhere in the warp: rescale what has been summed so far
+                    // a maximum has outgrown its reference somewhere in the warp: rescale what has been summed so far
 #pragma unroll
                     for (int n = 0; n < NT; n++)
 #pragma unroll
                         for (int i = 0; i < 2; i++) {
-                            float v = fmaxf(fmaxf(m[n][i], fmaxf(sc[0][n][i], sc[0][n][2 + i])), fmaxf(sc[1][n][i], sc[1][n][2 + i]));
+                            float v = fmaxf(m[n][i], top[n][i]);
                             v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
                             v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
                             v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
@@ -462,10 +490,10 @@ kv8_few_kernel(Kv8FewParams f, int *err)
                             m[n][i] = v;
                         }
                 }
+                uint32_t pf[KH][NT][2];
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const float vn0 = vs[h][0] * rv * 32768.f, vn1 = vs[h][1] * rv * 32768.f;
-                    uint32_t pf[NT][2];
+                for (int h = 0; h < KH; h++) {
+                    const float vn0 = vs[h][0] * rv * 1024.f, vn1 = vs[h][1] * rv * 1024.f;
 #pragma unroll
                     for (int n = 0; n < NT; n++) {
                         float w[4];
@@ -477,26 +505,28 @@ kv8_few_kernel(Kv8FewParams f, int *err)
                             w[e] = q * (e < 2 ? vn0 : vn1);
                             if (edge && sc[h][n][e] == -INFINITY) w[e] = 0.f;    // (a value that is no number, for a row that does not see it)
                         }
-                        pf[n][0] = transpose8(pack_f16(w[0], w[1]));
-                        pf[n][1] = transpose8(pack_f16(w[2], w[3]));
+                        pf[h][n][0] = transpose8(pack_f16(w[0], w[1]));
+                        pf[h][n][1] = transpose8(pack_f16(w[2], w[3]));
                     }
+                }
+#pragma unroll
+                for (int h = 0; h < KH; h++)
 #pragma unroll
                     for (int c = 0; c < CH / 2; c++) {
                         uint32_t w0, w1, w2, w3;
-                        ldsm_x4_t(st + row_at[h] + piece[c] + v_codes, w0, w1, w2, w3);
+                        ldsm_x4_t(sv + piece[h][c], w0, w1, w2, w3);
                         const uint32_t a0 = codes_f16(w0, 0x4240), a1 = codes_f16(w0, 0x4341), a2 = codes_f16(w1, 0x4240), a3 = codes_f16(w1, 0x4341);
                         const uint32_t b0 = codes_f16(w2, 0x4240), b1 = codes_f16(w2, 0x4341), b2 = codes_f16(w3, 0x4240), b3 = codes_f16(w3, 0x4341);
 #pragma unroll
                         for (int n = 0; n < NT; n++) {
-                            mma_f16(o[2 * c][n], a0, a1, a2, a3, pf[n][0], pf[n][1]);
-                            mma_f16(o[2 * c + 1][n], b0, b1, b2, b3, pf[n][0], pf[n][1]);
+                            mma_f16(o[2 * c][n], a0, a1, a2, a3, pf[h][n][0], pf[h][n][1]);
+                            mma_f16(o[2 * c + 1][n], b0, b1, b2, b3, pf[h][n][0], pf[h][n][1]);
                         }
                     }
-                }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(empty0 + 8 * s);
             }
-            js += it.len;
+            js += len;
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -504,7 +534,7 @@ kv8_few_kernel(Kv8FewParams f, int *err)
                     l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], 4);
                     l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], 8);
                     l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], 16);
-                    // ---- merge the four warps (they saw disjoint keys) in warp order
+                    // ---- merge the warps (they saw disjoint keys) in warp order
                     const int col = 8 * n + 2 * c4 + i;
 #pragma unroll
                     for (int c = 0; c < CH; c++)
@@ -512,22 +542,21 @@ kv8_few_kernel(Kv8FewParams f, int *err)
                     if (row8 == 0) *(float2 *)(ml + (warp * COLS + col) * 2) = make_float2(m[n][i], l[n][i]);
                 }
             if (lane == 0) mv[warp] = vm;
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            const int rows = nt * r;
-            const bool whole = it.len == it.n;
-            const int place = cta * 2 + (start_of(cta) >= it.first ? 0 : 1);     // of a piece in the scratch
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory");
+            const int rows = nt * r, t0 = info[I_T0], pieces = info[I_PIECES], place = info[I_PLACE];
+            const bool whole = pieces == 1;
             float top_v = 0.f;
 #pragma unroll
-            for (int w = 0; w < 4; w++) top_v = fmaxf(top_v, mv[w]);
-            for (int idx = threadIdx.x; idx < rows * (D / 4); idx += 128) {
+            for (int w = 0; w < WARPS; w++) top_v = fmaxf(top_v, mv[w]);
+            for (int idx = threadIdx.x; idx < rows * (D / 4); idx += 32 * WARPS) {
                 const int row = idx / (D / 4), q4 = idx % (D / 4);
                 float top = -INFINITY;
 #pragma unroll
-                for (int w = 0; w < 4; w++) top = fmaxf(top, ml[(w * COLS + row) * 2]);
+                for (int w = 0; w < WARPS; w++) top = fmaxf(top, ml[(w * COLS + row) * 2]);
                 float denom = 0.f;
                 float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                for (int w = 0; w < 4; w++) {
+                for (int w = 0; w < WARPS; w++) {
                     const float mw = ml[(w * COLS + row) * 2];
                     const float e = mw == -INFINITY ? 0.f : fast_exp2(mw - top);
                     denom += ml[(w * COLS + row) * 2 + 1] * (mw == -INFINITY ? 1.f : e);       // (zero, or no number)
@@ -535,10 +564,10 @@ kv8_few_kernel(Kv8FewParams f, int *err)
                     const float4 v = *(const float4 *)(mo + (w * COLS + row) * OROW + 4 * q4);
                     acc.x += v.x * fo; acc.y += v.y * fo; acc.z += v.z * fo; acc.w += v.w * fo;
                 }
-                const float unit = top_v * (1.f / 32768.f);
+                const float unit = top_v * (1.f / 1024.f);
                 acc.x *= unit; acc.y *= unit; acc.z *= unit; acc.w *= unit;
-                const int head = g * r + row % r;
-                if ((p.sinks || p.zero_sink) && it.off == 0) {
+                const int head = heads + row % r;
+                if ((p.sinks || p.zero_sink) && info[I_BEGINS]) {
                     // the sink joins the first piece's sum as one more score; the merge of the pieces carries it like any other
                     const float sk = p.sinks ? p.sinks[head] * log2e : 0.f;
                     const float t = fmaxf(top, sk);
@@ -556,23 +585,26 @@ kv8_few_kernel(Kv8FewParams f, int *err)
                     if (q4 == 0) *(float2 *)(f.part_ml + ((size_t)place * COLS + row) * 2) = make_float2(top, denom);
                 }
             }
-            asm volatile("bar.sync 1, 128;" ::: "memory");    // the buffer is free again
-            if (whole) continue;
-
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory");    // the buffer is free again
             // ---- merge the pieces: whoever stored its piece last, in the order of the keys ----------------------------------------
-            const int c_first = (int)(((it.first + 1) * ctas - 1) / total), pieces = (int)(((it.first + it.n) * ctas - 1) / total) - c_first + 1;
-            if (threadIdx.x == 0) {
-                __threadfence();                              // (after the barrier: it covers every thread's stores)
-                int *cnt = f.counters + (size_t)it.tile * groups + g;
-                const int last = atomicAdd(cnt, 1) == pieces - 1;
-                if (last) *cnt = 0;
-                *last_flag = last;
+            bool last = false;
+            const int c_first = info[I_FIRST], first_place = info[I_FIRST_PLACE];
+            if (!whole) {
+                if (threadIdx.x == 0) {
+                    __threadfence();                          // (after the barrier: it covers every thread's stores)
+                    int *cnt = f.counters + info[I_COUNTER];
+                    const int is = atomicAdd(cnt, 1) == pieces - 1;
+                    if (is) *cnt = 0;
+                    *last_flag = is;
+                }
+                asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory");
+                last = *last_flag;                            // (written again behind two barriers)
             }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            if (!*last_flag) continue;                        // (the flag is written again behind two barriers)
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_empty + 8 * (number & 1));
+            if (!last) continue;
             __threadfence();
-            const int first_place = c_first * 2 + (start_of(c_first) >= it.first ? 0 : 1);
-            for (int idx = threadIdx.x; idx < rows * (D / 4); idx += 128) {
+            for (int idx = threadIdx.x; idx < rows * (D / 4); idx += 32 * WARPS) {
                 const int row = idx / (D / 4), q4 = idx % (D / 4);
                 float top = -INFINITY, denom = 0.f;
                 float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -599,7 +631,7 @@ kv8_few_kernel(Kv8FewParams f, int *err)
                     top = t;
                 }
                 const float inv = denom == 0.f ? 0.f : 1.0f / denom;
-                *(uint2 *)((__nv_bfloat16 *)p.out + ((size_t)(t0 + row / r) * p.H + g * r + row % r) * D + 4 * q4) =
+                *(uint2 *)((__nv_bfloat16 *)p.out + ((size_t)(t0 + row / r) * p.H + heads + row % r) * D + 4 * q4) =
                     make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
             }
         }
@@ -610,25 +642,28 @@ kv8_few_kernel(Kv8FewParams f, int *err)
     __syncthreads();
 }
 
-template <int D, int NT, int STAGES, bool OPTS>
+template <int D, int NT, int STAGES, int KH, int CTAS, bool OPTS>
 static int launch_kv8_few_opts(const Kv8FewParams &f, int ctas, cudaStream_t st)
 {
-    constexpr int fixed = 128 + 256 + 2 * (128 + 8 * NT * D * 2) + (4 * 8 * NT * (D + 6) + 4) * 4 + 128, most = fixed + 4 * (KF_MAX_TILES + 1) + STAGES * ABN * (2 * D + 8);
+    constexpr int fixed = 128 + 256 + 2 * (128 + 8 * NT * D * 2) + 8 / KH * (8 * NT * (D + 6) + 1) * 4 + 128;
+    constexpr int most = fixed + 4 * (KF_MAX_TILES + 1) + STAGES * ABN * (2 * D + 8);
     const int smem = fixed + 4 * (f.n_tiles + 1) + STAGES * (ABN / f.a.block_size) * f.a.record;
+    const auto kernel = kv8_few_kernel<D, NT, STAGES, OPTS, KH, CTAS>;
     static bool configured[64] = {false};                     // (the opt-in is a property of the function on one device)
     if (!configured[current_device()]) {
-        cudaError_t e = cudaFuncSetAttribute(kv8_few_kernel<D, NT, STAGES, OPTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
         if (e != cudaSuccess) return fail(HFB_ECUDA, "kv8_attention_few: cannot opt in to %d bytes of shared memory: %s", most, cudaGetErrorString(e));
         configured[current_device()] = true;
     }
-    g_launch_err = launch_pdl(kv8_few_kernel<D, NT, STAGES, OPTS>, dim3(ctas), dim3(KF_THREADS), smem, st, f, error_word());
+    g_launch_err = launch_pdl(kernel, dim3(ctas), dim3(32 * (8 / KH + 1)), smem, st, f, error_word());
     return check_pdl_launch(g_launch_err, "kv8_attention_few");
 }
 
-template <int D, int NT, int STAGES>
+template <int D, int NT, int STAGES, int KH, int CTAS>
 static int launch_kv8_few(const Kv8FewParams &f, int ctas, cudaStream_t st)
 {
-    return f.a.slopes || f.a.softcap > 0.f ? launch_kv8_few_opts<D, NT, STAGES, true>(f, ctas, st) : launch_kv8_few_opts<D, NT, STAGES, false>(f, ctas, st);
+    return f.a.slopes || f.a.softcap > 0.f ? launch_kv8_few_opts<D, NT, STAGES, KH, CTAS, true>(f, ctas, st)
+                                           : launch_kv8_few_opts<D, NT, STAGES, KH, CTAS, false>(f, ctas, st);
 }
 
 }  // namespace hfb
@@ -668,6 +703,6 @@ extern "C" int hfb_kv8_attention_few(const void *q, const void *cache, const int
     f.part_o = (float *)scratch; f.part_ml = (float *)scratch + (size_t)ctas * 2 * 16 * d;
     f.counters = counters; f.n_tiles = n_tiles; f.min_steps = min_steps; f.tile_cost = tile_cost; f.kv_share = share; f.settled = settled;
     cudaStream_t st = (cudaStream_t)s;
-    if (d == 128) return cols <= 8 ? launch_kv8_few<128, 1, 4>(f, ctas, st) : launch_kv8_few<128, 2, 4>(f, ctas, st);
-    return cols <= 8 ? launch_kv8_few<64, 1, 4>(f, ctas, st) : launch_kv8_few<64, 2, 4>(f, ctas, st);
+    if (d == 128) return cols <= 8 ? launch_kv8_few<128, 1, 4, 1, 2>(f, ctas, st) : launch_kv8_few<128, 2, 4, 1, 1>(f, ctas, st);
+    return cols <= 8 ? launch_kv8_few<64, 1, 4, 1, 2>(f, ctas, st) : launch_kv8_few<64, 2, 4, 1, 2>(f, ctas, st);
 }

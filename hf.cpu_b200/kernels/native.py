@@ -146,8 +146,8 @@ class NativeBackend:
         self.decay_chunks = os.environ.get("HFB_DECAY_CHUNKS", "1") != "0"     # portions of a recurrence with scalar decays in chunks
         self._kv8_counters = {}
         # attention of few queries over the 8-bit cache: CTAs per SM by (heads of 128, more than 8 places a tile), fewest steps of a CTA
-        self.kv8_ctas_per_sm, self.kv8_min_steps = {(False, False): 4, (False, True): 3, (True, False): 2, (True, True): 2}, 1
-        self.kv8_tile_cost = 2                    # ... and what a tile's start and end are reckoned as, in steps
+        self.kv8_ctas_per_sm, self.kv8_min_steps = {(False, False): 2, (False, True): 2, (True, False): 2, (True, True): 1}, 1
+        self.kv8_tile_cost = 6                    # ... and what a tile's start and end are reckoned as, in steps
         self.path = path
         self.launches = 0          # kernels launched through this binding (one per successful call)
 
