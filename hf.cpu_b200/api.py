@@ -13,6 +13,7 @@ from typing import Callable, Dict, List, Optional, Sequence, Union
 
 import torch
 
+from . import kernels
 from .engine import Engine, FinishEvent, Request, Scheduler, TokenEvent
 from .models import Model, load_model
 from .sampling import SamplingParams
@@ -32,7 +33,9 @@ class Completion:
 class Session:
     def __init__(self, model: Union[str, Model], dtype: str = "bfloat16", device: str = "cuda:0", ctx_max: int = 0,
                  batch: int = 0, kv_block: int = 16, kv_pages: int = 0, kv_mem: int = 0, max_seqs: int = 64,
-                 max_batched_tokens: int = 2048, eos_ids: Optional[Sequence[int]] = None):
+                 max_batched_tokens: int = 2048, eos_ids: Optional[Sequence[int]] = None, kv_dtype: str = "auto"):
+        """``kv_dtype``: "auto" (the cache holds the run's type) or "int8" (whole numbers with a scale per token and head: half the
+        bytes of bfloat16, so twice the tokens in the same memory)."""
         if isinstance(model, str):
             if dtype not in _DTYPES:
                 raise ValueError(f"dtype must be one of {sorted(_DTYPES)}")
@@ -40,29 +43,31 @@ class Session:
         self.model = model
         ctx_max = min(ctx_max or model.plan.max_positions, model.plan.max_positions)
         if not kv_pages:
-            kv_pages = self._default_pages(model, kv_block, kv_mem, max_seqs, ctx_max)
-        self.engine = Engine(model, block_size=kv_block, num_pages=kv_pages, max_requests=max_seqs, ctx_max=ctx_max)
+            kv_pages = self._default_pages(model, kv_block, kv_mem, max_seqs, ctx_max, kv_dtype)
+        self.engine = Engine(model, block_size=kv_block, num_pages=kv_pages, max_requests=max_seqs, ctx_max=ctx_max, kv_dtype=kv_dtype)
         self.scheduler = Scheduler(self.engine, max_num_seqs=max_seqs, max_num_batched_tokens=max_batched_tokens,
                                    prefill_chunk=batch)
         self.eos_ids = list(eos_ids) if eos_ids is not None else list(model.plan.eos_token_ids)
         self._serial = 0
 
     @staticmethod
-    def _default_pages(model: Model, block: int, kv_mem: int, max_seqs: int, ctx_max: int) -> int:
+    def _default_pages(model: Model, block: int, kv_mem: int, max_seqs: int, ctx_max: int, kv_dtype: str = "auto") -> int:
         """Pages for every slot at full context, bounded by ``kv_mem`` bytes or by most of the free memory."""
-        per_token = 0
+        per_page = 0
         for i, e in enumerate(model.plan.schedule):
             spec = model.layers[e.layer].mixer.cache_spec()
-            if e.cache_of is None and spec is not None:
-                per_token += spec.num_kv_heads * (spec.head_dim + spec.value_dim) * (2 if model.run_dtype == torch.bfloat16 else 4)
+            if e.cache_of is None and spec is not None and kv_dtype == "int8" and kernels.kv8_takes(spec.head_dim, block):
+                per_page += spec.num_kv_heads * kernels.kv8_record_bytes(block, spec.head_dim)
+            elif e.cache_of is None and spec is not None:
+                per_page += block * spec.num_kv_heads * (spec.head_dim + spec.value_dim) * (2 if model.run_dtype == torch.bfloat16 else 4)
         want = max_seqs * ((ctx_max + block - 1) // block)
         if model.device.type == "cuda":
             free, _ = torch.cuda.mem_get_info(model.device)
             limit = kv_mem or int(free * 0.8)
         else:
             limit = kv_mem or 1 << 30
-        if per_token:
-            want = min(want, max(1, limit // (per_token * block)))
+        if per_page:
+            want = min(want, max(1, limit // per_page))
         return max(want, 1)
 
     def generate(self, prompt_ids: Union[Sequence[int], Sequence[Sequence[int]]], *, temp: float = 0.8,
@@ -116,6 +121,6 @@ class Session:
 
 def generate(model: str, prompt_ids, dtype: str = "bfloat16", **options):
     """One-shot form: load ``model`` (a folder), generate, return the completions."""
-    session_keys = ("device", "ctx_max", "batch", "kv_block", "kv_pages", "kv_mem", "max_seqs", "max_batched_tokens")
+    session_keys = ("device", "ctx_max", "batch", "kv_block", "kv_pages", "kv_mem", "max_seqs", "max_batched_tokens", "kv_dtype")
     sess = Session(model, dtype=dtype, **{k: options.pop(k) for k in session_keys if k in options})
     return sess.generate(prompt_ids, **options)

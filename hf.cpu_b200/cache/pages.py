@@ -23,6 +23,8 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import numpy as np
 import torch
 
+from .. import kernels
+from ..config.base import UnsupportedError
 from ..parts.base import CacheSpec
 
 
@@ -82,22 +84,35 @@ class PagePool:
 @dataclass
 class LayerCache:
     """One schedule entry's keys ``[num_pages, block_size, kv_heads, head_dim]`` and values (the same, or
-    ``value_dim`` wide)."""
+    ``value_dim`` wide); of a cache in 8 bits neither, but its records ``kv8`` (``kernels.kv8_cache``)."""
     group: int
     k: torch.Tensor
     v: torch.Tensor
+    kv8: Optional[torch.Tensor] = None
+
+    def tensors(self) -> tuple:
+        return (self.k, self.v) if self.kv8 is None else (self.kv8,)
 
 
 class CacheGroup:
     """Schedule entries with the same needs share page geometry, a pool and block tables."""
 
     def __init__(self, index: int, spec: CacheSpec, entries: Sequence[int], num_pages: int, block_size: int,
-                 dtype: torch.dtype, device: torch.device):
+                 dtype: torch.dtype, device: torch.device, eight_bits: bool = False):
         self.index, self.spec, self.entries = index, spec, list(entries)
         self.block_size, self.num_pages = block_size, num_pages
         self.pool = PagePool(num_pages)
         shape = (len(self.entries), num_pages, block_size, spec.num_kv_heads)
-        if spec.values_in_keys:
+        self.records = None
+        if eight_bits:
+            if spec.values_in_keys or spec.value_dim != spec.head_dim or not kernels.kv8_takes(spec.head_dim, block_size):
+                raise UnsupportedError(f"a cache in 8 bits holds keys and values of one size, a multiple of 16 up to {kernels.MAX_HEAD_DIM}, in pages of "
+                                       f"up to {kernels.KV8_BLOCK} tokens; this model has layers with "
+                                       + ("values inside their keys" if spec.values_in_keys else f"heads of {spec.head_dim} and {spec.value_dim}"))
+            self.storage = self.keys = self.values = None
+            self.records = kernels.kv8_cache(len(self.entries) * num_pages, block_size, spec.num_kv_heads, spec.head_dim, device).view(
+                len(self.entries), num_pages, spec.num_kv_heads, -1)
+        elif spec.values_in_keys:
             # one array of rows; whoever reads values reads them out of the keys
             self.storage = None
             self.keys = torch.zeros(shape + (spec.head_dim,), dtype=dtype, device=device)
@@ -115,11 +130,15 @@ class CacheGroup:
 
     @property
     def page_bytes(self) -> int:
+        if self.records is not None:
+            return len(self.entries) * self.spec.num_kv_heads * self.records.shape[-1]
         return (len(self.entries) * self.block_size * self.spec.num_kv_heads * (self.spec.head_dim + self.spec.value_dim)
                 * self.keys.element_size())
 
     def layer_cache(self, entry: int) -> LayerCache:
         i = self.entries.index(entry)
+        if self.records is not None:
+            return LayerCache(self.index, None, None, self.records[i])
         return LayerCache(self.index, self.keys[i], self.values[i] if self.values is not None else None)
 
     def first_needed_block(self, next_pos: int) -> int:
@@ -142,7 +161,7 @@ class KVCacheManager:
     """Owns every group's pool and every request's block tables."""
 
     def __init__(self, entry_specs: Dict[int, CacheSpec], block_size: int, num_pages: int,
-                 dtype: torch.dtype, device: torch.device, max_blocks_per_request: int):
+                 dtype: torch.dtype, device: torch.device, max_blocks_per_request: int, eight_bits: bool = False):
         if block_size < 1:
             raise ValueError("block_size must be at least 1")
         self.block_size, self.max_blocks = block_size, max_blocks_per_request
@@ -150,7 +169,7 @@ class KVCacheManager:
         for entry, spec in sorted(entry_specs.items()):
             by_spec.setdefault(spec, []).append(entry)
         self.groups: List[CacheGroup] = [
-            CacheGroup(i, spec, entries, num_pages, block_size, dtype, device)
+            CacheGroup(i, spec, entries, num_pages, block_size, dtype, device, eight_bits)
             for i, (spec, entries) in enumerate(by_spec.items())]
         self._entry_cache: Dict[int, LayerCache] = {}
         for g in self.groups:

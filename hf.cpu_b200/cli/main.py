@@ -143,7 +143,8 @@ class App:
             self.session = hfcpu_b200.Session(
                 self._random_model() if path.startswith("random:") else path, dtype=self.o["dtype"], ctx_max=int(self.o["ctx_max"]), batch=int(self.o["batch"]),
                 kv_block=self.o["kv_block"], kv_pages=int(self.o["kv_pages"]), kv_mem=int(self.o["kv_mem"]),
-                max_seqs=self.o["max_seqs"], max_batched_tokens=self.o["max_batched_tokens"], eos_ids=eos)
+                max_seqs=self.o["max_seqs"], max_batched_tokens=self.o["max_batched_tokens"], eos_ids=eos,
+                kv_dtype=self.o["kv_dtype"])
         except UnsupportedError as e:
             raise Failure("ENOTSUP", str(e)) from None
         except (ConfigError, WeightError, WeightFormatError) as e:

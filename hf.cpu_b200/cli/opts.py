@@ -57,6 +57,8 @@ OPTIONS: List[Opt] = [
     Opt("dtype", ENUM, SESSION, "bf16", "bf16 | fp32 (fp32 = the whole model in true 32-bit)",
         choices=("bf16", "fp32", "bfloat16", "float32")),
     Opt("kv-block", INT, SESSION, 16, "tokens per cache page", 1, 1024),
+    Opt("kv-dtype", ENUM, SESSION, "auto", "auto | int8: keys and values cached in the run's type, or in 8 bits with a scale per token and head",
+        choices=("auto", "int8")),
     Opt("kv-pages", SIZE, SESSION, 0, "cache pages per layer group, 0 = from --kv-mem or free memory"),
     Opt("kv-mem", SIZE, SESSION, 0, "bytes for the cache, 0 = most of the free memory"),
     Opt("max-seqs", INT, SESSION, 64, "requests decoded together at most", 1, 4096),

@@ -316,7 +316,7 @@ kv8_few_kernel(Kv8FewParams f, int *err)
             const int len = info[I_LEN], nt = info[I_NT], heads = info[I_HEADS];
             if (len == 0) break;
             const int pos_first = info[I_POS_FIRST], pos_last = info[I_POS_LAST], kt_first = info[I_KT];
-            const int lo_last = mask_lo(pos_last, p.window);
+            const int lo_first = mask_lo(pos_first, p.window), lo_last = mask_lo(pos_last, p.window);
             uint32_t qf[CH][NT][2];
             float fac[NT][2], off[NT][2], slope[NT][2];
             int pos[NT][2], lo[NT][2];
@@ -412,13 +412,13 @@ kv8_few_kernel(Kv8FewParams f, int *err)
                 // a tile wholly inside every row's range, with all of its pages, needs no mask
                 const bool edge = kt * ABN + ABN - 1 > pos_first || kt * ABN < lo_last || mask != all_pages;
                 if (edge) {
-                    // (rows behind the request's last and missing pages hold anything)
+                    // (rows behind the request's last, those that every token's mask has passed and missing pages hold anything)
 #pragma unroll
                     for (int h = 0; h < KH; h++)
 #pragma unroll
                         for (int u = 0; u < 2; u++) {
                             const int k = kbase + 16 * h + 8 * u + row8;
-                            if (kt * ABN + k > pos_last || !(mask >> (k / bs) & 1u)) ks[h][u] = vs[h][u] = 0.f;
+                            if (kt * ABN + k > pos_last || kt * ABN + k < lo_first || !(mask >> (k / bs) & 1u)) ks[h][u] = vs[h][u] = 0.f;
                         }
                 }
                 const float vs_top = fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[KH - 1][0], vs[KH - 1][1]));

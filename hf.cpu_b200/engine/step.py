@@ -17,8 +17,12 @@ import numpy as np
 import torch
 
 from .. import kernels
+from ..config.base import UnsupportedError
 from ..cache import KVCacheManager, OutOfPages, StateSlots
 from ..models import EMBEDDING_STATE, Model, block_state_key
+
+
+KV_DTYPES = ("auto", "int8")
 
 
 @dataclass
@@ -77,6 +81,7 @@ class StepBatch:
     kv_lens: List[int]                 # tokens each request holds after the step
     starts: List[int]                  # position of each request's first token of the step
     block_size: int
+    eight_bits: bool = False           # the cache holds keys and values in 8 bits
 
     @property
     def num_seqs(self) -> int:
@@ -97,6 +102,7 @@ class StepContext:
     def __init__(self, engine: "Engine"):
         self.engine = engine
         self.run_dtype = engine.model.run_dtype
+        self.eight_bits = engine.eight_bits
         self.device = engine.device
         self.num_tokens = self.num_seqs = self.num_logit_rows = 0
         self.logits_for_all = False
@@ -130,13 +136,17 @@ class Engine:
     """Model + cache + slots + the step function.
 
     ``num_pages`` pages of ``block_size`` tokens are made for every cache group.  ``ctx_max`` bounds
-    one request's length; ``max_requests`` bounds how many are live at once.
+    one request's length; ``max_requests`` bounds how many are live at once.  ``kv_dtype``: "auto", keys and values in the run's
+    type, or "int8", as whole numbers with a scale per token and head (``kernels.kv8_cache``): half the bytes of bfloat16.
     """
 
     def __init__(self, model: Model, *, block_size: int = 16, num_pages: int = 0, max_tokens: int = 0,
-                 max_requests: int = 64, ctx_max: int = 0):
+                 max_requests: int = 64, ctx_max: int = 0, kv_dtype: str = "auto"):
         if not model.bound:
             raise ValueError("the model has no weights bound")
+        if kv_dtype not in KV_DTYPES:
+            raise ValueError(f"kv_dtype must be one of {', '.join(KV_DTYPES)}")
+        self.eight_bits = kv_dtype == "int8"
         self.model, self.device = model, model.device
         plan = model.plan
         self.ctx_max = int(ctx_max) if ctx_max else plan.max_positions
@@ -162,6 +172,11 @@ class Engine:
         for i, e in enumerate(plan.schedule):
             if e.cache_of is not None and e.cache_of not in cache_specs:
                 raise ValueError(f"schedule entry {i} reads the cache of entry {e.cache_of}, which keeps none")
+        if self.eight_bits:
+            for e in plan.schedule:
+                mixer = model.layers[e.layer].mixer
+                if mixer.cache_spec() is not None and not mixer.caches_eight_bits:
+                    raise UnsupportedError(f"layer {e.layer} ({type(mixer).__name__}) does not run on a cache in 8 bits")
         # index arrays the mixers want built per step (tile lists of their kernels and the like): one owner per key,
         # so that layers with the same needs share one set
         self._array_owners: Dict[Hashable, object] = {}
@@ -170,7 +185,7 @@ class Engine:
             if key is not None:
                 self._array_owners.setdefault(key, l.mixer)
         self.cache = KVCacheManager(cache_specs, self.block_size, self.num_pages, model.run_dtype,
-                                    self.device, self.max_blocks)
+                                    self.device, self.max_blocks, self.eight_bits)
         self.slots = StateSlots(state_specs, self.max_requests, self.device)
         self.workspace = Workspace(self.device)
         self._pinned = self.device.type == "cuda"
@@ -183,6 +198,7 @@ class Engine:
         self._static_meta: Dict[int, torch.Tensor] = {}
         self._meta_ring = []            # [host buffer, device buffer, event of its last copy]
         self._meta_next = 0
+        self._places = None
         self.steps_run = 0
 
     # ---- requests -----------------------------------------------------------------------------
@@ -212,6 +228,36 @@ class Engine:
 
     def length(self, req) -> int:
         return self.cache.length(req)
+
+    def places(self, n: int) -> torch.Tensor:
+        """0, 1, ... n - 1 (int32): the slots of rows that lie one behind the other."""
+        if self._places is None or self._places.numel() < n:
+            self._places = torch.arange(max(n, 4096), dtype=torch.int32, device=self.device)
+        return self._places[:n]
+
+    def read_cache(self, req: Hashable, entry: int = 0):
+        """What a request holds in a schedule entry's cache: ``(first position, keys, values)`` with keys and values [tokens, heads, size]
+        in the run's type, from the first position whose page a window has not given back.  Values are None where they lie inside
+        the keys.  Reads what the steps run so far have written."""
+        cache = self.cache.entry_cache(entry)
+        if cache is None:
+            raise ValueError(f"schedule entry {entry} keeps no cache of its own")
+        bs, n, table = self.block_size, self.cache.length(req), self.cache.table(cache.group, req)
+        last = (n + bs - 1) // bs
+        first = next((b for b in range(last) if table[b] >= 0), last)
+        pages = torch.tensor(table[first:last], dtype=torch.int32, device=self.device)
+        start, count = first * bs, n - first * bs
+        if count <= 0:
+            start, count = n, 0
+        if cache.kv8 is None:
+            rows = [None if x is None else x[pages.long()].flatten(0, 1)[:count].clone() for x in (cache.k, cache.v)]
+            return start, rows[0], rows[1]
+        spec = self.cache.groups[cache.group].spec
+        k, v = (torch.empty(len(pages), bs, spec.num_kv_heads, spec.head_dim, dtype=self.model.run_dtype, device=self.device) for _ in range(2))
+        if len(pages):
+            used = torch.full((len(pages),), bs, dtype=torch.int32, device=self.device)
+            kernels.kv8_read(cache.kv8, pages, used, k, v)
+        return start, k.flatten(0, 1)[:count], v.flatten(0, 1)[:count]
 
     def live_requests(self):
         return list(self.slots.slot_of)
@@ -274,7 +320,7 @@ class Engine:
         kv_lens = [w[1] for w in wants]
         max_q = max(q_lens)
         MB = self.max_blocks if static else max(1, (max(kv_lens) + bs - 1) // bs)
-        batch = StepBatch(q_lens, kv_lens, starts, bs)
+        batch = StepBatch(q_lens, kv_lens, starts, bs, self.eight_bits)
         extras = [(key, {n: np.ascontiguousarray(v, dtype=np.int32) for n, v in mixer.step_arrays(batch).items()})
                   for key, mixer in self._array_owners.items()]
         total = 3 * T + (S + 1) + 2 * S + M + len(groups) * (T + S * MB) + sum(len(v) for _, arrs in extras for v in arrs.values())

@@ -136,7 +136,7 @@ class Model:
     def _replay_tensors(self, i: int, cache):
         a, b, c, d, e = self._replay_parts(i)
         own = (*a.replay_tensors(), *b.replay_tensors(), *c.replay_tensors(), *d.replay_tensors(), *e.replay_tensors())
-        return own if cache is None else (*own, cache.k, cache.v)
+        return own if cache is None else (*own, *cache.tensors())
 
     def _look_for_alike(self) -> None:
         """``_alike``: for each schedule entry a number that entries share whose kernels differ in their tensors only; None for the

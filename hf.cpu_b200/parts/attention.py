@@ -87,6 +87,7 @@ class OutputProduct:
 
 class PagedAttention(OutputProduct, Mixer):
     graph_safe = True
+    caches_eight_bits = True
     V_FIRST = "attn_v_first"          # the scratch buffer in which a step's first value-mixing layer leaves its values
 
     def __init__(self, hidden_size: int, num_heads: int, num_kv_heads: int, head_dim: int,
@@ -196,6 +197,8 @@ class PagedAttention(OutputProduct, Mixer):
 
     def step_arrays(self, batch):
         # the tile lists of the attention kernels: how they cut the step's tokens is the kernels' business
+        if getattr(batch, "eight_bits", False):
+            return kernels.kv8_step_arrays(batch.q_lens, self.H // self.G)
         return kernels.attention_step_arrays(batch.q_lens, self.H // self.G)
 
     def _projections(self):
@@ -299,15 +302,22 @@ class PagedAttention(OutputProduct, Mixer):
     def takes_stream(self, ctx, T, norm):
         """Whether :meth:`forward_from_stream` takes a step of ``T`` tokens: the plain rotated layer, few tokens."""
         return (self.is_plain(PagedAttention, "forward", "forward_then_norm", "_attend") and not self.general and not self.row_norm and self.rotary is not None and self.rotary.n_rot == self.d and self.d in (64, 128)
-                and kernels.few_tokens(T, ctx.run_dtype, norm, self.w_o, rope=self.w_qkv))
+                and (kernels.few_tokens(T, ctx.run_dtype, norm, self.w_o, self.w_qkv) if getattr(ctx, "eight_bits", False)
+                     else kernels.few_tokens(T, ctx.run_dtype, norm, self.w_o, rope=self.w_qkv)))
 
     def forward_from_stream(self, ctx, x, norm, cache, write_cache):
         """``x += mixer(norm(x))`` with the norm in the projections' kernel (``norm`` = (weight, eps) of an RMSNorm)."""
         T, meta = x.shape[0], ctx.group_meta(cache.group)
         q = ctx.buf("attn_q", (T, self.QD), ctx.run_dtype)
         with kernels.phase("qkv"):
-            kernels.few_rope_kv(x, norm, self.w_qkv, self.b_qkv, self.rotary.cos_sin, ctx.positions, meta.slots if write_cache else None, q,
-                                cache.k, cache.v, self.H, self.G, self.d)
+            if cache.kv8 is not None:
+                qkv = ctx.buf("attn_qkv", (T, self.QD + 2 * self.KD), ctx.run_dtype)
+                kernels.few_linear(x, norm, self.w_qkv, self.b_qkv, qkv, False)
+                kernels.rope_kv8_write(qkv, self.rotary.cos_sin, self.rotary.n_rot, ctx.positions, meta.slots if write_cache else None, q, cache.kv8,
+                                       self.H, self.G, self.d, meta.block_size)
+            else:
+                kernels.few_rope_kv(x, norm, self.w_qkv, self.b_qkv, self.rotary.cos_sin, ctx.positions, meta.slots if write_cache else None, q,
+                                    cache.k, cache.v, self.H, self.G, self.d)
         att = self._softmax_attention(ctx, q, cache, meta)
         with kernels.phase("wo"):
             kernels.few_linear(att, None, self.w_o, self.b_o, x, True)
@@ -320,19 +330,40 @@ class PagedAttention(OutputProduct, Mixer):
         q = ctx.buf("attn_q", (T, self.QD), xn.dtype)
         gates = ctx.buf("attn_head_gates", (T, self.H), torch.float32) if self.head_gate_name else None
         with kernels.phase("qkv"):
+            k, v, slots = self._kv_places(ctx, T, G, cache, meta, write_cache)
             kernels.linear_row_norm_kv(xn, self.w_qkv, ctx.buf("attn_qkv32", (T, self.w_qkv.shape[0]), torch.float32), *self.norm_w,
-                                       self.qk_norm_eps, meta.slots if write_cache else None, q, cache.k, cache.v, gates, self.H, G,
-                                       self.d, self.dv)
+                                       self.qk_norm_eps, slots, q, k, v, gates, self.H, G, self.d, self.dv)
+            self._kv_to_8bits(T, k, v, cache, meta, slots)
         return self._softmax_attention(ctx, q, cache, meta), gates
 
     def _softmax_attention(self, ctx, q, cache, meta):
         att = ctx.buf("attn_out", (q.shape[0], self.OD), q.dtype)
+        if cache.kv8 is not None:
+            # (all that lies before the step's tokens was written by earlier steps)
+            with kernels.phase("attn"):
+                kernels.paged_attention_kv8(q, cache.kv8, meta, ctx, self.H, self.G, self.d, self.mask, self.scale, att,
+                                            tiles=ctx.arrays(self.step_arrays_key()), settled=True, sinks=self.sinks, zero_sink=self.sink == "zero",
+                                            slopes=self.slopes, head_scales=self.head_scales, softcap=self.softcap)
+            return att
         with kernels.phase("attn"):
             kernels.paged_attention(q, cache.k, None if self.values_are_keys else cache.v, meta, ctx, self.H, self.G, self.d,
                                     self.mask, self.scale, att, tiles=ctx.arrays(self.step_arrays_key()), dv=self.dv,
                                     values_in_keys=self.values_are_keys, sinks=self.sinks, zero_sink=self.sink == "zero",
                                     slopes=self.slopes, head_scales=self.head_scales, softcap=self.softcap)
         return att
+
+    def _kv_places(self, ctx, T, G, cache, meta, write_cache):
+        """Where a tail that makes keys and values puts them: the cache at the step's slots, or, in front of a cache in 8 bits, rows of
+        the step's own, one behind the other."""
+        if cache.kv8 is None:
+            return cache.k, None if self.values_are_keys else cache.v, meta.slots if write_cache else None
+        shape = (T, 1, max(G, 1), self.d)
+        k, v = (ctx.buf(name, shape, ctx.run_dtype) for name in ("attn_new_k", "attn_new_v"))
+        return k, v, ctx.engine.places(T) if write_cache else None
+
+    def _kv_to_8bits(self, T, k, v, cache, meta, slots):
+        if cache.kv8 is not None and slots is not None:
+            kernels.kv8_write(k.view(T, self.KD), v.view(T, self.KD), meta.slots, cache.kv8, self.G, self.d, meta.block_size)
 
     def _attend(self, ctx, xn, cache, write_cache):
         T = xn.shape[0]
@@ -356,10 +387,17 @@ class PagedAttention(OutputProduct, Mixer):
                 first = ctx.buf(self.V_FIRST, (T, self.VD), torch.float32)
                 mix = (first, 1 if self.v_mix == "first" else 2, self.v_lambda)
             with kernels.phase("qkv"):
-                kernels.linear_rope_norm_kv(xn, self.w_qkv, self.b_qkv, qkv, cos_sin, n_rot, ctx.positions,
-                                            meta.slots if write_cache else None, q, cache.k, None if self.values_are_keys else cache.v,
+                k, v, slots = self._kv_places(ctx, T, G, cache, meta, write_cache)
+                kernels.linear_rope_norm_kv(xn, self.w_qkv, self.b_qkv, qkv, cos_sin, n_rot, ctx.positions, slots, q, k, v,
                                             self.H, G, self.d, dv_row, self.qk_norm_eps, norm_weights=self.norm_w, value_mix=mix,
                                             pairing=self.pairing)
+                self._kv_to_8bits(T, k, v, cache, meta, slots)
+        elif cache.kv8 is not None:
+            qkv = ctx.buf("attn_qkv", (T, self.QD + 2 * self.KD), xn.dtype)
+            with kernels.phase("qkv"):
+                kernels.linear(xn, self.w_qkv, self.b_qkv, qkv, accumulate=False)
+                kernels.rope_kv8_write(qkv, cos_sin, n_rot, ctx.positions, meta.slots if write_cache else None, q, cache.kv8, self.H, self.G, self.d,
+                                       meta.block_size)
         else:
             qkv = ctx.buf("attn_qkv", (T, self.QD + 2 * self.KD), xn.dtype)
             with kernels.phase("qkv"):

@@ -162,6 +162,9 @@ class PositionEncoding(Part):
 
 
 class Mixer(Part):
+    # whether this mixer also runs on a cache in 8 bits (``LayerCache.kv8``)
+    caches_eight_bits = False
+
     def cache_spec(self) -> Optional[CacheSpec]:
         return None
 
