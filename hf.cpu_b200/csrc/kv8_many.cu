@@ -1,0 +1,587 @@
+// Attention of prompt portions over the key/value cache in 8 bits (kv8.cuh) on tcgen05: bfloat16, head sizes 64 and 128, pages of 8..64
+// tokens, two tiles of 128 query rows a CTA.
+//
+// s_j = scale (q . code_j) ks_j, out = sum_j p_j vs_j code'_j / sum_j p_j.  The exponentials bound it (128 x 128 of them for every pair of
+// products of 128 x 128 x d), so nothing of the 8 bits is left to the threads that compute them but two factors:
+// * two warps of their own turn codes into float16 (exact: whole numbers below 2^11) in the layout of the tensor core's operands, 64 keys
+//   each of a tile of 128, while the softmax of the tile before runs.  Each fetches its half's codes itself, by bulk copies as soon as it
+//   has read the last ones, keys and values each into their own staging buffer: a tile's keys are on their way while its predecessor's
+//   values still wait for their place.
+// * the scales stay out of the operands: a score is multiplied by its key's, a weight by its value's, in float32, both read as
+//   broadcasts from shared memory.
+// * queries are multiplied by the power of two that brings a row's largest number to 2^14..2^15 (kv8_few.cu).
+// * a row's exponentials refer to R = (largest score) + log2(largest value scale) - 10: 2^(s - R) vs is at most 2^14 before R is raised, and
+//   is rounded once to float16.  Both sums carry the factor, which cancels.  R is raised, and the sums so far rescaled (the output in
+//   TMEM), only when it has been outgrown by 2^4.  (log2 of the scale is taken as -90 at least: smaller values are zeros.)
+// * a row belongs to one thread, which reads its scores from TMEM twice, 32 at a time, for the maximum and for the weights (128 at once
+//   beside their scales do not fit the registers of twelve warps); O lives in TMEM; one tile's softmax runs beside the other's products.
+// Barrier waits are bounded (HFB_ERR_WAIT, TMEM freed; tc_ptx.cuh).
+#include <cuda_fp16.h>
+
+#include "kv8.cuh"
+#include "tc_ptx.cuh"
+
+static thread_local cudaError_t g_launch_err = cudaSuccess;      // what the last launch_pdl returned
+
+namespace hfb {
+int *error_word();
+
+constexpr int KM_ROWS = 128, KM_KEYS = 128, KM_THREADS = 384, KM_TMEM_COLS = 512;
+constexpr uint32_t KM_SUB = 128 * 64 * 2;           // one swizzled sub-tile: 128 rows of 64 float16
+constexpr uint32_t KM_TILE = 2 * KM_SUB;            // a [128 x 128] operand (P)
+
+struct Kv8ManyParams {
+    Kv8Params a;
+    int per, n_tiles, settled;                       // tokens per query tile, double tiles in all
+};
+
+template <int D> constexpr uint32_t km_smem() { return 2 * KM_TILE + 4 * (D / 64) * KM_SUB + 2 * KM_KEYS * D + 2048 + 256; }
+
+__device__ __forceinline__ uint32_t km_off(int row, int c16)
+{
+    return (uint32_t)(c16 >> 3) * KM_SUB + (uint32_t)row * 128u + (uint32_t)(((c16 & 7) ^ (row & 7)) << 4);
+}
+__device__ __forceinline__ uint32_t km_codes(uint32_t w, uint32_t selector)
+{
+    uint32_t r;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(w), "r"(0x64646464u), "r"(selector));
+    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(r) : "r"(0x64806480u));                // 1024 + byte - 1152
+    return r;
+}
+__device__ __forceinline__ uint32_t km_pack(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float km_ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void km_st16(uint32_t taddr, const uint32_t *v)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+                   "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
+}
+__device__ __forceinline__ void km_store16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d)
+{
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ float4 km_load4(uint32_t addr)
+{
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ float km_load1(uint32_t addr)
+{
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ void km_bulk(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+template <int D>
+__global__ void __launch_bounds__(KM_THREADS, 1)
+kv8_many_kernel(Kv8ManyParams f, int *err)
+{
+    const Kv8Params &p = f.a;
+    extern __shared__ __align__(1024) uint8_t km_raw[];
+    const uint32_t base = (smem_u32(km_raw) + 1023u) & ~1023u;
+    uint8_t *gen = km_raw + (base - smem_u32(km_raw));
+    constexpr uint32_t HT = (D / 64) * KM_SUB;       // a [128 x D] float16 operand: Q, K or V
+    constexpr uint32_t CODES = KM_KEYS * D;          // a tile's key (or value) codes
+    const uint32_t sQ = base, sK = base + 2 * HT, sV = base + 3 * HT, sP = base + 4 * HT, stK = sP + 2 * KM_TILE, stV = stK + CODES;
+    const uint32_t sS = stV + CODES;                 // [2][keys' scales 128 | values' scales 128]
+    const uint32_t bars = sS + 2048;
+    const uint32_t q_ready = bars, s_full = bars + 16, p_ready = bars + 32, pv_done = bars + 48, s_free = bars + 64;       // + 8 * query tile
+    const uint32_t k_st_full = bars + 80, v_st_full = bars + 96;                                                          // + 8 * half
+    const uint32_t k_full = bars + 112, k_empty = bars + 120, v_full = bars + 128, v_empty = bars + 136;
+    const uint32_t sc_full = bars + 144, sc_empty = bars + 160;                                                           // + 8 * buffer
+    volatile uint32_t *tmem_slot = (volatile uint32_t *)(gen + (bars - base) + 192);
+    volatile int *abort_flag = (volatile int *)(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (base - smem_u32(km_raw) > (D == 128 ? 768u : 1024u)) {           // (see the launch)
+        if (threadIdx.x == 0) atomicOr(err, HFB_ERR_WAIT);
+        return;
+    }
+    if (!f.settled) pdl_wait();                      // nothing is read that the kernels in front may still write
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; i++) {
+            mbar_init(q_ready + 8 * i, 4); mbar_init(s_full + 8 * i, 1); mbar_init(p_ready + 8 * i, 4); mbar_init(pv_done + 8 * i, 1);
+            mbar_init(s_free + 8 * i, 4); mbar_init(sc_full + 8 * i, 2); mbar_init(sc_empty + 8 * i, 8);
+        }
+        for (int i = 0; i < 2; i++) { mbar_init(k_st_full + 8 * i, 1); mbar_init(v_st_full + 8 * i, 1); }
+        mbar_init(k_full, 2); mbar_init(v_full, 2); mbar_init(k_empty, 1); mbar_init(v_empty, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32((const void *)tmem_slot)), "r"(KM_TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    if (f.settled) pdl_wait();
+    pdl_trigger();
+
+    // Work items are (double tile, key/value head), heaviest first; the rounds run over the CTAs forwards and backwards in turn.
+    const int r = p.H / p.G, bs = p.block_size, pages = KM_KEYS / bs;
+    const int n_items = f.n_tiles * p.G, n_ctas = gridDim.x;
+    struct Item { int g, seq, t0, nt0, nt1, pos_last, lo_first, kt_lo, n_kt0, n_kt1, n_kt; };
+    auto item_of = [&](int round, Item &it) -> bool {
+        const int idx = round * n_ctas + ((round & 1) ? n_ctas - 1 - (int)blockIdx.x : (int)blockIdx.x);
+        if (idx >= n_items) return false;
+        const int tile = f.n_tiles - 1 - idx / p.G;
+        it.g = idx % p.G;
+        it.seq = p.tile_seq[tile]; it.t0 = p.tile_t0[tile];
+        const int nt = max(1, min(p.tile_nt[tile], 2 * f.per));
+        it.nt0 = min(nt, f.per); it.nt1 = nt - it.nt0;                  // tokens of the two query tiles
+        const int pos_last0 = p.positions[it.t0 + it.nt0 - 1];
+        it.pos_last = p.positions[it.t0 + nt - 1];
+        it.lo_first = mask_lo(p.positions[it.t0], p.window);
+        it.kt_lo = it.lo_first / KM_KEYS;
+        it.n_kt0 = max(1, pos_last0 / KM_KEYS + 1 - it.kt_lo);
+        it.n_kt1 = it.nt1 > 0 ? max(1, it.pos_last / KM_KEYS + 1 - it.kt_lo) : 0;
+        it.n_kt = max(it.n_kt0, it.n_kt1);
+        return true;
+    };
+    const int n_rounds = (n_items + n_ctas - 1) / n_ctas;
+
+    if (warp == 0 || warp == 1) {
+        if (warp == 1 && lane == 0) {
+            // ---- tensor-core issue ------------------------------------------------------------------------------------------------
+            constexpr uint32_t F16 = (1u << 7) | (1u << 10);             // (the operands' type bits of bfloat16: clear for float16)
+            constexpr uint32_t idesc_s = bf16_idesc(KM_ROWS, KM_KEYS, false) & ~F16, idesc_pv = bf16_idesc(KM_ROWS, D, true) & ~F16;
+            const uint32_t tS0 = tmem_base, tO0 = tmem_base + 256;
+            const uint64_t dq = sw128_desc(sQ), dk = sw128_desc(sK), dp = sw128_desc(sP), dv = sw128_desc_mn(sV, KM_SUB);
+            auto issue_s = [&](int i) {
+#pragma unroll
+                for (int kk = 0; kk < D / 16; kk++) {
+                    const uint64_t o = ((uint32_t)(kk >> 2) * KM_SUB + (uint32_t)(kk & 3) * 32u) >> 4;
+                    tc_mma_bf16(tS0 + i * 128, dq + o + (uint64_t)i * (HT >> 4), dk + o, idesc_s, kk > 0 ? 1u : 0u);
+                }
+                tc_commit(s_full + 8 * i);
+            };
+            auto issue_pv = [&](int i, bool accumulate) {
+#pragma unroll
+                for (int kk = 0; kk < KM_KEYS / 16; kk++) {
+                    const uint64_t o = ((uint32_t)(kk >> 2) * KM_SUB + (uint32_t)(kk & 3) * 32u) >> 4;
+                    tc_mma_bf16(tO0 + i * D, dp + o + (uint64_t)i * (KM_TILE >> 4), dv + (uint64_t)kk * (2048u >> 4), idesc_pv, (accumulate || kk > 0) ? 1u : 0u);
+                }
+                tc_commit(pv_done + 8 * i);
+            };
+            bool ok = true;
+            uint32_t gs = 0, g_tile0 = 0, g_tile1 = 0, q_uses0 = 0, q_uses1 = 0;      // steps so far, per query tile, and items per query tile
+            for (int round = 0; round < n_rounds && ok; round++) {
+                Item it;
+                if (!item_of(round, it)) continue;
+                ok = mbar_wait(q_ready, q_uses0++ & 1, abort_flag, err);
+                if (ok && it.n_kt1 > 0) ok = mbar_wait(q_ready + 8, q_uses1++ & 1, abort_flag, err);
+                if (ok) ok = mbar_wait(k_full, gs & 1, abort_flag, err);
+                if (ok) {
+                    tc_fence_after();
+                    issue_s(0);
+                    if (it.n_kt1 > 0) issue_s(1);
+                    tc_commit(k_empty);
+                }
+                for (int j = 0; j < it.n_kt && ok; j++, gs++) {
+                    // per query tile: the scores of step j + 1 as soon as those of step j have been read for the last time, then the
+                    // outputs of step j, whose last weights follow shortly
+                    const bool more = j + 1 < it.n_kt;
+                    if (more) ok = mbar_wait(k_full, (gs + 1) & 1, abort_flag, err);
+                    if (ok) ok = mbar_wait(v_full, gs & 1, abort_flag, err);
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const int n = i ? it.n_kt1 : it.n_kt0;
+                        const uint32_t ph = ((i ? g_tile1 : g_tile0) + j) & 1;
+                        if (ok && j + 1 < n) {
+                            ok = mbar_wait(s_free + 8 * i, ph, abort_flag, err);
+                            if (ok) { tc_fence_after(); issue_s(i); }
+                        }
+                        if (ok && more && i == 1) tc_commit(k_empty);
+                        if (ok && j < n) {
+                            ok = mbar_wait(p_ready + 8 * i, ph, abort_flag, err);
+                            if (ok) { tc_fence_after(); issue_pv(i, j > 0); }
+                        }
+                    }
+                    if (!ok) break;
+                    tc_commit(v_empty);
+                }
+                g_tile0 += it.n_kt0; g_tile1 += it.n_kt1;
+            }
+            // nothing of this CTA's is in flight once the last release of V has landed
+            if (ok && gs > 0) mbar_wait(v_empty, (gs - 1) & 1, abort_flag, err);
+        }
+    } else if (warp < 4) {
+        // ---- codes into operands: a warp has one half of a tile's keys, a lane two of them ----------------------------------------
+        const int half = warp - 2, half_pages = 64 / bs;
+        const uint32_t page_bytes = bs * D, k_in = k_st_full + 8 * half, v_in = v_st_full + 8 * half, half_at = (uint32_t)half * 64 * D;
+        auto convert = [&](uint32_t from, uint32_t to) {
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int row = half * 64 + 32 * u + lane;
+                uint4 w[D / 16];
+#pragma unroll
+                for (int c = 0; c < D / 16; c++)
+                    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[c].x), "=r"(w[c].y), "=r"(w[c].z), "=r"(w[c].w)
+                                 : "r"(from + (uint32_t)row * D + (uint32_t)kv8_piece(row % bs, c, D) * 16u));
+#pragma unroll
+                for (int c = 0; c < D / 16; c++) {
+                    km_store16(to + km_off(row, 2 * c), km_codes(w[c].x, 0x4140), km_codes(w[c].x, 0x4342), km_codes(w[c].y, 0x4140), km_codes(w[c].y, 0x4342));
+                    km_store16(to + km_off(row, 2 * c + 1), km_codes(w[c].z, 0x4140), km_codes(w[c].z, 0x4342), km_codes(w[c].w, 0x4140), km_codes(w[c].w, 0x4342));
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (also: the staging has been read before it is written again)
+            __syncwarp();
+        };
+        bool ok = true;
+        uint32_t gs = 0;                                                  // steps of the items before
+        for (int round = 0; round < n_rounds && ok; round++) {
+            Item it;
+            if (!item_of(round, it)) continue;
+            const int32_t *table = p.block_table + (size_t)it.seq * p.max_blocks;
+            // the page of step j that this lane asks for, -1 where there is none to be read
+            auto page_of = [&](int j) {
+                const int key0 = (it.kt_lo + j) * KM_KEYS + half * 64 + lane * bs, blk = key0 / bs;
+                if (j >= it.n_kt || lane >= half_pages || key0 > it.pos_last || key0 + bs <= it.lo_first) return -1;
+                const int page = blk < p.max_blocks ? table[blk] : -1;
+                if (page < 0 || page >= p.num_pages) { atomicOr(err, HFB_ERR_PAGE); return -1; }
+                return page;
+            };
+            auto fetch = [&](int page, uint32_t bar, uint32_t dst, uint32_t skip) {
+                const int n = __popc(__ballot_sync(0xffffffffu, page >= 0));
+                if (lane == 0) mbar_arrive_expect_tx(bar, n * page_bytes);
+                __syncwarp();
+                if (page >= 0) km_bulk(dst + half_at + lane * page_bytes, p.cache + ((size_t)page * p.G + it.g) * p.record + skip, page_bytes, bar);
+            };
+            // a key's scales; where it is not to be read (behind the last, passed by every row's mask, no page) 0 and -1
+            auto scales_of = [&](int j, int page, int u) {
+                const int in_half = 32 * u + lane, key = (it.kt_lo + j) * KM_KEYS + half * 64 + in_half;
+                const int its = __shfl_sync(0xffffffffu, page, in_half / bs);
+                if (its < 0 || key > it.pos_last || key < it.lo_first) return make_float2(0.f, -1.f);
+                const float *s = (const float *)(p.cache + ((size_t)its * p.G + it.g) * p.record + 2 * bs * D) + in_half % bs;
+                return make_float2(s[0], s[bs]);
+            };
+            int page = page_of(0);
+            fetch(page, k_in, stK, 0);
+            fetch(page, v_in, stV, page_bytes);
+            float2 sc0 = scales_of(0, page, 0), sc1 = scales_of(0, page, 1);
+            int next = page_of(1);                                        // the pages of step j + 1; `page`: of step j
+            for (int j = 0; j <= it.n_kt && ok; j++) {
+                // keys of step j, then values of step j - 1: the keys' place is free early in a step, the values' at its end
+                if (j < it.n_kt) {
+                    const uint32_t g = gs + j, b = g & 1, at = sS + b * 1024u + 4u * (half * 64 + lane);
+                    ok = mbar_wait(sc_empty + 8 * b, ((g >> 1) & 1) ^ 1, abort_flag, err);
+                    if (!ok) break;
+                    asm volatile("st.shared.f32 [%0], %1;\n\tst.shared.f32 [%0 + 512], %2;\n\tst.shared.f32 [%0 + 128], %3;\n\tst.shared.f32 [%0 + 640], %4;"
+                                 ::"r"(at), "f"(sc0.x), "f"(sc0.y), "f"(sc1.x), "f"(sc1.y) : "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(sc_full + 8 * b);
+                    ok = mbar_wait(k_in, g & 1, abort_flag, err) && mbar_wait(k_empty, (g & 1) ^ 1, abort_flag, err);
+                    if (!ok) break;
+                    convert(stK, sK);
+                    if (lane == 0) mbar_arrive(k_full);
+                    if (j + 1 < it.n_kt) {
+                        fetch(next, k_in, stK, 0);
+                        sc0 = scales_of(j + 1, next, 0);
+                        sc1 = scales_of(j + 1, next, 1);
+                    }
+                }
+                if (j > 0) {
+                    const uint32_t g = gs + j - 1;
+                    ok = mbar_wait(v_in, g & 1, abort_flag, err) && mbar_wait(v_empty, (g & 1) ^ 1, abort_flag, err);
+                    if (!ok) break;
+                    convert(stV, sV);
+                    if (lane == 0) mbar_arrive(v_full);
+                    if (j < it.n_kt) fetch(page, v_in, stV, page_bytes);
+                }
+                page = next;
+                next = page_of(j + 2);
+            }
+            gs += it.n_kt;
+        }
+    } else {
+        // ---- softmax and output: one thread per row -------------------------------------------------------------------------------
+        const float log2e = 1.4426950408889634f;
+        const int i = (warp - 4) >> 2;                                   // query tile
+        const int row = (warp & 3) * 32 + lane;                          // TMEM lane = row; a warp reads its own quarter
+        const int tl = row / r, hl = row % r;
+        const uint32_t lane_base = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t tS = lane_base + i * 128, tO = lane_base + 256 + i * D;
+        uint32_t g_mine = 0, gs = 0;                                     // this query tile's steps so far, and the item's
+        bool ok = true;
+        for (int round = 0; round < n_rounds && ok; round++) {
+            Item it;
+            if (!item_of(round, it)) continue;
+            const int n_mine = i ? it.n_kt1 : it.n_kt0, nt_mine = i ? it.nt1 : it.nt0, t_first = it.t0 + i * f.per;
+            const bool valid = tl < nt_mine;
+            const size_t th = ((size_t)(t_first + (valid ? tl : 0)) * p.H + it.g * r + hl) * D;
+            float unit = 0.f;                                            // from a product's sum to a score in the exponent's base 2
+            if (n_mine > 0) {
+                // the tile's products of the item before are done (their scores have all been waited for)
+                const uint4 *src = (const uint4 *)((const __nv_bfloat16 *)p.q + th);
+                uint4 raw[D / 8];
+                unsigned top = 0;
+#pragma unroll
+                for (int c = 0; c < D / 8; c++) {
+                    raw[c] = valid ? src[c] : make_uint4(0, 0, 0, 0);
+                    const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+#pragma unroll
+                    for (int u = 0; u < 4; u++) top = max(top, max(w[u] & 0x7fffu, (w[u] >> 16) & 0x7fffu));
+                }
+                const unsigned field = min(268u - (top >> 7), 253u);
+                const float by = __uint_as_float(field << 23);
+                unit = p.scale * log2e * __uint_as_float((254u - field) << 23);
+#pragma unroll
+                for (int c = 0; c < D / 8; c++) {
+                    const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+                    uint32_t h[4];
+#pragma unroll
+                    for (int u = 0; u < 4; u++) h[u] = km_pack(__uint_as_float(w[u] << 16) * by, __uint_as_float(w[u] & 0xffff0000u) * by);
+                    km_store16(sQ + i * HT + km_off(row, c), h[0], h[1], h[2], h[3]);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(q_ready + 8 * i);
+            }
+            const int pos = valid ? p.positions[t_first + tl] : -1;
+            const int lo = mask_lo(pos, p.window);
+            const float slope2 = (p.slopes && valid) ? p.slopes[it.g * r + hl] * log2e : 0.f;
+            const float hscale = (p.head_scales && valid) ? p.head_scales[it.g * r + hl] : 1.f;
+            const bool capped = p.softcap > 0.f, finished = capped || p.slopes || p.head_scales;     // (scores are finished in place)
+            const float cap_in = capped ? unit * hscale / (p.softcap * log2e) : 0.f, cap2 = p.softcap * log2e;
+            float ref = -INFINITY, l = 0.f, vm = 0.f;                    // what the exponentials refer to, their sum, largest scale so far
+            for (int j = 0; j < it.n_kt && ok; j++) {
+                const uint32_t b = (gs + j) & 1, sc_ph = ((gs + j) >> 1) & 1, s_at = sS + b * 1024u;
+                if (!mbar_wait(sc_full + 8 * b, sc_ph, abort_flag, err)) { ok = false; break; }
+                if (j >= n_mine) {                                       // (the other query tile's step)
+                    if (lane == 0) mbar_arrive(sc_empty + 8 * b);
+                    continue;
+                }
+                const uint32_t ph = (g_mine + j) & 1;
+                const int key0 = (it.kt_lo + j) * KM_KEYS;
+                {
+                    const float4 v = km_load4(s_at + 512u + 16u * lane);
+                    vm = fmaxf(vm, warp_max(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w))));
+                }
+                if (!mbar_wait(s_full + 8 * i, ph, abort_flag, err)) { ok = false; break; }
+                tc_fence_after();
+                // (rows beyond the tile's tokens go with the rows that see every key); a missing page's values have the scale -1
+                bool gap = false;
+                if (lane < pages) gap = km_load1(s_at + 512u + 4u * (lane * bs + bs - 1)) == -1.f;
+                gap = __any_sync(0xffffffffu, gap);
+                const bool all_visible = (!valid && !gap) || (key0 + KM_KEYS - 1 <= pos && key0 >= lo && !gap);
+                const float b0 = slope2 * (float)(key0 - pos), by_head = unit * hscale, sc = finished ? 1.f : unit;
+                // 32 scores from TMEM with their keys' scales, options and masks; what they lack is the factor sc > 0
+                auto scores = [&](int c0, f32pair (&x)[16]) {
+                    uint32_t raw[32];
+                    __syncwarp();
+                    tmem_ld16(tS + c0, raw);
+                    tmem_ld16(tS + c0 + 16, raw + 16);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int c = 0; c < 32; c += 4) {
+                        const float4 k = km_load4(s_at + 4u * (c0 + c));
+                        x[c / 2] = mul2(pair_of(__uint_as_float(raw[c]), __uint_as_float(raw[c + 1])), pair_of(k.x, k.y));
+                        x[c / 2 + 1] = mul2(pair_of(__uint_as_float(raw[c + 2]), __uint_as_float(raw[c + 3])), pair_of(k.z, k.w));
+                    }
+                    if (finished) {
+#pragma unroll
+                        for (int c = 0; c < 32; c += 2) {
+                            float2 v = halves(x[c / 2]);
+                            const float s0 = fmaf(slope2, (float)(c0 + c), b0), s1 = fmaf(slope2, (float)(c0 + c + 1), b0);
+                            v.x = capped ? fmaf(cap2, tanh_fast(v.x * cap_in), s0) : fmaf(v.x, by_head, s0);
+                            v.y = capped ? fmaf(cap2, tanh_fast(v.y * cap_in), s1) : fmaf(v.y, by_head, s1);
+                            x[c / 2] = pair_of(v.x, v.y);
+                        }
+                    }
+                    if (!all_visible) {
+#pragma unroll
+                        for (int c = 0; c < 32; c += 2) {
+                            float2 v = halves(x[c / 2]);
+                            const int key = key0 + c0 + c;
+                            if (!(valid && key >= lo && key <= pos) || (gap && km_load1(s_at + 512u + 4u * (c0 + c)) == -1.f)) v.x = -INFINITY;
+                            if (!(valid && key + 1 >= lo && key + 1 <= pos) || (gap && km_load1(s_at + 516u + 4u * (c0 + c)) == -1.f)) v.y = -INFINITY;
+                            x[c / 2] = pair_of(v.x, v.y);
+                        }
+                    }
+                };
+                float mx = -INFINITY;
+#pragma unroll 1
+                for (int c0 = 0; c0 < 128; c0 += 32) {
+                    f32pair x[16];
+                    scores(c0, x);
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int c = 0; c < 16; c++) { const float2 v = halves(x[c]); top[c & 3] = fmaxf(top[c & 3], fmaxf(v.x, v.y)); }
+                    mx = fmaxf(mx, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+                }
+                mx = mx * sc + log2f(fmaxf(vm, 8.0779357e-28f)) - 10.f;  // (2^-90)
+                float corr = 1.f;
+                if (mx > ref + 4.f || (ref == -INFINITY && mx > -INFINITY)) {
+                    corr = ref == -INFINITY ? 0.f : km_ex2(ref - mx);
+                    ref = mx;
+                }
+                if (j > 0) {
+                    // P of the step before has been used, and O holds everything up to it
+                    if (!mbar_wait(pv_done + 8 * i, ph ^ 1, abort_flag, err)) { ok = false; break; }
+                    tc_fence_after();
+                    if (__any_sync(0xffffffffu, corr != 1.f)) {
+#pragma unroll 1
+                        for (int c = 0; c < D / 16; c++) {
+                            uint32_t ov[16];
+                            tmem_ld16(tO + 16 * c, ov);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 16; e++) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * corr);
+                            km_st16(tO + 16 * c, ov);
+                        }
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    }
+                }
+                const float minus = ref == -INFINITY ? 0.f : -ref;
+                const f32pair sc2 = pair_of(sc, sc), minus2 = pair_of(minus, minus), one2 = pair_of(1.f, 1.f);
+                f32pair sum[2] = {pair_of(0.f, 0.f), pair_of(0.f, 0.f)};
+#pragma unroll 1
+                for (int c0 = 0; c0 < 128; c0 += 32) {
+                    f32pair x[16];
+                    scores(c0, x);
+                    if (c0 == 96) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(s_free + 8 * i);      // the tensor core may write the next scores
+                    }
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int c = 0; c < 16; c += 2) {
+                        const float4 v = km_load4(s_at + 512u + 4u * (c0 + 2 * c));
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            const float2 a = halves(fma2(x[c + u], sc2, minus2));
+                            const f32pair e = pair_of(km_ex2(a.x), km_ex2(a.y));
+                            sum[u] = fma2(e, one2, sum[u]);
+                            float2 w = halves(mul2(e, u ? pair_of(v.z, v.w) : pair_of(v.x, v.y)));
+                            if (!all_visible) {                          // (a value that is no number, for a row that does not see it)
+                                const float2 s = halves(x[c + u]);
+                                if (s.x == -INFINITY) w.x = 0.f;
+                                if (s.y == -INFINITY) w.y = 0.f;
+                            }
+                            pk[c + u] = km_pack(w.x, w.y);
+                        }
+                    }
+#pragma unroll
+                    for (int q = 0; q < 4; q++) km_store16(sP + i * KM_TILE + km_off(row, c0 / 8 + q), pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
+                }
+                {
+                    const float2 s0 = halves(sum[0]), s1 = halves(sum[1]);
+                    l = l * corr + ((s0.x + s0.y) + (s1.x + s1.y));
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) { mbar_arrive(sc_empty + 8 * b); mbar_arrive(p_ready + 8 * i); }
+            }
+            gs += it.n_kt;
+            g_mine += n_mine;
+            if (ok && n_mine > 0) ok = mbar_wait(pv_done + 8 * i, (g_mine - 1) & 1, abort_flag, err);
+            if (ok && n_mine > 0) {
+                tc_fence_after();
+                if (p.sinks || p.zero_sink) {
+                    // the sink: one more term of the sum, in the scale of the row's reference
+                    const float sk = p.sinks ? p.sinks[it.g * r + hl] * log2e : 0.f;
+                    l += exp2f(sk - (ref == -INFINITY ? 0.f : ref));
+                }
+                const float inv = l == 0.f ? 0.f : 1.0f / l;
+                uint4 *dst = (uint4 *)((__nv_bfloat16 *)p.out + th);
+#pragma unroll 1
+                for (int c = 0; c < D / 16; c += 4) {                    // four reads of 16 columns under way together
+                    uint32_t ov[64];
+#pragma unroll
+                    for (int u = 0; u < 4; u++) tmem_ld16(tO + 16 * (c + u), ov + 16 * u);   // all lanes take part, valid row or not
+                    tmem_wait_ld();
+                    if (valid) {
+#pragma unroll
+                        for (int u = 0; u < 4; u++) {
+                            __nv_bfloat162 h[8];
+#pragma unroll
+                            for (int e = 0; e < 8; e++)
+                                h[e] = __floats2bfloat162_rn(__uint_as_float(ov[16 * u + 2 * e]) * inv, __uint_as_float(ov[16 * u + 2 * e + 1]) * inv);
+                            dst[2 * (c + u)] = *(uint4 *)&h[0];
+                            dst[2 * (c + u) + 1] = *(uint4 *)&h[4];
+                        }
+                    }
+                }
+                tc_fence_before();
+            }
+        }
+    }
+
+    // ---- teardown -------------------------------------------------------------------------------------------------------------------
+    tc_fence_before();
+    __syncthreads();
+    if (*abort_flag && threadIdx.x == 0) {
+        for (int i = 0; i < 2000; i++) __nanosleep(1000);              // let copies still in flight land
+    }
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(KM_TMEM_COLS) : "memory");
+    }
+}
+
+template <int D>
+static int launch_kv8_many(const Kv8ManyParams &f, int grid, cudaStream_t st)
+{
+    constexpr uint32_t smem = km_smem<D>() + (D == 128 ? 768 : 1024);    // (the tiles begin on a multiple of 1,024; shared memory does after the first)
+    static_assert(smem <= 227 * 1024, "the tiles do not fit");
+    static bool configured[64] = {false};                                // (the opt-in is a property of the function on one device)
+    if (!configured[current_device()]) {
+        cudaError_t e = cudaFuncSetAttribute(kv8_many_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return fail(HFB_ECUDA, "kv8_attention_many: cannot opt in to %u bytes of shared memory: %s", smem, cudaGetErrorString(e));
+        configured[current_device()] = true;
+    }
+    g_launch_err = launch_pdl(kv8_many_kernel<D>, dim3(grid), dim3(KM_THREADS), smem, st, f, error_word());
+    return check_pdl_launch(g_launch_err, "kv8_attention_many");
+}
+
+}  // namespace hfb
+
+using namespace hfb;
+
+extern "C" int hfb_kv8_attention_many(const void *q, const void *cache, const int32_t *block_table, int max_blocks, const int32_t *positions,
+                                      const int32_t *tile_seq, const int32_t *tile_t0, const int32_t *tile_nt, int n_tiles, int settled, int block_size,
+                                      int64_t num_pages, int window, float scale, void *out, int H, int G, int d, const float *sinks, int zero_sink,
+                                      const float *slopes, const float *head_scales, float softcap, hfb_stream s)
+{
+    if (n_tiles <= 0) return HFB_OK;
+    if (d != 64 && d != 128) return fail(HFB_ENOTSUP, "kv8_attention_many: head size %d (64 and 128 only)", d);
+    if (H <= 0 || G <= 0 || H % G || H / G > KM_ROWS || max_blocks <= 0 || num_pages < 0)
+        return fail(HFB_EINVAL, "kv8_attention_many: bad arguments (H=%d G=%d)", H, G);
+    if (block_size < 8 || block_size > 64 || 64 % block_size) return fail(HFB_ENOTSUP, "kv8_attention_many: pages of %d tokens (8, 16, 32 and 64)", block_size);
+    if (!(scale > 0.f)) return fail(HFB_ENOTSUP, "kv8_attention_many: the factor on the scores must be positive");
+    if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache) & 15) return fail(HFB_EINVAL, "kv8_attention_many: misaligned arrays");
+    Kv8ManyParams f = {};
+    f.a.q = q; f.a.cache = (const uint8_t *)cache; f.a.out = out; f.a.block_table = block_table; f.a.positions = positions;
+    f.a.tile_seq = tile_seq; f.a.tile_t0 = tile_t0; f.a.tile_nt = tile_nt; f.a.max_blocks = max_blocks; f.a.block_size = block_size;
+    f.a.record = kv8_record_bytes(block_size, d); f.a.window = window; f.a.H = H; f.a.G = G; f.a.num_pages = num_pages; f.a.scale = scale;
+    f.a.sinks = sinks; f.a.slopes = slopes; f.a.head_scales = head_scales; f.a.zero_sink = zero_sink; f.a.softcap = softcap > 0.f ? softcap : 0.f;
+    f.per = KM_ROWS / (H / G); f.n_tiles = n_tiles; f.settled = settled;
+    int sms = 0, dev = 0;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    const long long items = (long long)n_tiles * G;
+    const int grid = (int)(items < sms ? items : (sms > 0 ? sms : 1));
+    return d == 128 ? launch_kv8_many<128>(f, grid, (cudaStream_t)s) : launch_kv8_many<64>(f, grid, (cudaStream_t)s);
+}

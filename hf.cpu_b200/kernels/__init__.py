@@ -402,20 +402,28 @@ def kv8_head_groups(heads_per_group: int) -> int:
     return next(s for s in range(1, heads_per_group + 1) if heads_per_group <= 16 * s and heads_per_group % s == 0)
 
 
+KV8_MANY = 64               # query rows (tokens times heads on a key/value head) of a request from which its portion is a prompt's
+
+
 def kv8_step_arrays(q_lens, heads_per_group: int):
-    """Tile lists of a step's tokens for :func:`paged_attention_kv8`, as named int32 arrays: a tile is up to ``few.nt`` consecutive tokens of
-    request ``few.seq`` from token ``few.t0`` of the step on, with their heads at most 16 places."""
+    """Tile lists of a step's tokens for :func:`paged_attention_kv8`, as named int32 arrays: a tile is ``nt`` consecutive tokens of request
+    ``seq`` from token ``t0`` of the step on.  "few": up to 16 (token, head) places of requests that bring few tokens; "many": two tiles
+    of 128 rows of those that bring more."""
     import numpy as np
     q = np.asarray(q_lens, dtype=np.int32)
-    share = kv8_head_groups(heads_per_group)
-    per = 1 if share > 1 else max(1, 16 // heads_per_group)
-    if int(q.max()) == 1:
-        return {"few.seq": np.arange(len(q), dtype=np.int32), "few.t0": np.arange(len(q), dtype=np.int32), "few.nt": np.ones(len(q), dtype=np.int32)}
-    tiles = -(-q // per)
-    seq = np.repeat(np.arange(len(q), dtype=np.int32), tiles)
-    number = np.arange(len(seq), dtype=np.int32) - np.repeat(np.cumsum(tiles) - tiles, tiles).astype(np.int32)
     first = (np.cumsum(q) - q).astype(np.int32)
-    return {"few.seq": seq, "few.t0": first[seq] + number * per, "few.nt": np.minimum(per, q[seq] - number * per).astype(np.int32)}
+    share = kv8_head_groups(heads_per_group)
+    long = (q > 1) & (q * heads_per_group > KV8_MANY) & (heads_per_group <= 128)
+    out = {}
+    for name, of, per in (("few", np.flatnonzero(~long), 1 if share > 1 else max(1, 16 // heads_per_group)),
+                          ("many", np.flatnonzero(long), 2 * (128 // max(1, min(heads_per_group, 128))))):
+        if len(of) == 0:
+            continue
+        tiles = -(-q[of] // per)
+        seq = np.repeat(of, tiles).astype(np.int32)
+        at = (np.arange(len(seq)) - np.repeat(np.cumsum(tiles) - tiles, tiles)).astype(np.int32) * np.int32(per)
+        out.update({name + ".seq": seq, name + ".t0": first[seq] + at, name + ".nt": np.minimum(per, q[seq] - at).astype(np.int32)})
+    return out
 
 
 def paged_attention_kv8(q, cache, meta, ctx, H, G, d, window, scale, out, tiles=None, settled: bool = False, sinks=None, zero_sink=False,

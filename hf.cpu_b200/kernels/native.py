@@ -417,8 +417,16 @@ class NativeBackend:
         self._here(q, cache, meta.block_table, ctx.token_seq, ctx.positions, out, sinks, slopes, head_scales)
         self._on_gpu(q, cache, meta.block_table, ctx.token_seq, ctx.positions, out, sinks, slopes, head_scales)
         opt_args = (_p(sinks), c_int(1 if zero_sink else 0), _p(slopes), _p(head_scales), c_float(softcap))
-        if (self.attention == "fast" and "few.seq" in tiles and q.dtype == torch.bfloat16 and d in (64, 128) and meta.block_size in (8, 16, 32, 64)):
-            self._kv8_few(q, cache, meta, ctx, H, G, d, window, scale, out, tiles, settled, opt_args)
+        if (self.attention == "fast" and ("few.seq" in tiles or "many.seq" in tiles) and q.dtype == torch.bfloat16 and d in (64, 128)
+                and meta.block_size in (8, 16, 32, 64) and scale > 0 and q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0):
+            if "many.seq" in tiles:
+                seq = tiles["many.seq"]
+                self._check(self.lib.hfb_kv8_attention_many(
+                    _p(q), _p(cache), _p(meta.block_table), c_int(meta.max_blocks), _p(ctx.positions), _p(seq), _p(tiles["many.t0"]),
+                    _p(tiles["many.nt"]), c_int(seq.shape[0]), c_int(1 if settled else 0), c_int(meta.block_size), c_int64(cache.shape[0]),
+                    c_int(window), c_float(scale), _p(out), c_int(H), c_int(G), c_int(d), *opt_args, self._stream()), "kv8_attention_many")
+            if "few.seq" in tiles:
+                self._kv8_few(q, cache, meta, ctx, H, G, d, window, scale, out, tiles, settled, opt_args)
             return
         self._check(self.lib.hfb_kv8_attention_plain(
             _p(q), _p(cache), c_int(_dt(q)), _p(meta.block_table), c_int(meta.max_blocks), _p(ctx.token_seq), _p(ctx.positions),

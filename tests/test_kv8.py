@@ -60,9 +60,11 @@ def test_tile_lists_cover_every_token_once(q_lens, r):
             assert nt >= 1 and first[s] <= t0 and t0 + nt <= first[s + 1]
             if h == "few":
                 assert nt * (r // share) <= 16 and (nt == 1 or share == 1)
+            else:
+                assert h == "many" and nt <= 2 * (128 // r)
             seen[t0:t0 + nt] += 1
+        assert len(set(len(x) for n, x in a.items() if n.startswith(h))) == 1
     assert (seen == 1).all()
-    assert len(set(len(x) for n, x in a.items() if n.startswith("few."))) == 1
 
 
 def _args(T=4, H=4, G=2, d=32, bs=8, dtype=torch.bfloat16):
