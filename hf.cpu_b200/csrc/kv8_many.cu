@@ -3,8 +3,8 @@
 //
 // s_j = scale (q . code_j) ks_j, out = sum_j p_j vs_j code'_j / sum_j p_j.  The exponentials bound it (128 x 128 of them for every pair of
 // products of 128 x 128 x d), so nothing of the 8 bits is left to the threads that compute them but two factors:
-// * two warps of their own turn codes into float16 (exact: whole numbers below 2^11) in the layout of the tensor core's operands, 64 keys
-//   each of a tile of 128, while the softmax of the tile before runs.  Each fetches its half's codes itself, by bulk copies as soon as it
+// * four warps of their own turn codes into float16 (exact: whole numbers below 2^11) in the layout of the tensor core's operands, 32 keys
+//   each of a tile of 128, while the softmax of the tile before runs.  Each fetches its keys' codes itself, by bulk copies as soon as it
 //   has read the last ones, keys and values each into their own staging buffer: a tile's keys are on their way while its predecessor's
 //   values still wait for their place.
 // * the scales stay out of the operands: a score is multiplied by its key's, a weight by its value's, in float32, both read as
@@ -14,7 +14,7 @@
 //   is rounded once to float16.  Both sums carry the factor, which cancels.  R is raised, and the sums so far rescaled (the output in
 //   TMEM), only when it has been outgrown by 2^4.  (log2 of the scale is taken as -90 at least: smaller values are zeros.)
 // * a row belongs to one thread, which reads its scores from TMEM twice, 32 at a time, for the maximum and for the weights (128 at once
-//   beside their scales do not fit the registers of twelve warps); O lives in TMEM; one tile's softmax runs beside the other's products.
+//   beside their scales do not fit the registers of thirteen warps); O lives in TMEM; one tile's softmax runs beside the other's products.
 // Barrier waits are bounded (HFB_ERR_WAIT, TMEM freed; tc_ptx.cuh).
 #include <cuda_fp16.h>
 
@@ -26,7 +26,7 @@ static thread_local cudaError_t g_launch_err = cudaSuccess;      // what the las
 namespace hfb {
 int *error_word();
 
-constexpr int KM_ROWS = 128, KM_KEYS = 128, KM_THREADS = 384, KM_TMEM_COLS = 512;
+constexpr int KM_ROWS = 128, KM_KEYS = 128, KM_THREADS = 416, KM_TMEM_COLS = 512;
 constexpr uint32_t KM_SUB = 128 * 64 * 2;           // one swizzled sub-tile: 128 rows of 64 float16
 constexpr uint32_t KM_TILE = 2 * KM_SUB;            // a [128 x 128] operand (P)
 
@@ -102,10 +102,10 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
     const uint32_t sS = stV + CODES;                 // [2][keys' scales 128 | values' scales 128]
     const uint32_t bars = sS + 2048;
     const uint32_t q_ready = bars, s_full = bars + 16, p_ready = bars + 32, pv_done = bars + 48, s_free = bars + 64;       // + 8 * query tile
-    const uint32_t k_st_full = bars + 80, v_st_full = bars + 96;                                                          // + 8 * half
-    const uint32_t k_full = bars + 112, k_empty = bars + 120, v_full = bars + 128, v_empty = bars + 136;
-    const uint32_t sc_full = bars + 144, sc_empty = bars + 160;                                                           // + 8 * buffer
-    volatile uint32_t *tmem_slot = (volatile uint32_t *)(gen + (bars - base) + 192);
+    const uint32_t k_st_full = bars + 80, v_st_full = bars + 112;                                                         // + 8 * quarter
+    const uint32_t k_full = bars + 144, k_empty = bars + 152, v_full = bars + 160, v_empty = bars + 168;
+    const uint32_t sc_full = bars + 176, sc_empty = bars + 192;                                                           // + 8 * buffer
+    volatile uint32_t *tmem_slot = (volatile uint32_t *)(gen + (bars - base) + 224);
     volatile int *abort_flag = (volatile int *)(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (base - smem_u32(km_raw) > (D == 128 ? 768u : 1024u)) {           // (see the launch)
@@ -116,15 +116,15 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; i++) {
             mbar_init(q_ready + 8 * i, 4); mbar_init(s_full + 8 * i, 1); mbar_init(p_ready + 8 * i, 4); mbar_init(pv_done + 8 * i, 1);
-            mbar_init(s_free + 8 * i, 4); mbar_init(sc_full + 8 * i, 2); mbar_init(sc_empty + 8 * i, 8);
+            mbar_init(s_free + 8 * i, 4); mbar_init(sc_full + 8 * i, 4); mbar_init(sc_empty + 8 * i, 8);
         }
-        for (int i = 0; i < 2; i++) { mbar_init(k_st_full + 8 * i, 1); mbar_init(v_st_full + 8 * i, 1); }
-        mbar_init(k_full, 2); mbar_init(v_full, 2); mbar_init(k_empty, 1); mbar_init(v_empty, 1);
+        for (int i = 0; i < 4; i++) { mbar_init(k_st_full + 8 * i, 1); mbar_init(v_st_full + 8 * i, 1); }
+        mbar_init(k_full, 4); mbar_init(v_full, 4); mbar_init(k_empty, 1); mbar_init(v_empty, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == 1) {
+    if (warp == 12) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(smem_u32((const void *)tmem_slot)), "r"(KM_TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -159,8 +159,8 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
     };
     const int n_rounds = (n_items + n_ctas - 1) / n_ctas;
 
-    if (warp == 0 || warp == 1) {
-        if (warp == 1 && lane == 0) {
+    if (warp == 12) {
+        if (lane == 0) {
             // ---- tensor-core issue ------------------------------------------------------------------------------------------------
             constexpr uint32_t F16 = (1u << 7) | (1u << 10);             // (the operands' type bits of bfloat16: clear for float16)
             constexpr uint32_t idesc_s = bf16_idesc(KM_ROWS, KM_KEYS, false) & ~F16, idesc_pv = bf16_idesc(KM_ROWS, D, true) & ~F16;
@@ -201,7 +201,6 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                     // outputs of step j, whose last weights follow shortly
                     const bool more = j + 1 < it.n_kt;
                     if (more) ok = mbar_wait(k_full, (gs + 1) & 1, abort_flag, err);
-                    if (ok) ok = mbar_wait(v_full, gs & 1, abort_flag, err);
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
                         const int n = i ? it.n_kt1 : it.n_kt0;
@@ -211,6 +210,7 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                             if (ok) { tc_fence_after(); issue_s(i); }
                         }
                         if (ok && more && i == 1) tc_commit(k_empty);
+                        if (ok && i == 0) ok = mbar_wait(v_full, gs & 1, abort_flag, err);
                         if (ok && j < n) {
                             ok = mbar_wait(p_ready + 8 * i, ph, abort_flag, err);
                             if (ok) { tc_fence_after(); issue_pv(i, j > 0); }
@@ -224,24 +224,21 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
             // nothing of this CTA's is in flight once the last release of V has landed
             if (ok && gs > 0) mbar_wait(v_empty, (gs - 1) & 1, abort_flag, err);
         }
-    } else if (warp < 4) {
-        // ---- codes into operands: a warp has one half of a tile's keys, a lane two of them ----------------------------------------
-        const int half = warp - 2, half_pages = 64 / bs;
-        const uint32_t page_bytes = bs * D, k_in = k_st_full + 8 * half, v_in = v_st_full + 8 * half, half_at = (uint32_t)half * 64 * D;
+    } else if (warp >= 8) {
+        // ---- codes into operands: a warp has a quarter of a tile's keys, a lane one of them ----------------------------------------
+        const int part = bs < 32 ? bs : 32, copies = 32 / part;                     // keys of one copy: a page of the quarter, or half a page
+        const int row = (warp - 8) * 32 + lane;
+        const uint32_t part_bytes = part * D, page_bytes = bs * D, k_in = k_st_full + 8 * (warp - 8), v_in = v_st_full + 8 * (warp - 8);
         auto convert = [&](uint32_t from, uint32_t to) {
+            uint4 w[D / 16];
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int row = half * 64 + 32 * u + lane;
-                uint4 w[D / 16];
+            for (int c = 0; c < D / 16; c++)
+                asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[c].x), "=r"(w[c].y), "=r"(w[c].z), "=r"(w[c].w)
+                             : "r"(from + (uint32_t)row * D + (uint32_t)kv8_piece(row % bs, c, D) * 16u));
 #pragma unroll
-                for (int c = 0; c < D / 16; c++)
-                    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[c].x), "=r"(w[c].y), "=r"(w[c].z), "=r"(w[c].w)
-                                 : "r"(from + (uint32_t)row * D + (uint32_t)kv8_piece(row % bs, c, D) * 16u));
-#pragma unroll
-                for (int c = 0; c < D / 16; c++) {
-                    km_store16(to + km_off(row, 2 * c), km_codes(w[c].x, 0x4140), km_codes(w[c].x, 0x4342), km_codes(w[c].y, 0x4140), km_codes(w[c].y, 0x4342));
-                    km_store16(to + km_off(row, 2 * c + 1), km_codes(w[c].z, 0x4140), km_codes(w[c].z, 0x4342), km_codes(w[c].w, 0x4140), km_codes(w[c].w, 0x4342));
-                }
+            for (int c = 0; c < D / 16; c++) {
+                km_store16(to + km_off(row, 2 * c), km_codes(w[c].x, 0x4140), km_codes(w[c].x, 0x4342), km_codes(w[c].y, 0x4140), km_codes(w[c].y, 0x4342));
+                km_store16(to + km_off(row, 2 * c + 1), km_codes(w[c].z, 0x4140), km_codes(w[c].z, 0x4342), km_codes(w[c].w, 0x4140), km_codes(w[c].w, 0x4342));
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (also: the staging has been read before it is written again)
             __syncwarp();
@@ -254,39 +251,39 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
             const int32_t *table = p.block_table + (size_t)it.seq * p.max_blocks;
             // the page of step j that this lane asks for, -1 where there is none to be read
             auto page_of = [&](int j) {
-                const int key0 = (it.kt_lo + j) * KM_KEYS + half * 64 + lane * bs, blk = key0 / bs;
-                if (j >= it.n_kt || lane >= half_pages || key0 > it.pos_last || key0 + bs <= it.lo_first) return -1;
+                const int key0 = (it.kt_lo + j) * KM_KEYS + (warp - 8) * 32 + lane * part, blk = key0 / bs;
+                if (j >= it.n_kt || lane >= copies || key0 > it.pos_last || key0 + part <= it.lo_first) return -1;
                 const int page = blk < p.max_blocks ? table[blk] : -1;
                 if (page < 0 || page >= p.num_pages) { atomicOr(err, HFB_ERR_PAGE); return -1; }
                 return page;
             };
             auto fetch = [&](int page, uint32_t bar, uint32_t dst, uint32_t skip) {
                 const int n = __popc(__ballot_sync(0xffffffffu, page >= 0));
-                if (lane == 0) mbar_arrive_expect_tx(bar, n * page_bytes);
+                if (lane == 0) mbar_arrive_expect_tx(bar, n * part_bytes);
                 __syncwarp();
-                if (page >= 0) km_bulk(dst + half_at + lane * page_bytes, p.cache + ((size_t)page * p.G + it.g) * p.record + skip, page_bytes, bar);
+                const uint32_t first = (uint32_t)((warp - 8) * 32 + lane * part);          // row of the tile
+                if (page >= 0) km_bulk(dst + first * D, p.cache + ((size_t)page * p.G + it.g) * p.record + skip + (first % bs) * D, part_bytes, bar);
             };
             // a key's scales; where it is not to be read (behind the last, passed by every row's mask, no page) 0 and -1
-            auto scales_of = [&](int j, int page, int u) {
-                const int in_half = 32 * u + lane, key = (it.kt_lo + j) * KM_KEYS + half * 64 + in_half;
-                const int its = __shfl_sync(0xffffffffu, page, in_half / bs);
+            auto scales_of = [&](int j, int page) {
+                const int key = (it.kt_lo + j) * KM_KEYS + row;
+                const int its = __shfl_sync(0xffffffffu, page, lane / part);
                 if (its < 0 || key > it.pos_last || key < it.lo_first) return make_float2(0.f, -1.f);
-                const float *s = (const float *)(p.cache + ((size_t)its * p.G + it.g) * p.record + 2 * bs * D) + in_half % bs;
+                const float *s = (const float *)(p.cache + ((size_t)its * p.G + it.g) * p.record + 2 * bs * D) + row % bs;
                 return make_float2(s[0], s[bs]);
             };
             int page = page_of(0);
             fetch(page, k_in, stK, 0);
             fetch(page, v_in, stV, page_bytes);
-            float2 sc0 = scales_of(0, page, 0), sc1 = scales_of(0, page, 1);
+            float2 sc = scales_of(0, page);
             int next = page_of(1);                                        // the pages of step j + 1; `page`: of step j
             for (int j = 0; j <= it.n_kt && ok; j++) {
                 // keys of step j, then values of step j - 1: the keys' place is free early in a step, the values' at its end
                 if (j < it.n_kt) {
-                    const uint32_t g = gs + j, b = g & 1, at = sS + b * 1024u + 4u * (half * 64 + lane);
+                    const uint32_t g = gs + j, b = g & 1, at = sS + b * 1024u + 4u * row;
                     ok = mbar_wait(sc_empty + 8 * b, ((g >> 1) & 1) ^ 1, abort_flag, err);
                     if (!ok) break;
-                    asm volatile("st.shared.f32 [%0], %1;\n\tst.shared.f32 [%0 + 512], %2;\n\tst.shared.f32 [%0 + 128], %3;\n\tst.shared.f32 [%0 + 640], %4;"
-                                 ::"r"(at), "f"(sc0.x), "f"(sc0.y), "f"(sc1.x), "f"(sc1.y) : "memory");
+                    asm volatile("st.shared.f32 [%0], %1;\n\tst.shared.f32 [%0 + 512], %2;" ::"r"(at), "f"(sc.x), "f"(sc.y) : "memory");
                     __syncwarp();
                     if (lane == 0) mbar_arrive(sc_full + 8 * b);
                     ok = mbar_wait(k_in, g & 1, abort_flag, err) && mbar_wait(k_empty, (g & 1) ^ 1, abort_flag, err);
@@ -295,8 +292,7 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                     if (lane == 0) mbar_arrive(k_full);
                     if (j + 1 < it.n_kt) {
                         fetch(next, k_in, stK, 0);
-                        sc0 = scales_of(j + 1, next, 0);
-                        sc1 = scales_of(j + 1, next, 1);
+                        sc = scales_of(j + 1, next);
                     }
                 }
                 if (j > 0) {
@@ -315,7 +311,7 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
     } else {
         // ---- softmax and output: one thread per row -------------------------------------------------------------------------------
         const float log2e = 1.4426950408889634f;
-        const int i = (warp - 4) >> 2;                                   // query tile
+        const int i = warp >> 2;                                         // query tile
         const int row = (warp & 3) * 32 + lane;                          // TMEM lane = row; a warp reads its own quarter
         const int tl = row / r, hl = row % r;
         const uint32_t lane_base = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
@@ -535,7 +531,7 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
         for (int i = 0; i < 2000; i++) __nanosleep(1000);              // let copies still in flight land
     }
     __syncthreads();
-    if (warp == 1) {
+    if (warp == 12) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(KM_TMEM_COLS) : "memory");
     }
