@@ -76,6 +76,14 @@ __device__ __forceinline__ float4 km_load4(uint32_t addr)
     asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
     return v;
 }
+// Waits for what has been asked of TMEM, and ties the registers to the wait: nothing that reads them may move in front of it.
+__device__ __forceinline__ void km_wait(uint32_t (&v)[32])
+{
+#define KM_REGS(o) "+r"(v[o]), "+r"(v[o + 1]), "+r"(v[o + 2]), "+r"(v[o + 3]), "+r"(v[o + 4]), "+r"(v[o + 5]), "+r"(v[o + 6]), "+r"(v[o + 7])
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : KM_REGS(0), KM_REGS(8)::"memory");
+    asm volatile("" : KM_REGS(16), KM_REGS(24)::"memory");
+#undef KM_REGS
+}
 __device__ __forceinline__ float km_load1(uint32_t addr)
 {
     float v;
@@ -380,19 +388,22 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                 gap = __any_sync(0xffffffffu, gap);
                 const bool all_visible = (!valid && !gap) || (key0 + KM_KEYS - 1 <= pos && key0 >= lo && !gap);
                 const float b0 = slope2 * (float)(key0 - pos), by_head = unit * hscale, sc = finished ? 1.f : unit;
+                // a step without options in which every row sees every key, as most are
+                const bool open = __all_sync(0xffffffffu, all_visible) && !finished;
+                auto load32 = [&](int c0, uint32_t (&raw)[32]) { tmem_ld16(tS + c0, raw); tmem_ld16(tS + c0 + 16, raw + 16); };
+                auto by_scales = [&](int c0, const uint32_t (&raw)[32], int c, f32pair &a, f32pair &b) {
+                    const float4 k = km_load4(s_at + 4u * (c0 + c));
+                    a = mul2(pair_of(__uint_as_float(raw[c]), __uint_as_float(raw[c + 1])), pair_of(k.x, k.y));
+                    b = mul2(pair_of(__uint_as_float(raw[c + 2]), __uint_as_float(raw[c + 3])), pair_of(k.z, k.w));
+                };
                 // 32 scores from TMEM with their keys' scales, options and masks; what they lack is the factor sc > 0
                 auto scores = [&](int c0, f32pair (&x)[16]) {
                     uint32_t raw[32];
                     __syncwarp();
-                    tmem_ld16(tS + c0, raw);
-                    tmem_ld16(tS + c0 + 16, raw + 16);
-                    tmem_wait_ld();
+                    load32(c0, raw);
+                    km_wait(raw);
 #pragma unroll
-                    for (int c = 0; c < 32; c += 4) {
-                        const float4 k = km_load4(s_at + 4u * (c0 + c));
-                        x[c / 2] = mul2(pair_of(__uint_as_float(raw[c]), __uint_as_float(raw[c + 1])), pair_of(k.x, k.y));
-                        x[c / 2 + 1] = mul2(pair_of(__uint_as_float(raw[c + 2]), __uint_as_float(raw[c + 3])), pair_of(k.z, k.w));
-                    }
+                    for (int c = 0; c < 32; c += 4) by_scales(c0, raw, c, x[c / 2], x[c / 2 + 1]);
                     if (finished) {
 #pragma unroll
                         for (int c = 0; c < 32; c += 2) {
@@ -415,6 +426,27 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                     }
                 };
                 float mx = -INFINITY;
+                uint32_t ra[32], rb[32];
+                if (open) {
+                    // (the next 32 are on their way while these are worked on)
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    auto largest = [&](int c0, const uint32_t (&raw)[32]) {
+#pragma unroll
+                        for (int c = 0; c < 32; c += 4) {
+                            f32pair a, b;
+                            by_scales(c0, raw, c, a, b);
+                            const float2 x = halves(a), y = halves(b);
+                            top[(c >> 1) & 3] = fmaxf(top[(c >> 1) & 3], fmaxf(x.x, x.y));
+                            top[((c >> 1) + 1) & 3] = fmaxf(top[((c >> 1) + 1) & 3], fmaxf(y.x, y.y));
+                        }
+                    };
+                    load32(0, ra); km_wait(ra);
+                    load32(32, rb); largest(0, ra); km_wait(rb);
+                    load32(64, ra); largest(32, rb); km_wait(ra);
+                    load32(96, rb); largest(64, ra); km_wait(rb);
+                    largest(96, rb);
+                    mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                } else
 #pragma unroll 1
                 for (int c0 = 0; c0 < 128; c0 += 32) {
                     f32pair x[16];
@@ -450,6 +482,35 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                 const float minus = ref == -INFINITY ? 0.f : -ref;
                 const f32pair sc2 = pair_of(sc, sc), minus2 = pair_of(minus, minus), one2 = pair_of(1.f, 1.f);
                 f32pair sum[2] = {pair_of(0.f, 0.f), pair_of(0.f, 0.f)};
+                __syncwarp();
+                if (open) {
+                    auto weights = [&](int c0, const uint32_t (&raw)[32]) {
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int c = 0; c < 32; c += 4) {
+                            f32pair a, b;
+                            by_scales(c0, raw, c, a, b);
+                            const float4 v = km_load4(s_at + 512u + 4u * (c0 + c));
+                            const float2 x = halves(fma2(a, sc2, minus2)), y = halves(fma2(b, sc2, minus2));
+                            const f32pair ea = pair_of(km_ex2(x.x), km_ex2(x.y)), eb = pair_of(km_ex2(y.x), km_ex2(y.y));
+                            sum[0] = fma2(ea, one2, sum[0]);
+                            sum[1] = fma2(eb, one2, sum[1]);
+                            const float2 wa = halves(mul2(ea, pair_of(v.x, v.y))), wb = halves(mul2(eb, pair_of(v.z, v.w)));
+                            pk[c / 2] = km_pack(wa.x, wa.y);
+                            pk[c / 2 + 1] = km_pack(wb.x, wb.y);
+                        }
+#pragma unroll
+                        for (int q = 0; q < 4; q++) km_store16(sP + i * KM_TILE + km_off(row, c0 / 8 + q), pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
+                    };
+                    load32(0, ra); km_wait(ra);
+                    load32(32, rb); weights(0, ra); km_wait(rb);
+                    load32(64, ra); weights(32, rb); km_wait(ra);
+                    load32(96, rb); weights(64, ra); km_wait(rb);
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(s_free + 8 * i);          // the tensor core may write the next scores
+                    weights(96, rb);
+                } else
 #pragma unroll 1
                 for (int c0 = 0; c0 < 128; c0 += 32) {
                     f32pair x[16];
