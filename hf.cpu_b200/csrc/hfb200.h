@@ -231,10 +231,13 @@ int hfb_kv8_attention_few(const void *q, const void *cache, const int32_t *block
                           int zero_sink, const float *slopes, const float *head_scales, float softcap, hfb_stream s);
 
 /* ... of prompt portions on tcgen05: bfloat16, head sizes 64 and 128, pages of 8, 16, 32 or 64 tokens, at most 128 heads on a key/value
- * head, scale > 0.  A tile is up to 2 * (128 / (H / G)) consecutive tokens of one request. */
+ * head, scale > 0.  A tile is up to 2 * (128 / (H / G)) consecutive tokens of one request.  The work is cut evenly over `ctas` CTAs (one
+ * an SM) as above, with hfb_kv8_attention_many_scratch bytes of scratch and 2 * n_tiles * G counters. */
+size_t hfb_kv8_attention_many_scratch(int ctas, int d);
 int hfb_kv8_attention_many(const void *q, const void *cache, const int32_t *block_table, int max_blocks, const int32_t *positions,
-                           const int32_t *tile_seq, const int32_t *tile_t0, const int32_t *tile_nt, int n_tiles, int settled, int block_size,
-                           int64_t num_pages, int window, float scale, void *out, int H, int G, int d, const float *sinks, int zero_sink,
+                           const int32_t *tile_seq, const int32_t *tile_t0, const int32_t *tile_nt, int n_tiles, int ctas, int tile_cost,
+                           int settled, int block_size, int64_t num_pages, int window, float scale, void *out, void *scratch,
+                           size_t scratch_bytes, int *counters, int counters_len, int H, int G, int d, const float *sinks, int zero_sink,
                            const float *slopes, const float *head_scales, float softcap, hfb_stream s);
 
 /* Launches may overlap with the kernel in front (programmatic dependent launch): on by default, off with HFB_PDL=0. */

@@ -15,6 +15,9 @@
 //   TMEM), only when it has been outgrown by 2^4.  (log2 of the scale is taken as -90 at least: smaller values are zeros.)
 // * a row belongs to one thread, which reads its scores from TMEM twice, 32 at a time, for the maximum and for the weights (128 at once
 //   beside their scales do not fit the registers of thirteen warps); O lives in TMEM; one tile's softmax runs beside the other's products.
+// * work is cut evenly (as in kv8_few.cu): a step is a tile of keys of one double tile and key/value head, CTA c of C walks steps c N / C to
+//   (c + 1) N / C.  What a CTA has of a double tile that others share goes to scratch, and whoever brings its last piece merges them, in
+//   the order of the keys.  (Whole double tiles a CTA: 228 items of 2,048 tokens and 28 heads are two rounds on 148 SMs where 1.5 would do.)
 // Barrier waits are bounded (HFB_ERR_WAIT, TMEM freed; tc_ptx.cuh).
 #include <cuda_fp16.h>
 
@@ -32,7 +35,9 @@ constexpr uint32_t KM_TILE = 2 * KM_SUB;            // a [128 x 128] operand (P)
 
 struct Kv8ManyParams {
     Kv8Params a;
-    int per, n_tiles, settled;                       // tokens per query tile, double tiles in all
+    int per, n_tiles, tile_cost, settled;            // tokens per query tile, double tiles in all, steps that a tile's start and end are reckoned as
+    float *part_o, *part_ml;                         // pieces of double tiles: [CTAs, 2, 2, D / 4, 128, 4] and [CTAs, 2, 2, 128, 2]
+    int *counters;                                   // ... one per (double tile, head, query tile), zero between launches
 };
 
 template <int D> constexpr uint32_t km_smem() { return 2 * KM_TILE + 4 * (D / 64) * KM_SUB + 2 * KM_KEYS * D + 2048 + 256; }
@@ -132,6 +137,47 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
+    // ---- this CTA's steps -------------------------------------------------------------------------------------------------------
+    const int r = p.H / p.G, bs = p.block_size, pages = KM_KEYS / bs;
+    struct Tile { int seq, t0, nt, pos_last, lo_first, kt_lo, n_kt0, n_kt; };
+    auto tile_of = [&](int i) {
+        Tile x;
+        x.seq = p.tile_seq[i]; x.t0 = p.tile_t0[i];
+        x.nt = max(1, min(p.tile_nt[i], 2 * f.per));                     // (what the tile has places for)
+        x.pos_last = p.positions[x.t0 + x.nt - 1];
+        x.lo_first = mask_lo(p.positions[x.t0], p.window);
+        x.kt_lo = x.lo_first / KM_KEYS;
+        x.n_kt0 = max(1, p.positions[x.t0 + min(x.nt, f.per) - 1] / KM_KEYS + 1 - x.kt_lo);
+        x.n_kt = max(x.n_kt0, x.pos_last / KM_KEYS + 1 - x.kt_lo);
+        return x;
+    };
+    int *scan = (int *)(gen + (sP - base));                              // (the weights' place, still free)
+    const int each = (f.n_tiles + KM_THREADS - 1) / KM_THREADS, i0 = min((int)threadIdx.x * each, f.n_tiles), i1 = min(i0 + each, f.n_tiles);
+    int mine = 0;
+    for (int i = i0; i < i1; i++) mine += tile_of(i).n_kt + f.tile_cost;
+    int up = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, up, o); if (lane >= o) up += v; }
+    if (lane == 31) scan[warp] = up;
+    __syncthreads();
+    int before = up - mine, per_head = 0;
+    for (int w = 0; w < KM_THREADS / 32; w++) { if (w < warp) before += scan[w]; per_head += scan[w]; }
+    const long long total = (long long)per_head * p.G;
+    const int ctas = (int)min((long long)gridDim.x, total), cta = blockIdx.x;
+    if (cta >= ctas) return;
+    auto start_of = [&](int c) { return total * c / ctas; };
+    const long long x_start = start_of(cta), x_end = start_of(cta + 1);
+    if ((long long)before * p.G <= x_start && x_start < (long long)(before + mine) * p.G) {
+        int i = i0, at = before;
+        for (;; i++) {
+            const int n = tile_of(i).n_kt + f.tile_cost;
+            if ((long long)(at + n) * p.G > x_start) break;
+            at += n;
+        }
+        scan[32] = i; scan[33] = at;
+    }
+    __syncthreads();
+    const int first_tile = scan[32], first_before = scan[33];
     if (warp == 12) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(smem_u32((const void *)tmem_slot)), "r"(KM_TMEM_COLS) : "memory");
@@ -144,28 +190,32 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
     if (f.settled) pdl_wait();
     pdl_trigger();
 
-    // Work items are (double tile, key/value head), heaviest first; the rounds run over the CTAs forwards and backwards in turn.
-    const int r = p.H / p.G, bs = p.block_size, pages = KM_KEYS / bs;
-    const int n_items = f.n_tiles * p.G, n_ctas = gridDim.x;
-    struct Item { int g, seq, t0, nt0, nt1, pos_last, lo_first, kt_lo, n_kt0, n_kt1, n_kt; };
-    auto item_of = [&](int round, Item &it) -> bool {
-        const int idx = round * n_ctas + ((round & 1) ? n_ctas - 1 - (int)blockIdx.x : (int)blockIdx.x);
-        if (idx >= n_items) return false;
-        const int tile = f.n_tiles - 1 - idx / p.G;
-        it.g = idx % p.G;
-        it.seq = p.tile_seq[tile]; it.t0 = p.tile_t0[tile];
-        const int nt = max(1, min(p.tile_nt[tile], 2 * f.per));
-        it.nt0 = min(nt, f.per); it.nt1 = nt - it.nt0;                  // tokens of the two query tiles
-        const int pos_last0 = p.positions[it.t0 + it.nt0 - 1];
-        it.pos_last = p.positions[it.t0 + nt - 1];
-        it.lo_first = mask_lo(p.positions[it.t0], p.window);
-        it.kt_lo = it.lo_first / KM_KEYS;
-        it.n_kt0 = max(1, pos_last0 / KM_KEYS + 1 - it.kt_lo);
-        it.n_kt1 = it.nt1 > 0 ? max(1, it.pos_last / KM_KEYS + 1 - it.kt_lo) : 0;
-        it.n_kt = max(it.n_kt0, it.n_kt1);
-        return true;
+    // A piece: steps off .. off + n_kt of one double tile and head; n_kt0, n_kt1: how many of them the two query tiles take part in.
+    // Every role walks the same ones.
+    struct Item { int g, seq, t0, nt0, nt1, pos_last, lo_first, kt_lo, n_kt0, n_kt1, n_kt, tile, all; long long first; bool begins; };
+    struct Walk { long long x; int tile, before; };
+    auto item_of = [&](Walk &w, Item &it) -> bool {
+        for (;;) {
+            if (w.x >= x_end) return false;
+            const Tile tl = tile_of(w.tile);
+            const int n = tl.n_kt + f.tile_cost;
+            const long long t_first = (long long)w.before * p.G;
+            if (w.x >= t_first + (long long)n * p.G) { w.before += n; w.tile++; continue; }
+            it.g = (int)((w.x - t_first) / n);
+            it.first = t_first + (long long)it.g * n + f.tile_cost;      // (the tile's own steps lie behind the empty ones)
+            const long long begin = max(w.x, it.first);
+            w.x = min(x_end, it.first + tl.n_kt);
+            const int off = (int)(begin - it.first);
+            it.n_kt = (int)max(0ll, w.x - begin);
+            if (it.n_kt == 0) continue;
+            it.tile = w.tile; it.all = tl.n_kt; it.begins = off == 0;
+            it.seq = tl.seq; it.t0 = tl.t0; it.pos_last = tl.pos_last; it.lo_first = tl.lo_first; it.kt_lo = tl.kt_lo + off;
+            it.nt0 = min(tl.nt, f.per); it.nt1 = tl.nt - it.nt0;         // tokens of the two query tiles
+            it.n_kt0 = max(0, min(it.n_kt, tl.n_kt0 - off));
+            it.n_kt1 = it.nt1 > 0 ? it.n_kt : 0;
+            return true;
+        }
     };
-    const int n_rounds = (n_items + n_ctas - 1) / n_ctas;
 
     if (warp == 12) {
         if (lane == 0) {
@@ -192,15 +242,14 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
             };
             bool ok = true;
             uint32_t gs = 0, g_tile0 = 0, g_tile1 = 0, q_uses0 = 0, q_uses1 = 0;      // steps so far, per query tile, and items per query tile
-            for (int round = 0; round < n_rounds && ok; round++) {
-                Item it;
-                if (!item_of(round, it)) continue;
-                ok = mbar_wait(q_ready, q_uses0++ & 1, abort_flag, err);
+            Walk walk = {x_start, first_tile, first_before};
+            for (Item it; ok && item_of(walk, it);) {
+                if (it.n_kt0 > 0) ok = mbar_wait(q_ready, q_uses0++ & 1, abort_flag, err);
                 if (ok && it.n_kt1 > 0) ok = mbar_wait(q_ready + 8, q_uses1++ & 1, abort_flag, err);
                 if (ok) ok = mbar_wait(k_full, gs & 1, abort_flag, err);
                 if (ok) {
                     tc_fence_after();
-                    issue_s(0);
+                    if (it.n_kt0 > 0) issue_s(0);
                     if (it.n_kt1 > 0) issue_s(1);
                     tc_commit(k_empty);
                 }
@@ -253,9 +302,8 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
         };
         bool ok = true;
         uint32_t gs = 0;                                                  // steps of the items before
-        for (int round = 0; round < n_rounds && ok; round++) {
-            Item it;
-            if (!item_of(round, it)) continue;
+        Walk walk = {x_start, first_tile, first_before};
+        for (Item it; ok && item_of(walk, it);) {
             const int32_t *table = p.block_table + (size_t)it.seq * p.max_blocks;
             // the page of step j that this lane asks for, -1 where there is none to be read
             auto page_of = [&](int j) {
@@ -326,9 +374,8 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
         const uint32_t tS = lane_base + i * 128, tO = lane_base + 256 + i * D;
         uint32_t g_mine = 0, gs = 0;                                     // this query tile's steps so far, and the item's
         bool ok = true;
-        for (int round = 0; round < n_rounds && ok; round++) {
-            Item it;
-            if (!item_of(round, it)) continue;
+        Walk walk = {x_start, first_tile, first_before};
+        for (Item it; ok && item_of(walk, it);) {
             const int n_mine = i ? it.n_kt1 : it.n_kt0, nt_mine = i ? it.nt1 : it.nt0, t_first = it.t0 + i * f.per;
             const bool valid = tl < nt_mine;
             const size_t th = ((size_t)(t_first + (valid ? tl : 0)) * p.H + it.g * r + hl) * D;
@@ -440,11 +487,17 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                             top[((c >> 1) + 1) & 3] = fmaxf(top[((c >> 1) + 1) & 3], fmaxf(y.x, y.y));
                         }
                     };
-                    load32(0, ra); km_wait(ra);
-                    load32(32, rb); largest(0, ra); km_wait(rb);
-                    load32(64, ra); largest(32, rb); km_wait(ra);
-                    load32(96, rb); largest(64, ra); km_wait(rb);
-                    largest(96, rb);
+                    load32(0, ra);
+                    km_wait(ra);
+#pragma unroll 1
+                    for (int c0 = 0; c0 < 128; c0 += 64) {
+                        load32(c0 + 32, rb);
+                        largest(c0, ra);
+                        km_wait(rb);
+                        load32((c0 + 64) & 127, ra);                     // (the last time: for the weights)
+                        largest(c0 + 32, rb);
+                        km_wait(ra);
+                    }
                     mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
                 } else
 #pragma unroll 1
@@ -502,14 +555,21 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
 #pragma unroll
                         for (int q = 0; q < 4; q++) km_store16(sP + i * KM_TILE + km_off(row, c0 / 8 + q), pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
                     };
-                    load32(0, ra); km_wait(ra);
-                    load32(32, rb); weights(0, ra); km_wait(rb);
-                    load32(64, ra); weights(32, rb); km_wait(ra);
-                    load32(96, rb); weights(64, ra); km_wait(rb);
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(s_free + 8 * i);          // the tensor core may write the next scores
-                    weights(96, rb);
+#pragma unroll 1
+                    for (int c0 = 0; c0 < 128; c0 += 64) {
+                        load32(c0 + 32, rb);
+                        weights(c0, ra);
+                        km_wait(rb);
+                        if (c0 == 0) {
+                            load32(64, ra);
+                        } else {
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(s_free + 8 * i);  // the tensor core may write the next scores
+                        }
+                        weights(c0 + 32, rb);
+                        if (c0 == 0) km_wait(ra);
+                    }
                 } else
 #pragma unroll 1
                 for (int c0 = 0; c0 < 128; c0 += 32) {
@@ -553,15 +613,26 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
             gs += it.n_kt;
             g_mine += n_mine;
             if (ok && n_mine > 0) ok = mbar_wait(pv_done + 8 * i, (g_mine - 1) & 1, abort_flag, err);
-            if (ok && n_mine > 0) {
-                tc_fence_after();
-                if (p.sinks || p.zero_sink) {
-                    // the sink: one more term of the sum, in the scale of the row's reference
-                    const float sk = p.sinks ? p.sinks[it.g * r + hl] * log2e : 0.f;
-                    l += exp2f(sk - (ref == -INFINITY ? 0.f : ref));
-                }
+            {
+                // (a wait that ran out ends the walk of the query tile's warps together: none may be left at a barrier)
+                int all;
+                asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.and.pred q, %2, 128, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+                             : "=r"(all) : "r"((int)ok), "r"(1 + i) : "memory");
+                ok = all;
+            }
+            if (!ok || nt_mine <= 0) continue;
+            tc_fence_after();
+            if (it.begins && (p.sinks || p.zero_sink)) {
+                // the sink: one more term of the sum, in the scale of the row's reference
+                const float sk = p.sinks ? (valid ? p.sinks[it.g * r + hl] : 0.f) * log2e : 0.f;
+                if (ref == -INFINITY && l == 0.f) ref = sk;
+                l += exp2f(sk - (ref == -INFINITY ? 0.f : ref));
+            }
+            // the pieces of this double tile and head: of CTAs c_first .. c_first + pieces - 1, each its first but for the first one's last
+            const int c_first = (int)(((it.first + 1) * ctas - 1) / total), pieces = (int)(((it.first + it.all) * ctas - 1) / total) - c_first + 1;
+            uint4 *dst = (uint4 *)((__nv_bfloat16 *)p.out + th);
+            if (pieces == 1) {
                 const float inv = l == 0.f ? 0.f : 1.0f / l;
-                uint4 *dst = (uint4 *)((__nv_bfloat16 *)p.out + th);
 #pragma unroll 1
                 for (int c = 0; c < D / 16; c += 4) {                    // four reads of 16 columns under way together
                     uint32_t ov[64];
@@ -579,8 +650,71 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                             dst[2 * (c + u) + 1] = *(uint4 *)&h[4];
                         }
                     }
+                    __syncwarp();
                 }
                 tc_fence_before();
+                continue;
+            }
+            auto place_of = [&](int c) { return (size_t)((c * 2 + (start_of(c) >= it.first ? 0 : 1)) * 2 + i); };
+            {
+                float4 *po = (float4 *)f.part_o + place_of(cta) * (D / 4) * 128 + row;
+                if (n_mine > 0) {
+#pragma unroll 1
+                    for (int c = 0; c < D / 16; c++) {
+                        uint32_t ov[16];
+                        tmem_ld16(tO + 16 * c, ov);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int u = 0; u < 4; u++)
+                            po[(4 * c + u) * 128] = make_float4(__uint_as_float(ov[4 * u]), __uint_as_float(ov[4 * u + 1]), __uint_as_float(ov[4 * u + 2]), __uint_as_float(ov[4 * u + 3]));
+                    }
+                    tc_fence_before();
+                } else {
+                    for (int c = 0; c < D / 4; c++) po[c * 128] = make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+                ((float2 *)f.part_ml)[place_of(cta) * 128 + row] = make_float2(ref, l);
+            }
+            int *flag = (int *)(gen + (bars - base) + 232 + 4 * i);
+            asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
+            if ((threadIdx.x & 127) == 0) {
+                __threadfence();                                         // (after the barrier: it covers the four warps' stores)
+                int *cnt = f.counters + ((size_t)it.tile * p.G + it.g) * 2 + i;
+                const int last = atomicAdd(cnt, 1) == pieces - 1;
+                if (last) *cnt = 0;
+                *(volatile int *)flag = last;
+            }
+            asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
+            if (!*(volatile int *)flag || !valid) continue;              // (the flag is written again behind two barriers)
+            __threadfence();
+            float top = -INFINITY, sum = 0.f;
+            for (int c = 0; c < pieces; c++) top = fmaxf(top, __ldcg((const float2 *)f.part_ml + place_of(c_first + c) * 128 + row).x);
+            for (int c = 0; c < pieces; c++) {
+                const float2 ml = __ldcg((const float2 *)f.part_ml + place_of(c_first + c) * 128 + row);
+                sum += ml.y * (ml.x == -INFINITY ? 1.f : exp2f(ml.x - top));           // (zero, or no number)
+            }
+            const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+#pragma unroll 1
+            for (int c = 0; c < D / 4; c += 8) {
+                float4 acc[8];
+#pragma unroll
+                for (int u = 0; u < 8; u++) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int k = 0; k < pieces; k++) {
+                    const size_t at = place_of(c_first + k);
+                    const float2 ml = __ldcg((const float2 *)f.part_ml + at * 128 + row);
+                    const float e = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
+                    const float4 *po = (const float4 *)f.part_o + (at * (D / 4) + c) * 128 + row;
+#pragma unroll
+                    for (int u = 0; u < 8; u++) {
+                        const float4 v = __ldcg(po + u * 128);
+                        acc[u].x += v.x * e; acc[u].y += v.y * e; acc[u].z += v.z * e; acc[u].w += v.w * e;
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 8; u += 2) {
+                    __nv_bfloat162 h[4] = {__floats2bfloat162_rn(acc[u].x * inv, acc[u].y * inv), __floats2bfloat162_rn(acc[u].z * inv, acc[u].w * inv),
+                                           __floats2bfloat162_rn(acc[u + 1].x * inv, acc[u + 1].y * inv), __floats2bfloat162_rn(acc[u + 1].z * inv, acc[u + 1].w * inv)};
+                    dst[(c + u) / 2] = *(uint4 *)h;
+                }
             }
         }
     }
@@ -617,9 +751,12 @@ static int launch_kv8_many(const Kv8ManyParams &f, int grid, cudaStream_t st)
 
 using namespace hfb;
 
+extern "C" size_t hfb_kv8_attention_many_scratch(int ctas, int d) { return (size_t)ctas * 4 * 128 * (d + 2) * sizeof(float); }
+
 extern "C" int hfb_kv8_attention_many(const void *q, const void *cache, const int32_t *block_table, int max_blocks, const int32_t *positions,
-                                      const int32_t *tile_seq, const int32_t *tile_t0, const int32_t *tile_nt, int n_tiles, int settled, int block_size,
-                                      int64_t num_pages, int window, float scale, void *out, int H, int G, int d, const float *sinks, int zero_sink,
+                                      const int32_t *tile_seq, const int32_t *tile_t0, const int32_t *tile_nt, int n_tiles, int ctas, int tile_cost, int settled, int block_size,
+                                      int64_t num_pages, int window, float scale, void *out, void *scratch,
+                                      size_t scratch_bytes, int *counters, int counters_len, int H, int G, int d, const float *sinks, int zero_sink,
                                       const float *slopes, const float *head_scales, float softcap, hfb_stream s)
 {
     if (n_tiles <= 0) return HFB_OK;
@@ -629,16 +766,17 @@ extern "C" int hfb_kv8_attention_many(const void *q, const void *cache, const in
     if (block_size < 8 || block_size > 64 || 64 % block_size) return fail(HFB_ENOTSUP, "kv8_attention_many: pages of %d tokens (8, 16, 32 and 64)", block_size);
     if (!(scale > 0.f)) return fail(HFB_ENOTSUP, "kv8_attention_many: the factor on the scores must be positive");
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache) & 15) return fail(HFB_EINVAL, "kv8_attention_many: misaligned arrays");
+    if (ctas < 1 || tile_cost < 0 || !scratch || ((uintptr_t)scratch & 15) || scratch_bytes < hfb_kv8_attention_many_scratch(ctas, d) || !counters ||
+        (long long)counters_len < (long long)n_tiles * G * 2)
+        return fail(HFB_EINVAL, "kv8_attention_many: %d CTAs need scratch and counters", ctas);
     Kv8ManyParams f = {};
     f.a.q = q; f.a.cache = (const uint8_t *)cache; f.a.out = out; f.a.block_table = block_table; f.a.positions = positions;
     f.a.tile_seq = tile_seq; f.a.tile_t0 = tile_t0; f.a.tile_nt = tile_nt; f.a.max_blocks = max_blocks; f.a.block_size = block_size;
     f.a.record = kv8_record_bytes(block_size, d); f.a.window = window; f.a.H = H; f.a.G = G; f.a.num_pages = num_pages; f.a.scale = scale;
     f.a.sinks = sinks; f.a.slopes = slopes; f.a.head_scales = head_scales; f.a.zero_sink = zero_sink; f.a.softcap = softcap > 0.f ? softcap : 0.f;
-    f.per = KM_ROWS / (H / G); f.n_tiles = n_tiles; f.settled = settled;
-    int sms = 0, dev = 0;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    const long long items = (long long)n_tiles * G;
-    const int grid = (int)(items < sms ? items : (sms > 0 ? sms : 1));
+    f.per = KM_ROWS / (H / G); f.n_tiles = n_tiles; f.tile_cost = tile_cost; f.settled = settled;
+    f.counters = counters;
+    f.part_o = (float *)scratch; f.part_ml = (float *)scratch + (size_t)ctas * 4 * 128 * d;
+    const int grid = ctas;
     return d == 128 ? launch_kv8_many<128>(f, grid, (cudaStream_t)s) : launch_kv8_many<64>(f, grid, (cudaStream_t)s);
 }

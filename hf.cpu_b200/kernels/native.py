@@ -116,6 +116,7 @@ class NativeBackend:
         self.lib.hfb_linear_tc_workspace.restype = ctypes.c_size_t
         self.lib.hfb_attention_fast_scratch.restype = ctypes.c_size_t
         self.lib.hfb_kv8_attention_few_scratch.restype = ctypes.c_size_t
+        self.lib.hfb_kv8_attention_many_scratch.restype = ctypes.c_size_t
         # "fast": tiled tensor-core attention where the sizes allow; "plain": one block per (token, head) always
         self.attention = os.environ.get("HFB_ATTENTION", "fast")
         self.attention_tc = os.environ.get("HFB_ATTN_TC", "1") != "0"     # tcgen05 attention for prompt portions
@@ -420,11 +421,7 @@ class NativeBackend:
         if (self.attention == "fast" and ("few.seq" in tiles or "many.seq" in tiles) and q.dtype == torch.bfloat16 and d in (64, 128)
                 and meta.block_size in (8, 16, 32, 64) and scale > 0 and q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0):
             if "many.seq" in tiles:
-                seq = tiles["many.seq"]
-                self._check(self.lib.hfb_kv8_attention_many(
-                    _p(q), _p(cache), _p(meta.block_table), c_int(meta.max_blocks), _p(ctx.positions), _p(seq), _p(tiles["many.t0"]),
-                    _p(tiles["many.nt"]), c_int(seq.shape[0]), c_int(1 if settled else 0), c_int(meta.block_size), c_int64(cache.shape[0]),
-                    c_int(window), c_float(scale), _p(out), c_int(H), c_int(G), c_int(d), *opt_args, self._stream()), "kv8_attention_many")
+                self._kv8_many(q, cache, meta, ctx, H, G, d, window, scale, out, tiles, settled, opt_args)
             if "few.seq" in tiles:
                 self._kv8_few(q, cache, meta, ctx, H, G, d, window, scale, out, tiles, settled, opt_args)
             return
@@ -449,6 +446,17 @@ class NativeBackend:
         if have is None or have.numel() < n:
             have = self._kv8_counters[key] = torch.zeros(max(n, 4096), dtype=torch.int32, device=device)
         return have
+
+    def _kv8_many(self, q, cache, meta, ctx, H, G, d, window, scale, out, tiles, settled, opt_args):
+        seq, t0, nt = tiles["many.seq"], tiles["many.t0"], tiles["many.nt"]
+        n, ctas = seq.shape[0], self.sm_count
+        need = self.lib.hfb_kv8_attention_many_scratch(c_int(ctas), c_int(d))
+        scratch, counters = ctx.buf("kv8_scratch", (need,), torch.uint8), self._kv8_zeros(q.device, 2 * n * G)
+        self._check(self.lib.hfb_kv8_attention_many(
+            _p(q), _p(cache), _p(meta.block_table), c_int(meta.max_blocks), _p(ctx.positions), _p(seq), _p(t0), _p(nt), c_int(n), c_int(ctas),
+            c_int(1), c_int(1 if settled else 0), c_int(meta.block_size), c_int64(cache.shape[0]), c_int(window), c_float(scale), _p(out),
+            _p(scratch), ctypes.c_size_t(need), _p(counters), c_int(counters.numel()), c_int(H), c_int(G), c_int(d), *opt_args,
+            self._stream()), "kv8_attention_many")
 
     def _kv8_few(self, q, cache, meta, ctx, H, G, d, window, scale, out, tiles, settled, opt_args):
         from . import kv8_head_groups
