@@ -5,8 +5,7 @@
 // products of 128 x 128 x d), so nothing of the 8 bits is left to the threads that compute them but two factors:
 // * four warps of their own turn codes into float16 (exact: whole numbers below 2^11) in the layout of the tensor core's operands, 32 keys
 //   each of a tile of 128, while the softmax of the tile before runs.  Each fetches its keys' codes itself, by bulk copies as soon as it
-//   has read the last ones, keys and values each into their own staging buffer: a tile's keys are on their way while its predecessor's
-//   values still wait for their place.
+//   has read the last ones.  Both operands have two places, so that the conversion runs a tile ahead of the products.
 // * the scales stay out of the operands: a score is multiplied by its key's, a weight by its value's, in float32, both read as
 //   broadcasts from shared memory.
 // * queries are multiplied by the power of two that brings a row's largest number to 2^14..2^15 (kv8_few.cu).
@@ -14,7 +13,9 @@
 //   is rounded once to float16.  Both sums carry the factor, which cancels.  R is raised, and the sums so far rescaled (the output in
 //   TMEM), only when it has been outgrown by 2^4.  (log2 of the scale is taken as -90 at least: smaller values are zeros.)
 // * a row belongs to one thread, which reads its scores from TMEM twice, 32 at a time, for the maximum and for the weights (128 at once
-//   beside their scales do not fit the registers of thirteen warps); O lives in TMEM; one tile's softmax runs beside the other's products.
+//   beside their scales do not fit the registers of thirteen warps).  The weights go back to TMEM in the scores' place, as the second
+//   product's left operand; O lives in TMEM too.  One query tile's softmax runs beside the other's products: its own next scores follow its
+//   outputs in the tensor core's order, which is all that keeps them off the weights.
 // * work is cut evenly (as in kv8_few.cu): a step is a tile of keys of one double tile and key/value head, CTA c of C walks steps c N / C to
 //   (c + 1) N / C.  What a CTA has of a double tile that others share goes to scratch, and whoever brings its last piece merges them, in
 //   the order of the keys.  (Whole double tiles a CTA: 228 items of 2,048 tokens and 28 heads are two rounds on 148 SMs where 1.5 would do.)
@@ -31,7 +32,6 @@ int *error_word();
 
 constexpr int KM_ROWS = 128, KM_KEYS = 128, KM_THREADS = 416, KM_TMEM_COLS = 512;
 constexpr uint32_t KM_SUB = 128 * 64 * 2;           // one swizzled sub-tile: 128 rows of 64 float16
-constexpr uint32_t KM_TILE = 2 * KM_SUB;            // a [128 x 128] operand (P)
 
 struct Kv8ManyParams {
     Kv8Params a;
@@ -40,7 +40,7 @@ struct Kv8ManyParams {
     int *counters;                                   // ... one per (double tile, head, query tile), zero between launches
 };
 
-template <int D> constexpr uint32_t km_smem() { return 2 * KM_TILE + 4 * (D / 64) * KM_SUB + 2 * KM_KEYS * D + 2048 + 256; }
+template <int D> constexpr uint32_t km_smem() { return 6 * (D / 64) * KM_SUB + 2 * KM_KEYS * D + 2048 + 256; }
 
 __device__ __forceinline__ uint32_t km_off(int row, int c16)
 {
@@ -70,6 +70,13 @@ __device__ __forceinline__ void km_st16(uint32_t taddr, const uint32_t *v)
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
                  ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
                    "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
+}
+// D += A B with A in TMEM (a row a lane, two numbers a column)
+__device__ __forceinline__ void km_mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
 }
 __device__ __forceinline__ void km_store16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d)
 {
@@ -111,13 +118,13 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
     uint8_t *gen = km_raw + (base - smem_u32(km_raw));
     constexpr uint32_t HT = (D / 64) * KM_SUB;       // a [128 x D] float16 operand: Q, K or V
     constexpr uint32_t CODES = KM_KEYS * D;          // a tile's key (or value) codes
-    const uint32_t sQ = base, sK = base + 2 * HT, sV = base + 3 * HT, sP = base + 4 * HT, stK = sP + 2 * KM_TILE, stV = stK + CODES;
+    const uint32_t sQ = base, sK = base + 2 * HT, sV = base + 4 * HT, stK = base + 6 * HT, stV = stK + CODES;      // (keys and values: two each)
     const uint32_t sS = stV + CODES;                 // [2][keys' scales 128 | values' scales 128]
     const uint32_t bars = sS + 2048;
-    const uint32_t q_ready = bars, s_full = bars + 16, p_ready = bars + 32, pv_done = bars + 48, s_free = bars + 64;       // + 8 * query tile
+    const uint32_t q_ready = bars, s_full = bars + 16, p_ready = bars + 32, pv_done = bars + 48;                          // + 8 * query tile
     const uint32_t k_st_full = bars + 80, v_st_full = bars + 112;                                                         // + 8 * quarter
-    const uint32_t k_full = bars + 144, k_empty = bars + 152, v_full = bars + 160, v_empty = bars + 168;
-    const uint32_t sc_full = bars + 176, sc_empty = bars + 192;                                                           // + 8 * buffer
+    const uint32_t k_full = bars + 144, k_empty = bars + 160, v_full = bars + 176, v_empty = bars + 192;                  // + 8 * place
+    const uint32_t sc_full = bars + 208, sc_empty = bars + 64;                                                            // + 8 * buffer
     volatile uint32_t *tmem_slot = (volatile uint32_t *)(gen + (bars - base) + 224);
     volatile int *abort_flag = (volatile int *)(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -129,10 +136,10 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; i++) {
             mbar_init(q_ready + 8 * i, 4); mbar_init(s_full + 8 * i, 1); mbar_init(p_ready + 8 * i, 4); mbar_init(pv_done + 8 * i, 1);
-            mbar_init(s_free + 8 * i, 4); mbar_init(sc_full + 8 * i, 4); mbar_init(sc_empty + 8 * i, 8);
+            mbar_init(k_full + 8 * i, 4); mbar_init(v_full + 8 * i, 4); mbar_init(k_empty + 8 * i, 1); mbar_init(v_empty + 8 * i, 1);
+            mbar_init(sc_full + 8 * i, 4); mbar_init(sc_empty + 8 * i, 8);
         }
         for (int i = 0; i < 4; i++) { mbar_init(k_st_full + 8 * i, 1); mbar_init(v_st_full + 8 * i, 1); }
-        mbar_init(k_full, 4); mbar_init(v_full, 4); mbar_init(k_empty, 1); mbar_init(v_empty, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -151,7 +158,7 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
         x.n_kt = max(x.n_kt0, x.pos_last / KM_KEYS + 1 - x.kt_lo);
         return x;
     };
-    int *scan = (int *)(gen + (sP - base));                              // (the weights' place, still free)
+    int *scan = (int *)(gen + (sV - base));                              // (the values' place, still free)
     const int each = (f.n_tiles + KM_THREADS - 1) / KM_THREADS, i0 = min((int)threadIdx.x * each, f.n_tiles), i1 = min(i0 + each, f.n_tiles);
     int mine = 0;
     for (int i = i0; i < i1; i++) mine += tile_of(i).n_kt + f.tile_cost;
@@ -223,63 +230,60 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
             constexpr uint32_t F16 = (1u << 7) | (1u << 10);             // (the operands' type bits of bfloat16: clear for float16)
             constexpr uint32_t idesc_s = bf16_idesc(KM_ROWS, KM_KEYS, false) & ~F16, idesc_pv = bf16_idesc(KM_ROWS, D, true) & ~F16;
             const uint32_t tS0 = tmem_base, tO0 = tmem_base + 256;
-            const uint64_t dq = sw128_desc(sQ), dk = sw128_desc(sK), dp = sw128_desc(sP), dv = sw128_desc_mn(sV, KM_SUB);
-            auto issue_s = [&](int i) {
+            const uint64_t dq = sw128_desc(sQ), dk = sw128_desc(sK), dv = sw128_desc_mn(sV, KM_SUB);
+            auto issue_s = [&](int i, uint32_t place) {
 #pragma unroll
                 for (int kk = 0; kk < D / 16; kk++) {
                     const uint64_t o = ((uint32_t)(kk >> 2) * KM_SUB + (uint32_t)(kk & 3) * 32u) >> 4;
-                    tc_mma_bf16(tS0 + i * 128, dq + o + (uint64_t)i * (HT >> 4), dk + o, idesc_s, kk > 0 ? 1u : 0u);
+                    tc_mma_bf16(tS0 + i * 128, dq + o + (uint64_t)i * (HT >> 4), dk + o + (uint64_t)place * (HT >> 4), idesc_s, kk > 0 ? 1u : 0u);
                 }
                 tc_commit(s_full + 8 * i);
             };
-            auto issue_pv = [&](int i, bool accumulate) {
+            auto issue_pv = [&](int i, uint32_t place, bool accumulate) {
 #pragma unroll
-                for (int kk = 0; kk < KM_KEYS / 16; kk++) {
-                    const uint64_t o = ((uint32_t)(kk >> 2) * KM_SUB + (uint32_t)(kk & 3) * 32u) >> 4;
-                    tc_mma_bf16(tO0 + i * D, dp + o + (uint64_t)i * (KM_TILE >> 4), dv + (uint64_t)kk * (2048u >> 4), idesc_pv, (accumulate || kk > 0) ? 1u : 0u);
-                }
+                for (int kk = 0; kk < KM_KEYS / 16; kk++)                // (two weights a column of TMEM)
+                    km_mma_ts(tO0 + i * D, tS0 + i * 128 + kk * 8, dv + (uint64_t)place * (HT >> 4) + (uint64_t)kk * (2048u >> 4), idesc_pv,
+                              (accumulate || kk > 0) ? 1u : 0u);
                 tc_commit(pv_done + 8 * i);
             };
             bool ok = true;
-            uint32_t gs = 0, g_tile0 = 0, g_tile1 = 0, q_uses0 = 0, q_uses1 = 0;      // steps so far, per query tile, and items per query tile
+            uint32_t gs = 0, g_tile0 = 0, g_tile1 = 0, q_uses0 = 0, q_uses1 = 0;      // steps so far, per query tile, and pieces per query tile
             Walk walk = {x_start, first_tile, first_before};
             for (Item it; ok && item_of(walk, it);) {
                 if (it.n_kt0 > 0) ok = mbar_wait(q_ready, q_uses0++ & 1, abort_flag, err);
                 if (ok && it.n_kt1 > 0) ok = mbar_wait(q_ready + 8, q_uses1++ & 1, abort_flag, err);
-                if (ok) ok = mbar_wait(k_full, gs & 1, abort_flag, err);
+                if (ok) ok = mbar_wait(k_full + 8 * (gs & 1), (gs >> 1) & 1, abort_flag, err);
                 if (ok) {
                     tc_fence_after();
-                    if (it.n_kt0 > 0) issue_s(0);
-                    if (it.n_kt1 > 0) issue_s(1);
-                    tc_commit(k_empty);
+                    if (it.n_kt0 > 0) issue_s(0, gs & 1);
+                    if (it.n_kt1 > 0) issue_s(1, gs & 1);
+                    tc_commit(k_empty + 8 * (gs & 1));
                 }
                 for (int j = 0; j < it.n_kt && ok; j++, gs++) {
-                    // per query tile: the scores of step j + 1 as soon as those of step j have been read for the last time, then the
-                    // outputs of step j, whose last weights follow shortly
-                    const bool more = j + 1 < it.n_kt;
-                    if (more) ok = mbar_wait(k_full, (gs + 1) & 1, abort_flag, err);
+                    const uint32_t here = gs & 1, next = here ^ 1;
+                    ok = mbar_wait(v_full + 8 * here, (gs >> 1) & 1, abort_flag, err);
+                    if (ok && j + 1 < it.n_kt) ok = mbar_wait(k_full + 8 * next, ((gs + 1) >> 1) & 1, abort_flag, err);
+                    // per query tile: the outputs of step j, then the scores of step j + 1 in the place of the weights
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
                         const int n = i ? it.n_kt1 : it.n_kt0;
-                        const uint32_t ph = ((i ? g_tile1 : g_tile0) + j) & 1;
-                        if (ok && j + 1 < n) {
-                            ok = mbar_wait(s_free + 8 * i, ph, abort_flag, err);
-                            if (ok) { tc_fence_after(); issue_s(i); }
-                        }
-                        if (ok && more && i == 1) tc_commit(k_empty);
-                        if (ok && i == 0) ok = mbar_wait(v_full, gs & 1, abort_flag, err);
                         if (ok && j < n) {
-                            ok = mbar_wait(p_ready + 8 * i, ph, abort_flag, err);
-                            if (ok) { tc_fence_after(); issue_pv(i, j > 0); }
+                            ok = mbar_wait(p_ready + 8 * i, ((i ? g_tile1 : g_tile0) + j) & 1, abort_flag, err);
+                            if (ok) {
+                                tc_fence_after();
+                                issue_pv(i, here, j > 0);
+                                if (j + 1 < n) issue_s(i, next);
+                            }
                         }
                     }
                     if (!ok) break;
-                    tc_commit(v_empty);
+                    tc_commit(v_empty + 8 * here);
+                    if (j + 1 < it.n_kt) tc_commit(k_empty + 8 * next);
                 }
                 g_tile0 += it.n_kt0; g_tile1 += it.n_kt1;
             }
             // nothing of this CTA's is in flight once the last release of V has landed
-            if (ok && gs > 0) mbar_wait(v_empty, (gs - 1) & 1, abort_flag, err);
+            if (ok && gs > 0) mbar_wait(v_empty + 8 * ((gs - 1) & 1), ((gs - 1) >> 1) & 1, abort_flag, err);
         }
     } else if (warp >= 8) {
         // ---- codes into operands: a warp has a quarter of a tile's keys, a lane one of them ----------------------------------------
@@ -332,34 +336,27 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
             fetch(page, k_in, stK, 0);
             fetch(page, v_in, stV, page_bytes);
             float2 sc = scales_of(0, page);
-            int next = page_of(1);                                        // the pages of step j + 1; `page`: of step j
-            for (int j = 0; j <= it.n_kt && ok; j++) {
-                // keys of step j, then values of step j - 1: the keys' place is free early in a step, the values' at its end
-                if (j < it.n_kt) {
-                    const uint32_t g = gs + j, b = g & 1, at = sS + b * 1024u + 4u * row;
-                    ok = mbar_wait(sc_empty + 8 * b, ((g >> 1) & 1) ^ 1, abort_flag, err);
-                    if (!ok) break;
-                    asm volatile("st.shared.f32 [%0], %1;\n\tst.shared.f32 [%0 + 512], %2;" ::"r"(at), "f"(sc.x), "f"(sc.y) : "memory");
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(sc_full + 8 * b);
-                    ok = mbar_wait(k_in, g & 1, abort_flag, err) && mbar_wait(k_empty, (g & 1) ^ 1, abort_flag, err);
-                    if (!ok) break;
-                    convert(stK, sK);
-                    if (lane == 0) mbar_arrive(k_full);
-                    if (j + 1 < it.n_kt) {
-                        fetch(next, k_in, stK, 0);
-                        sc = scales_of(j + 1, next);
-                    }
+            int next = page_of(1);                                        // the pages of step j + 1
+            for (int j = 0; j < it.n_kt && ok; j++) {
+                const uint32_t g = gs + j, b = g & 1, ph = (g >> 1) & 1, at = sS + b * 1024u + 4u * row;
+                ok = mbar_wait(sc_empty + 8 * b, ph ^ 1, abort_flag, err);
+                if (!ok) break;
+                asm volatile("st.shared.f32 [%0], %1;\n\tst.shared.f32 [%0 + 512], %2;" ::"r"(at), "f"(sc.x), "f"(sc.y) : "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(sc_full + 8 * b);
+                ok = mbar_wait(k_in, g & 1, abort_flag, err) && mbar_wait(k_empty + 8 * b, ph ^ 1, abort_flag, err);
+                if (!ok) break;
+                convert(stK, sK + b * HT);
+                if (lane == 0) mbar_arrive(k_full + 8 * b);
+                if (j + 1 < it.n_kt) {
+                    fetch(next, k_in, stK, 0);
+                    sc = scales_of(j + 1, next);
                 }
-                if (j > 0) {
-                    const uint32_t g = gs + j - 1;
-                    ok = mbar_wait(v_in, g & 1, abort_flag, err) && mbar_wait(v_empty, (g & 1) ^ 1, abort_flag, err);
-                    if (!ok) break;
-                    convert(stV, sV);
-                    if (lane == 0) mbar_arrive(v_full);
-                    if (j < it.n_kt) fetch(page, v_in, stV, page_bytes);
-                }
-                page = next;
+                ok = mbar_wait(v_in, g & 1, abort_flag, err) && mbar_wait(v_empty + 8 * b, ph ^ 1, abort_flag, err);
+                if (!ok) break;
+                convert(stV, sV + b * HT);
+                if (lane == 0) mbar_arrive(v_full + 8 * b);
+                if (j + 1 < it.n_kt) fetch(next, v_in, stV, page_bytes);
                 next = page_of(j + 2);
             }
             gs += it.n_kt;
@@ -421,7 +418,7 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                     if (lane == 0) mbar_arrive(sc_empty + 8 * b);
                     continue;
                 }
-                const uint32_t ph = (g_mine + j) & 1;
+                const uint32_t ph = (g_mine + j) & 1;                    // (O holds everything up to the step before once these scores are there)
                 const int key0 = (it.kt_lo + j) * KM_KEYS;
                 {
                     const float4 v = km_load4(s_at + 512u + 16u * lane);
@@ -515,21 +512,15 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                     corr = ref == -INFINITY ? 0.f : km_ex2(ref - mx);
                     ref = mx;
                 }
-                if (j > 0) {
-                    // P of the step before has been used, and O holds everything up to it
-                    if (!mbar_wait(pv_done + 8 * i, ph ^ 1, abort_flag, err)) { ok = false; break; }
-                    tc_fence_after();
-                    if (__any_sync(0xffffffffu, corr != 1.f)) {
+                if (j > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
 #pragma unroll 1
-                        for (int c = 0; c < D / 16; c++) {
-                            uint32_t ov[16];
-                            tmem_ld16(tO + 16 * c, ov);
-                            tmem_wait_ld();
+                    for (int c = 0; c < D / 16; c++) {
+                        uint32_t ov[16];
+                        tmem_ld16(tO + 16 * c, ov);
+                        tmem_wait_ld();
 #pragma unroll
-                            for (int e = 0; e < 16; e++) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * corr);
-                            km_st16(tO + 16 * c, ov);
-                        }
-                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                        for (int e = 0; e < 16; e++) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * corr);
+                        km_st16(tO + 16 * c, ov);
                     }
                 }
                 const float minus = ref == -INFINITY ? 0.f : -ref;
@@ -552,21 +543,14 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                             pk[c / 2] = km_pack(wa.x, wa.y);
                             pk[c / 2 + 1] = km_pack(wb.x, wb.y);
                         }
-#pragma unroll
-                        for (int q = 0; q < 4; q++) km_store16(sP + i * KM_TILE + km_off(row, c0 / 8 + q), pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
+                        km_st16(tS + c0 / 2, pk);                        // (over scores that have been read)
                     };
 #pragma unroll 1
                     for (int c0 = 0; c0 < 128; c0 += 64) {
                         load32(c0 + 32, rb);
                         weights(c0, ra);
                         km_wait(rb);
-                        if (c0 == 0) {
-                            load32(64, ra);
-                        } else {
-                            tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(s_free + 8 * i);  // the tensor core may write the next scores
-                        }
+                        if (c0 == 0) load32(64, ra);
                         weights(c0 + 32, rb);
                         if (c0 == 0) km_wait(ra);
                     }
@@ -575,11 +559,6 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                 for (int c0 = 0; c0 < 128; c0 += 32) {
                     f32pair x[16];
                     scores(c0, x);
-                    if (c0 == 96) {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(s_free + 8 * i);      // the tensor core may write the next scores
-                    }
                     uint32_t pk[16];
 #pragma unroll
                     for (int c = 0; c < 16; c += 2) {
@@ -598,14 +577,14 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                             pk[c + u] = km_pack(w.x, w.y);
                         }
                     }
-#pragma unroll
-                    for (int q = 0; q < 4; q++) km_store16(sP + i * KM_TILE + km_off(row, c0 / 8 + q), pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
+                    __syncwarp();
+                    km_st16(tS + c0 / 2, pk);
                 }
                 {
                     const float2 s0 = halves(sum[0]), s1 = halves(sum[1]);
                     l = l * corr + ((s0.x + s0.y) + (s1.x + s1.y));
                 }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) { mbar_arrive(sc_empty + 8 * b); mbar_arrive(p_ready + 8 * i); }
