@@ -4,8 +4,10 @@
 // s_j = scale (q . code_j) ks_j, out = sum_j p_j vs_j code'_j / sum_j p_j.  The exponentials bound it (128 x 128 of them for every pair of
 // products of 128 x 128 x d), so nothing of the 8 bits is left to the threads that compute them but two factors:
 // * four warps of their own turn codes into float16 (exact: whole numbers below 2^11) in the layout of the tensor core's operands, 32 keys
-//   each of a tile of 128, while the softmax of the tile before runs.  Each fetches its keys' codes itself, by bulk copies as soon as it
-//   has read the last ones.  Both operands have two places, so that the conversion runs a tile ahead of the products.
+//   each of a tile of 128, while the softmax of the tile before runs.  A thread owns a key: it asks for its
+//   codes of the next tile as soon as it has converted the last ones, and keeps them in registers.  (From a staging buffer, filled by bulk
+//   copies, every step waited for a copy of its own: 420 us where this takes ###.)  Both operands have two places, so that the
+//   conversion runs a tile ahead of the products.
 // * the scales stay out of the operands: a score is multiplied by its key's, a weight by its value's, in float32, both read as
 //   broadcasts from shared memory.
 // * queries are multiplied by the power of two that brings a row's largest number to 2^14..2^15 (kv8_few.cu).
@@ -40,7 +42,7 @@ struct Kv8ManyParams {
     int *counters;                                   // ... one per (double tile, head, query tile), zero between launches
 };
 
-template <int D> constexpr uint32_t km_smem() { return 6 * (D / 64) * KM_SUB + 2 * KM_KEYS * D + 2048 + 256; }
+template <int D> constexpr uint32_t km_smem() { return 6 * (D / 64) * KM_SUB + 2048 + 256; }
 
 __device__ __forceinline__ uint32_t km_off(int row, int c16)
 {
@@ -102,11 +104,6 @@ __device__ __forceinline__ float km_load1(uint32_t addr)
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
     return v;
 }
-__device__ __forceinline__ void km_bulk(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
-{
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
-}
 
 template <int D>
 __global__ void __launch_bounds__(KM_THREADS, 1)
@@ -117,21 +114,15 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
     const uint32_t base = (smem_u32(km_raw) + 1023u) & ~1023u;
     uint8_t *gen = km_raw + (base - smem_u32(km_raw));
     constexpr uint32_t HT = (D / 64) * KM_SUB;       // a [128 x D] float16 operand: Q, K or V
-    constexpr uint32_t CODES = KM_KEYS * D;          // a tile's key (or value) codes
-    const uint32_t sQ = base, sK = base + 2 * HT, sV = base + 4 * HT, stK = base + 6 * HT, stV = stK + CODES;      // (keys and values: two each)
-    const uint32_t sS = stV + CODES;                 // [2][keys' scales 128 | values' scales 128]
+    const uint32_t sQ = base, sK = base + 2 * HT, sV = base + 4 * HT;         // (keys and values: two each)
+    const uint32_t sS = base + 6 * HT;               // [2][keys' scales 128 | values' scales 128]
     const uint32_t bars = sS + 2048;
     const uint32_t q_ready = bars, s_full = bars + 16, p_ready = bars + 32, pv_done = bars + 48;                          // + 8 * query tile
-    const uint32_t k_st_full = bars + 80, v_st_full = bars + 112;                                                         // + 8 * quarter
     const uint32_t k_full = bars + 144, k_empty = bars + 160, v_full = bars + 176, v_empty = bars + 192;                  // + 8 * place
     const uint32_t sc_full = bars + 208, sc_empty = bars + 64;                                                            // + 8 * buffer
     volatile uint32_t *tmem_slot = (volatile uint32_t *)(gen + (bars - base) + 224);
     volatile int *abort_flag = (volatile int *)(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (base - smem_u32(km_raw) > (D == 128 ? 768u : 1024u)) {           // (see the launch)
-        if (threadIdx.x == 0) atomicOr(err, HFB_ERR_WAIT);
-        return;
-    }
     if (!f.settled) pdl_wait();                      // nothing is read that the kernels in front may still write
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; i++) {
@@ -139,7 +130,6 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
             mbar_init(k_full + 8 * i, 4); mbar_init(v_full + 8 * i, 4); mbar_init(k_empty + 8 * i, 1); mbar_init(v_empty + 8 * i, 1);
             mbar_init(sc_full + 8 * i, 4); mbar_init(sc_empty + 8 * i, 8);
         }
-        for (int i = 0; i < 4; i++) { mbar_init(k_st_full + 8 * i, 1); mbar_init(v_st_full + 8 * i, 1); }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -287,21 +277,14 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
         }
     } else if (warp >= 8) {
         // ---- codes into operands: a warp has a quarter of a tile's keys, a lane one of them ----------------------------------------
-        const int part = bs < 32 ? bs : 32, copies = 32 / part;                     // keys of one copy: a page of the quarter, or half a page
         const int row = (warp - 8) * 32 + lane;
-        const uint32_t part_bytes = part * D, page_bytes = bs * D, k_in = k_st_full + 8 * (warp - 8), v_in = v_st_full + 8 * (warp - 8);
-        auto convert = [&](uint32_t from, uint32_t to) {
-            uint4 w[D / 16];
-#pragma unroll
-            for (int c = 0; c < D / 16; c++)
-                asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[c].x), "=r"(w[c].y), "=r"(w[c].z), "=r"(w[c].w)
-                             : "r"(from + (uint32_t)row * D + (uint32_t)kv8_piece(row % bs, c, D) * 16u));
+        auto convert = [&](const uint4 (&w)[D / 16], uint32_t to) {
 #pragma unroll
             for (int c = 0; c < D / 16; c++) {
                 km_store16(to + km_off(row, 2 * c), km_codes(w[c].x, 0x4140), km_codes(w[c].x, 0x4342), km_codes(w[c].y, 0x4140), km_codes(w[c].y, 0x4342));
                 km_store16(to + km_off(row, 2 * c + 1), km_codes(w[c].z, 0x4140), km_codes(w[c].z, 0x4342), km_codes(w[c].w, 0x4140), km_codes(w[c].w, 0x4342));
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (also: the staging has been read before it is written again)
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
         };
         bool ok = true;
@@ -309,34 +292,33 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
         Walk walk = {x_start, first_tile, first_before};
         for (Item it; ok && item_of(walk, it);) {
             const int32_t *table = p.block_table + (size_t)it.seq * p.max_blocks;
-            // the page of step j that this lane asks for, -1 where there is none to be read
+            // the page of this thread's key in step j; -1 where there is none to be read (behind the last, passed by every row's mask, no page)
             auto page_of = [&](int j) {
-                const int key0 = (it.kt_lo + j) * KM_KEYS + (warp - 8) * 32 + lane * part, blk = key0 / bs;
-                if (j >= it.n_kt || lane >= copies || key0 > it.pos_last || key0 + part <= it.lo_first) return -1;
+                const int key = (it.kt_lo + j) * KM_KEYS + row, blk = key / bs;
+                if (j >= it.n_kt || key > it.pos_last || key < it.lo_first) return -1;
                 const int page = blk < p.max_blocks ? table[blk] : -1;
                 if (page < 0 || page >= p.num_pages) { atomicOr(err, HFB_ERR_PAGE); return -1; }
                 return page;
             };
-            auto fetch = [&](int page, uint32_t bar, uint32_t dst, uint32_t skip) {
-                const int n = __popc(__ballot_sync(0xffffffffu, page >= 0));
-                if (lane == 0) mbar_arrive_expect_tx(bar, n * part_bytes);
-                __syncwarp();
-                const uint32_t first = (uint32_t)((warp - 8) * 32 + lane * part);          // row of the tile
-                if (page >= 0) km_bulk(dst + first * D, p.cache + ((size_t)page * p.G + it.g) * p.record + skip + (first % bs) * D, part_bytes, bar);
+            const int in_page = row % bs;                                 // (tiles begin on pages)
+            auto record_of = [&](int page) { return p.cache + ((size_t)page * p.G + it.g) * p.record; };
+            auto load = [&](int page, int skip, uint4 (&w)[D / 16]) {
+                const uint8_t *src = record_of(max(page, 0)) + skip + in_page * D;
+#pragma unroll
+                for (int c = 0; c < D / 16; c++)
+                    w[c] = page >= 0 ? *(const uint4 *)(src + kv8_piece(in_page, c, D) * 16) : make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
             };
-            // a key's scales; where it is not to be read (behind the last, passed by every row's mask, no page) 0 and -1
-            auto scales_of = [&](int j, int page) {
-                const int key = (it.kt_lo + j) * KM_KEYS + row;
-                const int its = __shfl_sync(0xffffffffu, page, lane / part);
-                if (its < 0 || key > it.pos_last || key < it.lo_first) return make_float2(0.f, -1.f);
-                const float *s = (const float *)(p.cache + ((size_t)its * p.G + it.g) * p.record + 2 * bs * D) + row % bs;
+            auto scales_of = [&](int page) {                              // (-1 tells the softmax that there is no such key)
+                if (page < 0) return make_float2(0.f, -1.f);
+                const float *s = (const float *)(record_of(page) + 2 * bs * D) + in_page;
                 return make_float2(s[0], s[bs]);
             };
             int page = page_of(0);
-            fetch(page, k_in, stK, 0);
-            fetch(page, v_in, stV, page_bytes);
-            float2 sc = scales_of(0, page);
-            int next = page_of(1);                                        // the pages of step j + 1
+            uint4 k[D / 16], v[D / 16];
+            load(page, 0, k);
+            load(page, bs * D, v);
+            float2 sc = scales_of(page);
+            page = page_of(1);
             for (int j = 0; j < it.n_kt && ok; j++) {
                 const uint32_t g = gs + j, b = g & 1, ph = (g >> 1) & 1, at = sS + b * 1024u + 4u * row;
                 ok = mbar_wait(sc_empty + 8 * b, ph ^ 1, abort_flag, err);
@@ -344,20 +326,16 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                 asm volatile("st.shared.f32 [%0], %1;\n\tst.shared.f32 [%0 + 512], %2;" ::"r"(at), "f"(sc.x), "f"(sc.y) : "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(sc_full + 8 * b);
-                ok = mbar_wait(k_in, g & 1, abort_flag, err) && mbar_wait(k_empty + 8 * b, ph ^ 1, abort_flag, err);
-                if (!ok) break;
-                convert(stK, sK + b * HT);
+                if (!mbar_wait(k_empty + 8 * b, ph ^ 1, abort_flag, err)) { ok = false; break; }
+                convert(k, sK + b * HT);
                 if (lane == 0) mbar_arrive(k_full + 8 * b);
-                if (j + 1 < it.n_kt) {
-                    fetch(next, k_in, stK, 0);
-                    sc = scales_of(j + 1, next);
-                }
-                ok = mbar_wait(v_in, g & 1, abort_flag, err) && mbar_wait(v_empty + 8 * b, ph ^ 1, abort_flag, err);
-                if (!ok) break;
-                convert(stV, sV + b * HT);
+                load(page, 0, k);                                         // (of step j + 1)
+                sc = scales_of(page);
+                if (!mbar_wait(v_empty + 8 * b, ph ^ 1, abort_flag, err)) { ok = false; break; }
+                convert(v, sV + b * HT);
                 if (lane == 0) mbar_arrive(v_full + 8 * b);
-                if (j + 1 < it.n_kt) fetch(next, v_in, stV, page_bytes);
-                next = page_of(j + 2);
+                load(page, bs * D, v);
+                page = page_of(j + 2);
             }
             gs += it.n_kt;
         }
@@ -701,10 +679,6 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
     // ---- teardown -------------------------------------------------------------------------------------------------------------------
     tc_fence_before();
     __syncthreads();
-    if (*abort_flag && threadIdx.x == 0) {
-        for (int i = 0; i < 2000; i++) __nanosleep(1000);              // let copies still in flight land
-    }
-    __syncthreads();
     if (warp == 12) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(KM_TMEM_COLS) : "memory");
@@ -714,7 +688,7 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
 template <int D>
 static int launch_kv8_many(const Kv8ManyParams &f, int grid, cudaStream_t st)
 {
-    constexpr uint32_t smem = km_smem<D>() + (D == 128 ? 768 : 1024);    // (the tiles begin on a multiple of 1,024; shared memory does after the first)
+    constexpr uint32_t smem = km_smem<D>() + 1024;                       // (the tiles begin on a multiple of 1,024)
     static_assert(smem <= 227 * 1024, "the tiles do not fit");
     static bool configured[64] = {false};                                // (the opt-in is a property of the function on one device)
     if (!configured[current_device()]) {
