@@ -2,22 +2,25 @@
 // tokens, two tiles of 128 query rows a CTA.
 //
 // s_j = scale (q . code_j) ks_j, out = sum_j p_j vs_j code'_j / sum_j p_j.  The exponentials bound it (128 x 128 of them for every pair of
-// products of 128 x 128 x d), so nothing of the 8 bits is left to the threads that compute them but two factors:
-// * four warps of their own turn codes into float16 (exact: whole numbers below 2^11) in the layout of the tensor core's operands, 32 keys
-//   each of a tile of 128, while the softmax of the tile before runs.  A thread owns a key: it asks for its
-//   codes of the next tile as soon as it has converted the last ones, and keeps them in registers.  (From a staging buffer, filled by bulk
-//   copies, every step waited for a copy of its own: 420 us where this takes ###.)  Both operands have two places, so that the
-//   conversion runs a tile ahead of the products.
-// * the scales stay out of the operands: a score is multiplied by its key's, a weight by its value's, in float32, both read as
-//   broadcasts from shared memory.
+// products of 128 x 128 x d), so nothing of the 8 bits is left to the threads that compute them:
+// * four warps of their own turn codes into float16 numbers, code * (scale / reference), in the layout of the tensor core's operands, 32 keys
+//   each of a tile of 128, while the softmax of the tile before runs.  The reference is the power of two above the largest scale of the 32
+//   keys, which is left to the softmax as one factor for 32 columns.  A number is rounded once to 11 bits (keys; their scale goes in as
+//   a sum of two float16) or, with its scale, twice (values); half a step is 2^-11 of the number, an eighth of what bfloat16 keys and
+//   values lose.  (Scales applied to scores and weights in float32 instead took two reads of shared memory for every four scores: each
+//   brings a thread 16 bytes, 512 a warp, and those reads alone were 4,700 of 9,400 cycles a step: 436 us where this takes ###.)
+// * a thread owns a key: it asks for its codes of the next tile as soon as it has converted the last ones, and keeps them in registers.
+//   Both operands have two places, so that the conversion runs a tile ahead of the products.
+// * a row whose key or value is no number makes its scores so and leaves its values zero: a weight of zero stays zero in the sums of the
+//   rows that do not see it.
 // * queries are multiplied by the power of two that brings a row's largest number to 2^14..2^15 (kv8_few.cu).
-// * a row's exponentials refer to R = (largest score) + log2(largest value scale) - 10: 2^(s - R) vs is at most 2^14 before R is raised, and
-//   is rounded once to float16.  Both sums carry the factor, which cancels.  R is raised, and the sums so far rescaled (the output in
-//   TMEM), only when it has been outgrown by 2^4.  (log2 of the scale is taken as -90 at least: smaller values are zeros.)
-// * a row belongs to one thread, which reads its scores from TMEM twice, 32 at a time, for the maximum and for the weights (128 at once
-//   beside their scales do not fit the registers of thirteen warps).  The weights go back to TMEM in the scores' place, as the second
-//   product's left operand; O lives in TMEM too.  One query tile's softmax runs beside the other's products: its own next scores follow its
-//   outputs in the tensor core's order, which is all that keeps them off the weights.
+// * a row's exponentials refer to R = (largest score + log2 of its value reference) - 10: a weight 2^(s - R) reference is at most 2^14
+//   before R is raised, and is rounded once to float16.  Both sums carry the factor, which cancels.  R is raised, and the sums so far
+//   rescaled (the output in TMEM), only when it has been outgrown by 2^4.  (Values below 2^-90 are zeros.)
+// * a row belongs to one thread, which reads its scores from TMEM twice, 32 at a time, for the maximum and for the weights.  The weights
+//   go back to TMEM in the scores' place, as the second product's left operand; O lives in TMEM too.  One query tile's softmax runs
+//   beside the other's products: its own next scores follow its outputs in the tensor core's order, which is all that keeps them off
+//   the weights.
 // * work is cut evenly (as in kv8_few.cu): a step is a tile of keys of one double tile and key/value head, CTA c of C walks steps c N / C to
 //   (c + 1) N / C.  What a CTA has of a double tile that others share goes to scratch, and whoever brings its last piece merges them, in
 //   the order of the keys.  (Whole double tiles a CTA: 228 items of 2,048 tokens and 28 heads are two rounds on 148 SMs where 1.5 would do.)
@@ -42,7 +45,7 @@ struct Kv8ManyParams {
     int *counters;                                   // ... one per (double tile, head, query tile), zero between launches
 };
 
-template <int D> constexpr uint32_t km_smem() { return 6 * (D / 64) * KM_SUB + 2048 + 256; }
+template <int D> constexpr uint32_t km_smem() { return 6 * (D / 64) * KM_SUB + 128 + 256; }
 
 __device__ __forceinline__ uint32_t km_off(int row, int c16)
 {
@@ -98,12 +101,6 @@ __device__ __forceinline__ void km_wait(uint32_t (&v)[32])
     asm volatile("" : KM_REGS(16), KM_REGS(24)::"memory");
 #undef KM_REGS
 }
-__device__ __forceinline__ float km_load1(uint32_t addr)
-{
-    float v;
-    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
-    return v;
-}
 
 template <int D>
 __global__ void __launch_bounds__(KM_THREADS, 1)
@@ -115,8 +112,8 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
     uint8_t *gen = km_raw + (base - smem_u32(km_raw));
     constexpr uint32_t HT = (D / 64) * KM_SUB;       // a [128 x D] float16 operand: Q, K or V
     const uint32_t sQ = base, sK = base + 2 * HT, sV = base + 4 * HT;         // (keys and values: two each)
-    const uint32_t sS = base + 6 * HT;               // [2][keys' scales 128 | values' scales 128]
-    const uint32_t bars = sS + 2048;
+    const uint32_t sS = base + 6 * HT;               // [2][16]: per quarter of a tile the keys' reference, log2 of the values', the keys there are
+    const uint32_t bars = sS + 128;
     const uint32_t q_ready = bars, s_full = bars + 16, p_ready = bars + 32, pv_done = bars + 48;                          // + 8 * query tile
     const uint32_t k_full = bars + 144, k_empty = bars + 160, v_full = bars + 176, v_empty = bars + 192;                  // + 8 * place
     const uint32_t sc_full = bars + 208, sc_empty = bars + 64;                                                            // + 8 * buffer
@@ -135,7 +132,7 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     // ---- this CTA's steps -------------------------------------------------------------------------------------------------------
-    const int r = p.H / p.G, bs = p.block_size, pages = KM_KEYS / bs;
+    const int r = p.H / p.G, bs = p.block_size;
     struct Tile { int seq, t0, nt, pos_last, lo_first, kt_lo, n_kt0, n_kt; };
     auto tile_of = [&](int i) {
         Tile x;
@@ -278,11 +275,17 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
     } else if (warp >= 8) {
         // ---- codes into operands: a warp has a quarter of a tile's keys, a lane one of them ----------------------------------------
         const int row = (warp - 8) * 32 + lane;
-        auto convert = [&](const uint4 (&w)[D / 16], uint32_t to) {
+        // code * (hi + lo), or code * hi
+        auto convert = [&](const uint4 (&w)[D / 16], uint32_t to, __half2 hi, __half2 lo, bool both) {
+            auto number = [&](uint32_t word, uint32_t selector) {
+                const uint32_t bits = km_codes(word, selector);
+                const __half2 c = *(const __half2 *)&bits, r = both ? __hfma2(c, hi, __hmul2(c, lo)) : __hmul2(c, hi);
+                return *(const uint32_t *)&r;
+            };
 #pragma unroll
             for (int c = 0; c < D / 16; c++) {
-                km_store16(to + km_off(row, 2 * c), km_codes(w[c].x, 0x4140), km_codes(w[c].x, 0x4342), km_codes(w[c].y, 0x4140), km_codes(w[c].y, 0x4342));
-                km_store16(to + km_off(row, 2 * c + 1), km_codes(w[c].z, 0x4140), km_codes(w[c].z, 0x4342), km_codes(w[c].w, 0x4140), km_codes(w[c].w, 0x4342));
+                km_store16(to + km_off(row, 2 * c), number(w[c].x, 0x4140), number(w[c].x, 0x4342), number(w[c].y, 0x4140), number(w[c].y, 0x4342));
+                km_store16(to + km_off(row, 2 * c + 1), number(w[c].z, 0x4140), number(w[c].z, 0x4342), number(w[c].w, 0x4140), number(w[c].w, 0x4342));
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -308,8 +311,8 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                 for (int c = 0; c < D / 16; c++)
                     w[c] = page >= 0 ? *(const uint4 *)(src + kv8_piece(in_page, c, D) * 16) : make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
             };
-            auto scales_of = [&](int page) {                              // (-1 tells the softmax that there is no such key)
-                if (page < 0) return make_float2(0.f, -1.f);
+            auto scales_of = [&](int page) {
+                if (page < 0) return make_float2(0.f, 0.f);
                 const float *s = (const float *)(record_of(page) + 2 * bs * D) + in_page;
                 return make_float2(s[0], s[bs]);
             };
@@ -318,23 +321,35 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
             load(page, 0, k);
             load(page, bs * D, v);
             float2 sc = scales_of(page);
+            bool there = page >= 0;
             page = page_of(1);
             for (int j = 0; j < it.n_kt && ok; j++) {
-                const uint32_t g = gs + j, b = g & 1, ph = (g >> 1) & 1, at = sS + b * 1024u + 4u * row;
+                const uint32_t g = gs + j, b = g & 1, ph = (g >> 1) & 1, at = sS + b * 64u + 4u * (warp - 8);
+                // the references: powers of two above the largest scales (maxima pass by what is no number)
+                const uint32_t kf = min((__float_as_uint(warp_max(fmaxf(sc.x, 0.f))) >> 23) + 1u, 253u);
+                const uint32_t vf = max(min((__float_as_uint(warp_max(fmaxf(sc.y, 0.f))) >> 23) + 1u, 253u), 37u);           // 2^-90
+                const bool number = sc.x == sc.x && sc.y == sc.y;
+                const float ks = number ? sc.x * __uint_as_float((254u - kf) << 23) : __uint_as_float(0x7fc00000u);
+                const __half k_hi = __float2half_rn(ks), k_lo = __float2half_rn(ks - __half2float(k_hi));
+                const __half v_hi = __float2half_rn(number ? sc.y * __uint_as_float((254u - vf) << 23) : 0.f);
+                const uint32_t present = __ballot_sync(0xffffffffu, there);
                 ok = mbar_wait(sc_empty + 8 * b, ph ^ 1, abort_flag, err);
                 if (!ok) break;
-                asm volatile("st.shared.f32 [%0], %1;\n\tst.shared.f32 [%0 + 512], %2;" ::"r"(at), "f"(sc.x), "f"(sc.y) : "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(sc_full + 8 * b);
+                if (lane == 0) {
+                    asm volatile("st.shared.f32 [%0], %1;\n\tst.shared.f32 [%0 + 16], %2;\n\tst.shared.u32 [%0 + 32], %3;"
+                                 ::"r"(at), "f"(__uint_as_float(kf << 23)), "f"((float)vf - 127.f), "r"(present) : "memory");
+                    mbar_arrive(sc_full + 8 * b);
+                }
                 if (!mbar_wait(k_empty + 8 * b, ph ^ 1, abort_flag, err)) { ok = false; break; }
-                convert(k, sK + b * HT);
+                convert(k, sK + b * HT, __half2half2(k_hi), __half2half2(k_lo), true);
                 if (lane == 0) mbar_arrive(k_full + 8 * b);
                 load(page, 0, k);                                         // (of step j + 1)
                 sc = scales_of(page);
                 if (!mbar_wait(v_empty + 8 * b, ph ^ 1, abort_flag, err)) { ok = false; break; }
-                convert(v, sV + b * HT);
+                convert(v, sV + b * HT, __half2half2(v_hi), __half2half2(v_hi), false);
                 if (lane == 0) mbar_arrive(v_full + 8 * b);
                 load(page, bs * D, v);
+                there = page >= 0;
                 page = page_of(j + 2);
             }
             gs += it.n_kt;
@@ -388,9 +403,9 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
             const float hscale = (p.head_scales && valid) ? p.head_scales[it.g * r + hl] : 1.f;
             const bool capped = p.softcap > 0.f, finished = capped || p.slopes || p.head_scales;     // (scores are finished in place)
             const float cap_in = capped ? unit * hscale / (p.softcap * log2e) : 0.f, cap2 = p.softcap * log2e;
-            float ref = -INFINITY, l = 0.f, vm = 0.f;                    // what the exponentials refer to, their sum, largest scale so far
+            float ref = -INFINITY, l = 0.f;                              // what the exponentials refer to, their sum
             for (int j = 0; j < it.n_kt && ok; j++) {
-                const uint32_t b = (gs + j) & 1, sc_ph = ((gs + j) >> 1) & 1, s_at = sS + b * 1024u;
+                const uint32_t b = (gs + j) & 1, sc_ph = ((gs + j) >> 1) & 1, s_at = sS + b * 64u;
                 if (!mbar_wait(sc_full + 8 * b, sc_ph, abort_flag, err)) { ok = false; break; }
                 if (j >= n_mine) {                                       // (the other query tile's step)
                     if (lane == 0) mbar_arrive(sc_empty + 8 * b);
@@ -398,93 +413,79 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                 }
                 const uint32_t ph = (g_mine + j) & 1;                    // (O holds everything up to the step before once these scores are there)
                 const int key0 = (it.kt_lo + j) * KM_KEYS;
-                {
-                    const float4 v = km_load4(s_at + 512u + 16u * lane);
-                    vm = fmaxf(vm, warp_max(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w))));
-                }
                 if (!mbar_wait(s_full + 8 * i, ph, abort_flag, err)) { ok = false; break; }
                 tc_fence_after();
-                // (rows beyond the tile's tokens go with the rows that see every key); a missing page's values have the scale -1
-                bool gap = false;
-                if (lane < pages) gap = km_load1(s_at + 512u + 4u * (lane * bs + bs - 1)) == -1.f;
-                gap = __any_sync(0xffffffffu, gap);
-                const bool all_visible = (!valid && !gap) || (key0 + KM_KEYS - 1 <= pos && key0 >= lo && !gap);
-                const float b0 = slope2 * (float)(key0 - pos), by_head = unit * hscale, sc = finished ? 1.f : unit;
-                // a step without options in which every row sees every key, as most are
-                const bool open = __all_sync(0xffffffffu, all_visible) && !finished;
+                // what the quarters of the tile share
+                const float4 kr = km_load4(s_at), lv = km_load4(s_at + 16u), there4 = km_load4(s_at + 32u);
+                const float k_ref[4] = {kr.x, kr.y, kr.z, kr.w}, v_log[4] = {lv.x, lv.y, lv.z, lv.w};
+                const uint32_t there[4] = {__float_as_uint(there4.x), __float_as_uint(there4.y), __float_as_uint(there4.z), __float_as_uint(there4.w)};
+                __syncwarp();
+                if (lane == 0) mbar_arrive(sc_empty + 8 * b);
+                // a step without options in which every row sees every key, as most are (rows beyond the tile's tokens go with those)
+                const bool full = (there[0] & there[1] & there[2] & there[3]) == 0xffffffffu;
+                const bool open = __all_sync(0xffffffffu, !valid || (key0 + KM_KEYS - 1 <= pos && key0 >= lo)) && full && !finished;
+                const float b0 = slope2 * (float)(key0 - pos), by_head = unit * hscale;
                 auto load32 = [&](int c0, uint32_t (&raw)[32]) { tmem_ld16(tS + c0, raw); tmem_ld16(tS + c0 + 16, raw + 16); };
-                auto by_scales = [&](int c0, const uint32_t (&raw)[32], int c, f32pair &a, f32pair &b) {
-                    const float4 k = km_load4(s_at + 4u * (c0 + c));
-                    a = mul2(pair_of(__uint_as_float(raw[c]), __uint_as_float(raw[c + 1])), pair_of(k.x, k.y));
-                    b = mul2(pair_of(__uint_as_float(raw[c + 2]), __uint_as_float(raw[c + 3])), pair_of(k.z, k.w));
-                };
-                // 32 scores from TMEM with their keys' scales, options and masks; what they lack is the factor sc > 0
-                auto scores = [&](int c0, f32pair (&x)[16]) {
-                    uint32_t raw[32];
-                    __syncwarp();
-                    load32(c0, raw);
-                    km_wait(raw);
+                // 32 finished scores (options, masks) in the exponent's base 2
+                auto finish = [&](int q, uint32_t (&raw)[32]) {
+                    const float in = capped ? cap_in * k_ref[q] : by_head * k_ref[q];
 #pragma unroll
-                    for (int c = 0; c < 32; c += 4) by_scales(c0, raw, c, x[c / 2], x[c / 2 + 1]);
-                    if (finished) {
-#pragma unroll
-                        for (int c = 0; c < 32; c += 2) {
-                            float2 v = halves(x[c / 2]);
-                            const float s0 = fmaf(slope2, (float)(c0 + c), b0), s1 = fmaf(slope2, (float)(c0 + c + 1), b0);
-                            v.x = capped ? fmaf(cap2, tanh_fast(v.x * cap_in), s0) : fmaf(v.x, by_head, s0);
-                            v.y = capped ? fmaf(cap2, tanh_fast(v.y * cap_in), s1) : fmaf(v.y, by_head, s1);
-                            x[c / 2] = pair_of(v.x, v.y);
-                        }
-                    }
-                    if (!all_visible) {
-#pragma unroll
-                        for (int c = 0; c < 32; c += 2) {
-                            float2 v = halves(x[c / 2]);
-                            const int key = key0 + c0 + c;
-                            if (!(valid && key >= lo && key <= pos) || (gap && km_load1(s_at + 512u + 4u * (c0 + c)) == -1.f)) v.x = -INFINITY;
-                            if (!(valid && key + 1 >= lo && key + 1 <= pos) || (gap && km_load1(s_at + 516u + 4u * (c0 + c)) == -1.f)) v.y = -INFINITY;
-                            x[c / 2] = pair_of(v.x, v.y);
-                        }
+                    for (int c = 0; c < 32; c++) {
+                        const int key = key0 + 32 * q + c;
+                        const float bias = fmaf(slope2, (float)(32 * q + c), b0), v = __uint_as_float(raw[c]);
+                        const float x = capped ? fmaf(cap2, tanh_fast(v * in), bias) : fmaf(v, in, bias);
+                        raw[c] = valid && key >= lo && key <= pos && (there[q] >> c & 1u) ? __float_as_uint(x) : 0xff800000u;
                     }
                 };
                 float mx = -INFINITY;
                 uint32_t ra[32], rb[32];
                 if (open) {
                     // (the next 32 are on their way while these are worked on)
-                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    auto largest = [&](int c0, const uint32_t (&raw)[32]) {
+                    auto largest = [&](int q, const uint32_t (&raw)[32]) {
+                        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                        for (int c = 0; c < 32; c += 4) {
-                            f32pair a, b;
-                            by_scales(c0, raw, c, a, b);
-                            const float2 x = halves(a), y = halves(b);
-                            top[(c >> 1) & 3] = fmaxf(top[(c >> 1) & 3], fmaxf(x.x, x.y));
-                            top[((c >> 1) + 1) & 3] = fmaxf(top[((c >> 1) + 1) & 3], fmaxf(y.x, y.y));
-                        }
+                        for (int c = 0; c < 32; c += 2)
+                            top[(c >> 1) & 3] = fmaxf(top[(c >> 1) & 3], fmaxf(__uint_as_float(raw[c]), __uint_as_float(raw[c + 1])));
+                        mx = fmaxf(mx, fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), unit * k_ref[q], v_log[q]));
                     };
-                    load32(0, ra);
-                    km_wait(ra);
-#pragma unroll 1
-                    for (int c0 = 0; c0 < 128; c0 += 64) {
-                        load32(c0 + 32, rb);
-                        largest(c0, ra);
-                        km_wait(rb);
-                        load32((c0 + 64) & 127, ra);                     // (the last time: for the weights)
-                        largest(c0 + 32, rb);
-                        km_wait(ra);
-                    }
-                    mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-                } else
-#pragma unroll 1
-                for (int c0 = 0; c0 < 128; c0 += 32) {
-                    f32pair x[16];
-                    scores(c0, x);
-                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    load32(0, ra); km_wait(ra);
+                    load32(32, rb); largest(0, ra); km_wait(rb);
+                    load32(64, ra); largest(1, rb); km_wait(ra);
+                    load32(96, rb); largest(2, ra); km_wait(rb);
+                    load32(0, ra); largest(3, rb); km_wait(ra);          // (for the weights)
+                } else if (p.slopes) {
 #pragma unroll
-                    for (int c = 0; c < 16; c++) { const float2 v = halves(x[c]); top[c & 3] = fmaxf(top[c & 3], fmaxf(v.x, v.y)); }
-                    mx = fmaxf(mx, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+                    for (int q = 0; q < 4; q++) {
+                        __syncwarp();
+                        load32(32 * q, ra);
+                        km_wait(ra);
+                        finish(q, ra);
+                        float top = -INFINITY;
+#pragma unroll
+                        for (int c = 0; c < 32; c++) top = fmaxf(top, __uint_as_float(ra[c]));
+                        mx = fmaxf(mx, top + v_log[q]);
+                    }
+                } else {
+                    // factors and a cap keep the order of the scores (or turn it round): the largest is found first and finished alone
+                    const float way = hscale < 0.f ? -1.f : 1.f;
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        __syncwarp();
+                        load32(32 * q, ra);
+                        km_wait(ra);
+                        float top = -INFINITY;
+#pragma unroll
+                        for (int c = 0; c < 32; c++) {
+                            const int key = key0 + 32 * q + c;
+                            const bool see = valid && key >= lo && key <= pos && (there[q] >> c & 1u);
+                            top = fmaxf(top, see ? __uint_as_float(ra[c]) * way : -INFINITY);
+                        }
+                        const float x = capped ? cap2 * tanh_fast(top * way * cap_in * k_ref[q]) : top * way * by_head * k_ref[q];
+                        if (top != -INFINITY) mx = fmaxf(mx, x + v_log[q]);
+                    }
                 }
-                mx = mx * sc + log2f(fmaxf(vm, 8.0779357e-28f)) - 10.f;  // (2^-90)
+                mx -= 10.f;
+                // raise the reference only when it has been outgrown by 2^4 (or there was none yet)
                 float corr = 1.f;
                 if (mx > ref + 4.f || (ref == -INFINITY && mx > -INFINITY)) {
                     corr = ref == -INFINITY ? 0.f : km_ex2(ref - mx);
@@ -502,70 +503,46 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                     }
                 }
                 const float minus = ref == -INFINITY ? 0.f : -ref;
-                const f32pair sc2 = pair_of(sc, sc), minus2 = pair_of(minus, minus), one2 = pair_of(1.f, 1.f);
-                f32pair sum[2] = {pair_of(0.f, 0.f), pair_of(0.f, 0.f)};
-                __syncwarp();
-                if (open) {
-                    auto weights = [&](int c0, const uint32_t (&raw)[32]) {
-                        uint32_t pk[16];
-#pragma unroll
-                        for (int c = 0; c < 32; c += 4) {
-                            f32pair a, b;
-                            by_scales(c0, raw, c, a, b);
-                            const float4 v = km_load4(s_at + 512u + 4u * (c0 + c));
-                            const float2 x = halves(fma2(a, sc2, minus2)), y = halves(fma2(b, sc2, minus2));
-                            const f32pair ea = pair_of(km_ex2(x.x), km_ex2(x.y)), eb = pair_of(km_ex2(y.x), km_ex2(y.y));
-                            sum[0] = fma2(ea, one2, sum[0]);
-                            sum[1] = fma2(eb, one2, sum[1]);
-                            const float2 wa = halves(mul2(ea, pair_of(v.x, v.y))), wb = halves(mul2(eb, pair_of(v.z, v.w)));
-                            pk[c / 2] = km_pack(wa.x, wa.y);
-                            pk[c / 2 + 1] = km_pack(wb.x, wb.y);
-                        }
-                        km_st16(tS + c0 / 2, pk);                        // (over scores that have been read)
-                    };
-#pragma unroll 1
-                    for (int c0 = 0; c0 < 128; c0 += 64) {
-                        load32(c0 + 32, rb);
-                        weights(c0, ra);
-                        km_wait(rb);
-                        if (c0 == 0) load32(64, ra);
-                        weights(c0 + 32, rb);
-                        if (c0 == 0) km_wait(ra);
-                    }
-                } else
-#pragma unroll 1
-                for (int c0 = 0; c0 < 128; c0 += 32) {
-                    f32pair x[16];
-                    scores(c0, x);
+                const f32pair one2 = pair_of(1.f, 1.f);
+                float step_sum = 0.f;
+                // weights 2^(score + log2 of the values' reference - R), over scores that have been read; the sum goes without the reference
+                auto weights = [&](int q, const uint32_t (&raw)[32], float factor) {
+                    const f32pair a2 = pair_of(factor, factor), m2 = pair_of(v_log[q] + minus, v_log[q] + minus);
+                    f32pair sum[2] = {pair_of(0.f, 0.f), pair_of(0.f, 0.f)};
                     uint32_t pk[16];
 #pragma unroll
-                    for (int c = 0; c < 16; c += 2) {
-                        const float4 v = km_load4(s_at + 512u + 4u * (c0 + 2 * c));
-#pragma unroll
-                        for (int u = 0; u < 2; u++) {
-                            const float2 a = halves(fma2(x[c + u], sc2, minus2));
-                            const f32pair e = pair_of(km_ex2(a.x), km_ex2(a.y));
-                            sum[u] = fma2(e, one2, sum[u]);
-                            float2 w = halves(mul2(e, u ? pair_of(v.z, v.w) : pair_of(v.x, v.y)));
-                            if (!all_visible) {                          // (a value that is no number, for a row that does not see it)
-                                const float2 s = halves(x[c + u]);
-                                if (s.x == -INFINITY) w.x = 0.f;
-                                if (s.y == -INFINITY) w.y = 0.f;
-                            }
-                            pk[c + u] = km_pack(w.x, w.y);
-                        }
+                    for (int c = 0; c < 32; c += 2) {
+                        const float2 x = halves(fma2(pair_of(__uint_as_float(raw[c]), __uint_as_float(raw[c + 1])), a2, m2));
+                        const float e0 = km_ex2(x.x), e1 = km_ex2(x.y);
+                        sum[(c >> 1) & 1] = fma2(pair_of(e0, e1), one2, sum[(c >> 1) & 1]);
+                        pk[c / 2] = km_pack(e0, e1);
                     }
-                    __syncwarp();
-                    km_st16(tS + c0 / 2, pk);
-                }
-                {
+                    km_st16(tS + 16 * q, pk);
                     const float2 s0 = halves(sum[0]), s1 = halves(sum[1]);
-                    l = l * corr + ((s0.x + s0.y) + (s1.x + s1.y));
+                    step_sum = fmaf((s0.x + s0.y) + (s1.x + s1.y), __uint_as_float((uint32_t)(127.f - v_log[q]) << 23), step_sum);
+                };
+                __syncwarp();
+                if (open) {
+                    load32(32, rb); weights(0, ra, unit * k_ref[0]); km_wait(rb);
+                    load32(64, ra); weights(1, rb, unit * k_ref[1]); km_wait(ra);
+                    load32(96, rb); weights(2, ra, unit * k_ref[2]); km_wait(rb);
+                    weights(3, rb, unit * k_ref[3]);
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        __syncwarp();
+                        load32(32 * q, ra);
+                        km_wait(ra);
+                        finish(q, ra);
+                        __syncwarp();
+                        weights(q, ra, 1.f);
+                    }
                 }
+                l = fmaf(l, corr, step_sum);
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) { mbar_arrive(sc_empty + 8 * b); mbar_arrive(p_ready + 8 * i); }
+                if (lane == 0) mbar_arrive(p_ready + 8 * i);
             }
             gs += it.n_kt;
             g_mine += n_mine;
