@@ -76,16 +76,32 @@ __device__ __forceinline__ void km_st16(uint32_t taddr, const uint32_t *v)
                  ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
                    "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
 }
-// D += A B with A in TMEM (a row a lane, two numbers a column)
-__device__ __forceinline__ void km_mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate)
+// D = A B or D += A B.  Of an operand descriptor only the low word differs from product to product; the high word is the layout (8-row groups
+// 1,024 bytes apart, 128-byte swizzle).  A single thread issues the products, and every instruction it spends on one is time the
+// tensor core may have to wait for.
+constexpr uint32_t KM_DESC_HIGH = (1024u >> 4) | (1u << 14) | (2u << 29);
+template <bool ADD> __device__ __forceinline__ void km_mma_ss(uint32_t tmem_d, uint32_t a, uint32_t b, uint32_t idesc)
 {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 x, {%1, %4};\n\tmov.b64 y, {%2, %4};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}"
+                 ::"r"(tmem_d), "r"(a), "r"(b), "r"(idesc), "n"(KM_DESC_HIGH), "n"(ADD ? 1 : 0) : "memory");
+}
+// ... with A in TMEM (a row a lane, two numbers a column)
+__device__ __forceinline__ void km_mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 y, {%2, %4};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}"
+                 ::"r"(tmem_d), "r"(tmem_a), "r"(b), "r"(idesc), "n"(KM_DESC_HIGH), "r"(accumulate) : "memory");
 }
 __device__ __forceinline__ void km_store16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d)
 {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ float km_load1(uint32_t addr)
+{
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+    return v;
 }
 __device__ __forceinline__ float4 km_load4(uint32_t addr)
 {
@@ -217,20 +233,32 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
             constexpr uint32_t F16 = (1u << 7) | (1u << 10);             // (the operands' type bits of bfloat16: clear for float16)
             constexpr uint32_t idesc_s = bf16_idesc(KM_ROWS, KM_KEYS, false) & ~F16, idesc_pv = bf16_idesc(KM_ROWS, D, true) & ~F16;
             const uint32_t tS0 = tmem_base, tO0 = tmem_base + 256;
-            const uint64_t dq = sw128_desc(sQ), dk = sw128_desc(sK), dv = sw128_desc_mn(sV, KM_SUB);
+            // the descriptors' low words, made once
+            uint32_t dq[2][D / 16], dk[2][D / 16], dv[2][KM_KEYS / 16];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+#pragma unroll
+                for (int kk = 0; kk < D / 16; kk++) {
+                    const uint32_t o = (uint32_t)(kk >> 2) * KM_SUB + (uint32_t)(kk & 3) * 32u + u * HT;
+                    dq[u][kk] = (uint32_t)sw128_desc(sQ + o);
+                    dk[u][kk] = (uint32_t)sw128_desc(sK + o);
+                }
+#pragma unroll
+                for (int kk = 0; kk < KM_KEYS / 16; kk++) dv[u][kk] = (uint32_t)sw128_desc_mn(sV + u * HT + kk * 2048u, KM_SUB);
+            }
             auto issue_s = [&](int i, uint32_t place) {
 #pragma unroll
                 for (int kk = 0; kk < D / 16; kk++) {
-                    const uint64_t o = ((uint32_t)(kk >> 2) * KM_SUB + (uint32_t)(kk & 3) * 32u) >> 4;
-                    tc_mma_bf16(tS0 + i * 128, dq + o + (uint64_t)i * (HT >> 4), dk + o + (uint64_t)place * (HT >> 4), idesc_s, kk > 0 ? 1u : 0u);
+                    const uint32_t b = place ? dk[1][kk] : dk[0][kk];
+                    if (kk == 0) km_mma_ss<false>(tS0 + i * 128, dq[i][kk], b, idesc_s);
+                    else km_mma_ss<true>(tS0 + i * 128, dq[i][kk], b, idesc_s);
                 }
                 tc_commit(s_full + 8 * i);
             };
             auto issue_pv = [&](int i, uint32_t place, bool accumulate) {
 #pragma unroll
                 for (int kk = 0; kk < KM_KEYS / 16; kk++)                // (two weights a column of TMEM)
-                    km_mma_ts(tO0 + i * D, tS0 + i * 128 + kk * 8, dv + (uint64_t)place * (HT >> 4) + (uint64_t)kk * (2048u >> 4), idesc_pv,
-                              (accumulate || kk > 0) ? 1u : 0u);
+                    km_mma_ts(tO0 + i * D, tS0 + i * 128 + kk * 8, place ? dv[1][kk] : dv[0][kk], idesc_pv, (accumulate || kk > 0) ? 1u : 0u);
                 tc_commit(pv_done + 8 * i);
             };
             bool ok = true;
@@ -415,26 +443,26 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                 const int key0 = (it.kt_lo + j) * KM_KEYS;
                 if (!mbar_wait(s_full + 8 * i, ph, abort_flag, err)) { ok = false; break; }
                 tc_fence_after();
-                // what the quarters of the tile share
-                const float4 kr = km_load4(s_at), lv = km_load4(s_at + 16u), there4 = km_load4(s_at + 32u);
-                const float k_ref[4] = {kr.x, kr.y, kr.z, kr.w}, v_log[4] = {lv.x, lv.y, lv.z, lv.w};
-                const uint32_t there[4] = {__float_as_uint(there4.x), __float_as_uint(there4.y), __float_as_uint(there4.z), __float_as_uint(there4.w)};
-                __syncwarp();
-                if (lane == 0) mbar_arrive(sc_empty + 8 * b);
                 // a step without options in which every row sees every key, as most are (rows beyond the tile's tokens go with those)
-                const bool full = (there[0] & there[1] & there[2] & there[3]) == 0xffffffffu;
+                const float4 there4 = km_load4(s_at + 32u);
+                const bool full = (__float_as_uint(there4.x) & __float_as_uint(there4.y) & __float_as_uint(there4.z) & __float_as_uint(there4.w)) == 0xffffffffu;
                 const bool open = __all_sync(0xffffffffu, !valid || (key0 + KM_KEYS - 1 <= pos && key0 >= lo)) && full && !finished;
                 const float b0 = slope2 * (float)(key0 - pos), by_head = unit * hscale;
-                auto load32 = [&](int c0, uint32_t (&raw)[32]) { tmem_ld16(tS + c0, raw); tmem_ld16(tS + c0 + 16, raw + 16); };
+                // (loops over the quarters of a tile stay loops: eight warps of these run beside four that convert, and unrolled their
+                // instructions do not stay in the caches: ### us)
+                auto load32 = [&](int q, uint32_t (&raw)[32]) { tmem_ld16(tS + 32 * q, raw); tmem_ld16(tS + 32 * q + 16, raw + 16); };
+                auto k_ref = [&](int q) { return km_load1(s_at + 4u * q); };
+                auto v_log = [&](int q) { return km_load1(s_at + 16u + 4u * q); };
                 // 32 finished scores (options, masks) in the exponent's base 2
                 auto finish = [&](int q, uint32_t (&raw)[32]) {
-                    const float in = capped ? cap_in * k_ref[q] : by_head * k_ref[q];
+                    const float in = (capped ? cap_in : by_head) * k_ref(q);
+                    const uint32_t there = __float_as_uint(km_load1(s_at + 32u + 4u * q));
 #pragma unroll
                     for (int c = 0; c < 32; c++) {
                         const int key = key0 + 32 * q + c;
                         const float bias = fmaf(slope2, (float)(32 * q + c), b0), v = __uint_as_float(raw[c]);
                         const float x = capped ? fmaf(cap2, tanh_fast(v * in), bias) : fmaf(v, in, bias);
-                        raw[c] = valid && key >= lo && key <= pos && (there[q] >> c & 1u) ? __float_as_uint(x) : 0xff800000u;
+                        raw[c] = valid && key >= lo && key <= pos && (there >> c & 1u) ? __float_as_uint(x) : 0xff800000u;
                     }
                 };
                 float mx = -INFINITY;
@@ -446,42 +474,43 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
 #pragma unroll
                         for (int c = 0; c < 32; c += 2)
                             top[(c >> 1) & 3] = fmaxf(top[(c >> 1) & 3], fmaxf(__uint_as_float(raw[c]), __uint_as_float(raw[c + 1])));
-                        mx = fmaxf(mx, fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), unit * k_ref[q], v_log[q]));
+                        mx = fmaxf(mx, fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), unit * k_ref(q), v_log(q)));
                     };
-                    load32(0, ra); km_wait(ra);
-                    load32(32, rb); largest(0, ra); km_wait(rb);
-                    load32(64, ra); largest(1, rb); km_wait(ra);
-                    load32(96, rb); largest(2, ra); km_wait(rb);
-                    load32(0, ra); largest(3, rb); km_wait(ra);          // (for the weights)
-                } else if (p.slopes) {
-#pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        __syncwarp();
-                        load32(32 * q, ra);
+                    load32(0, ra);
+                    km_wait(ra);
+#pragma unroll 1
+                    for (int q = 0; q < 4; q += 2) {
+                        load32(q + 1, rb);
+                        largest(q, ra);
+                        km_wait(rb);
+                        load32((q + 2) & 3, ra);                         // (the last time: for the weights)
+                        largest(q + 1, rb);
                         km_wait(ra);
-                        finish(q, ra);
-                        float top = -INFINITY;
-#pragma unroll
-                        for (int c = 0; c < 32; c++) top = fmaxf(top, __uint_as_float(ra[c]));
-                        mx = fmaxf(mx, top + v_log[q]);
                     }
                 } else {
-                    // factors and a cap keep the order of the scores (or turn it round): the largest is found first and finished alone
+                    // without slopes, factors and a cap keep the order of the scores or turn it round: the largest is found first, and finished alone
                     const float way = hscale < 0.f ? -1.f : 1.f;
-#pragma unroll
+#pragma unroll 1
                     for (int q = 0; q < 4; q++) {
                         __syncwarp();
-                        load32(32 * q, ra);
+                        load32(q, ra);
                         km_wait(ra);
                         float top = -INFINITY;
+                        if (p.slopes) {
+                            finish(q, ra);
 #pragma unroll
-                        for (int c = 0; c < 32; c++) {
-                            const int key = key0 + 32 * q + c;
-                            const bool see = valid && key >= lo && key <= pos && (there[q] >> c & 1u);
-                            top = fmaxf(top, see ? __uint_as_float(ra[c]) * way : -INFINITY);
+                            for (int c = 0; c < 32; c++) top = fmaxf(top, __uint_as_float(ra[c]));
+                        } else {
+                            const uint32_t there = __float_as_uint(km_load1(s_at + 32u + 4u * q));
+#pragma unroll
+                            for (int c = 0; c < 32; c++) {
+                                const int key = key0 + 32 * q + c;
+                                const bool see = valid && key >= lo && key <= pos && (there >> c & 1u);
+                                top = fmaxf(top, see ? __uint_as_float(ra[c]) * way : -INFINITY);
+                            }
+                            if (top != -INFINITY) top = capped ? cap2 * tanh_fast(top * way * cap_in * k_ref(q)) : top * way * by_head * k_ref(q);
                         }
-                        const float x = capped ? cap2 * tanh_fast(top * way * cap_in * k_ref[q]) : top * way * by_head * k_ref[q];
-                        if (top != -INFINITY) mx = fmaxf(mx, x + v_log[q]);
+                        mx = fmaxf(mx, top + v_log(q));
                     }
                 }
                 mx -= 10.f;
@@ -506,8 +535,9 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                 const f32pair one2 = pair_of(1.f, 1.f);
                 float step_sum = 0.f;
                 // weights 2^(score + log2 of the values' reference - R), over scores that have been read; the sum goes without the reference
-                auto weights = [&](int q, const uint32_t (&raw)[32], float factor) {
-                    const f32pair a2 = pair_of(factor, factor), m2 = pair_of(v_log[q] + minus, v_log[q] + minus);
+                auto weights = [&](int q, const uint32_t (&raw)[32], bool scaled) {
+                    const float factor = scaled ? 1.f : unit * k_ref(q), log = v_log(q);
+                    const f32pair a2 = pair_of(factor, factor), m2 = pair_of(log + minus, log + minus);
                     f32pair sum[2] = {pair_of(0.f, 0.f), pair_of(0.f, 0.f)};
                     uint32_t pk[16];
 #pragma unroll
@@ -519,25 +549,32 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                     }
                     km_st16(tS + 16 * q, pk);
                     const float2 s0 = halves(sum[0]), s1 = halves(sum[1]);
-                    step_sum = fmaf((s0.x + s0.y) + (s1.x + s1.y), __uint_as_float((uint32_t)(127.f - v_log[q]) << 23), step_sum);
+                    step_sum = fmaf((s0.x + s0.y) + (s1.x + s1.y), __uint_as_float((uint32_t)(127.f - log) << 23), step_sum);
                 };
                 __syncwarp();
                 if (open) {
-                    load32(32, rb); weights(0, ra, unit * k_ref[0]); km_wait(rb);
-                    load32(64, ra); weights(1, rb, unit * k_ref[1]); km_wait(ra);
-                    load32(96, rb); weights(2, ra, unit * k_ref[2]); km_wait(rb);
-                    weights(3, rb, unit * k_ref[3]);
+#pragma unroll 1
+                    for (int q = 0; q < 4; q += 2) {
+                        load32(q + 1, rb);
+                        weights(q, ra, false);
+                        km_wait(rb);
+                        if (q == 0) load32(2, ra);
+                        weights(q + 1, rb, false);
+                        if (q == 0) km_wait(ra);
+                    }
                 } else {
-#pragma unroll
+#pragma unroll 1
                     for (int q = 0; q < 4; q++) {
                         __syncwarp();
-                        load32(32 * q, ra);
+                        load32(q, ra);
                         km_wait(ra);
                         finish(q, ra);
                         __syncwarp();
-                        weights(q, ra, 1.f);
+                        weights(q, ra, true);
                     }
                 }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(sc_empty + 8 * b);
                 l = fmaf(l, corr, step_sum);
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 tc_fence_before();
