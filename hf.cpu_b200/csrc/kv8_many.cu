@@ -9,8 +9,8 @@
 //   a sum of two float16) or, with its scale, twice (values); half a step is 2^-11 of the number, an eighth of what bfloat16 keys and
 //   values lose.  (Scales applied to scores and weights in float32 instead took two reads of shared memory for every four scores: each
 //   brings a thread 16 bytes, 512 a warp, and those reads alone were 4,700 of 9,400 cycles a step: 436 us where this takes ###.)
-// * a thread owns a key: it asks for its codes of the next tile as soon as it has converted the last ones, and keeps them in registers.
-//   Both operands have two places, so that the conversion runs a tile ahead of the products.
+// * each of these warps asks for its keys' codes of the next tile as soon as it has converted the last ones, and both operands have two
+//   places, so that the conversion runs a tile ahead of the products.
 // * a row whose key or value is no number makes its scores so and leaves its values zero: a weight of zero stays zero in the sums of the
 //   rows that do not see it.
 // * queries are multiplied by the power of two that brings a row's largest number to 2^14..2^15 (kv8_few.cu).
@@ -26,6 +26,8 @@
 //   the order of the keys.  (Whole double tiles a CTA: 228 items of 2,048 tokens and 28 heads are two rounds on 148 SMs where 1.5 would do.)
 // Barrier waits are bounded (HFB_ERR_WAIT, TMEM freed; tc_ptx.cuh).
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "kv8.cuh"
 #include "tc_ptx.cuh"
@@ -45,7 +47,7 @@ struct Kv8ManyParams {
     int *counters;                                   // ... one per (double tile, head, query tile), zero between launches
 };
 
-template <int D> constexpr uint32_t km_smem() { return 6 * (D / 64) * KM_SUB + 128 + 256; }
+template <int D> constexpr uint32_t km_smem() { return 6 * (D / 64) * KM_SUB + 2 * KM_KEYS * D + 128 + 256; }
 
 __device__ __forceinline__ uint32_t km_off(int row, int c16)
 {
@@ -128,7 +130,8 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
     uint8_t *gen = km_raw + (base - smem_u32(km_raw));
     constexpr uint32_t HT = (D / 64) * KM_SUB;       // a [128 x D] float16 operand: Q, K or V
     const uint32_t sQ = base, sK = base + 2 * HT, sV = base + 4 * HT;         // (keys and values: two each)
-    const uint32_t sS = base + 6 * HT;               // [2][16]: per quarter of a tile the keys' reference, log2 of the values', the keys there are
+    const uint32_t stK = base + 6 * HT, stV = stK + KM_KEYS * D;         // codes of the next keys and values
+    const uint32_t sS = stV + KM_KEYS * D;           // [2][16]: per quarter of a tile the keys' reference, log2 of the values', the keys there are
     const uint32_t bars = sS + 128;
     const uint32_t q_ready = bars, s_full = bars + 16, p_ready = bars + 32, pv_done = bars + 48;                          // + 8 * query tile
     const uint32_t k_full = bars + 144, k_empty = bars + 160, v_full = bars + 176, v_empty = bars + 192;                  // + 8 * place
@@ -303,17 +306,20 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
     } else if (warp >= 8) {
         // ---- codes into operands: a warp has a quarter of a tile's keys, a lane one of them ----------------------------------------
         const int row = (warp - 8) * 32 + lane;
-        // code * (hi + lo), or code * hi
-        auto convert = [&](const uint4 (&w)[D / 16], uint32_t to, __half2 hi, __half2 lo, bool both) {
+        // this thread's key: code * (hi + lo) with `both`, else code * hi
+        auto convert = [&](uint32_t from, uint32_t to, __half2 hi, __half2 lo, auto both) {
             auto number = [&](uint32_t word, uint32_t selector) {
                 const uint32_t bits = km_codes(word, selector);
-                const __half2 c = *(const __half2 *)&bits, r = both ? __hfma2(c, hi, __hmul2(c, lo)) : __hmul2(c, hi);
+                const __half2 c = *(const __half2 *)&bits, r = decltype(both)::value ? __hfma2(c, hi, __hmul2(c, lo)) : __hmul2(c, hi);
                 return *(const uint32_t *)&r;
             };
-#pragma unroll
+#pragma unroll 2
             for (int c = 0; c < D / 16; c++) {
-                km_store16(to + km_off(row, 2 * c), number(w[c].x, 0x4140), number(w[c].x, 0x4342), number(w[c].y, 0x4140), number(w[c].y, 0x4342));
-                km_store16(to + km_off(row, 2 * c + 1), number(w[c].z, 0x4140), number(w[c].z, 0x4342), number(w[c].w, 0x4140), number(w[c].w, 0x4342));
+                uint4 w;
+                asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                             : "r"(from + (uint32_t)row * D + (uint32_t)kv8_piece(row % bs, c, D) * 16u) : "memory");
+                km_store16(to + km_off(row, 2 * c), number(w.x, 0x4140), number(w.x, 0x4342), number(w.y, 0x4140), number(w.y, 0x4342));
+                km_store16(to + km_off(row, 2 * c + 1), number(w.z, 0x4140), number(w.z, 0x4342), number(w.w, 0x4140), number(w.w, 0x4342));
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -333,21 +339,27 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
             };
             const int in_page = row % bs;                                 // (tiles begin on pages)
             auto record_of = [&](int page) { return p.cache + ((size_t)page * p.G + it.g) * p.record; };
-            auto load = [&](int page, int skip, uint4 (&w)[D / 16]) {
-                const uint8_t *src = record_of(max(page, 0)) + skip + in_page * D;
+            // the warp's 32 keys' codes, 16 bytes a lane, neighbouring lanes neighbouring bytes (zeros of keys that are not there: their scales are)
+            auto fetch = [&](int page, int skip, uint32_t to) {
 #pragma unroll
-                for (int c = 0; c < D / 16; c++)
-                    w[c] = page >= 0 ? *(const uint4 *)(src + kv8_piece(in_page, c, D) * 16) : make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+                for (int n = 0; n < D / 16; n++) {
+                    const int at = n * 32 + lane, r_q = at / (D / 16), r_tile = (warp - 8) * 32 + r_q;
+                    const int its = __shfl_sync(0xffffffffu, page, r_q);
+                    const uint8_t *src = record_of(max(its, 0)) + skip + (r_tile % bs) * D + at % (D / 16) * 16;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                                 ::"r"(to + (uint32_t)(warp - 8) * 32u * D + at * 16u), "l"(src), "r"(its >= 0 ? 16 : 0) : "memory");
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
             };
+            auto fetched = [&] { asm volatile("cp.async.wait_group 1;" ::: "memory"); __syncwarp(); };       // (all but the last)
             auto scales_of = [&](int page) {
                 if (page < 0) return make_float2(0.f, 0.f);
                 const float *s = (const float *)(record_of(page) + 2 * bs * D) + in_page;
                 return make_float2(s[0], s[bs]);
             };
             int page = page_of(0);
-            uint4 k[D / 16], v[D / 16];
-            load(page, 0, k);
-            load(page, bs * D, v);
+            fetch(page, 0, stK);
+            fetch(page, bs * D, stV);
             float2 sc = scales_of(page);
             bool there = page >= 0;
             page = page_of(1);
@@ -369,19 +381,22 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                     mbar_arrive(sc_full + 8 * b);
                 }
                 if (!mbar_wait(k_empty + 8 * b, ph ^ 1, abort_flag, err)) { ok = false; break; }
-                convert(k, sK + b * HT, __half2half2(k_hi), __half2half2(k_lo), true);
+                fetched();
+                convert(stK, sK + b * HT, __half2half2(k_hi), __half2half2(k_lo), std::true_type());
                 if (lane == 0) mbar_arrive(k_full + 8 * b);
-                load(page, 0, k);                                         // (of step j + 1)
+                fetch(page, 0, stK);                                      // (of step j + 1)
                 sc = scales_of(page);
                 if (!mbar_wait(v_empty + 8 * b, ph ^ 1, abort_flag, err)) { ok = false; break; }
-                convert(v, sV + b * HT, __half2half2(v_hi), __half2half2(v_hi), false);
+                fetched();
+                convert(stV, sV + b * HT, __half2half2(v_hi), __half2half2(v_hi), std::false_type());
                 if (lane == 0) mbar_arrive(v_full + 8 * b);
-                load(page, bs * D, v);
+                fetch(page, bs * D, stV);
                 there = page >= 0;
                 page = page_of(j + 2);
             }
             gs += it.n_kt;
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
         // ---- softmax and output: one thread per row -------------------------------------------------------------------------------
         const float log2e = 1.4426950408889634f;

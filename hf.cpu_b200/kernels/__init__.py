@@ -339,17 +339,27 @@ def kv8_cache(num_pages: int, block_size: int, G: int, head_dim: int, device) ->
     return torch.zeros((int(num_pages), int(G), kv8_record_bytes(block_size, head_dim)), dtype=torch.uint8, device=device)
 
 
-def _kv8_ok(cache, block_size, G, d, what):
-    _need(cache.dtype == torch.uint8 and cache.dim() == 3 and cache.shape[1:] == (G, kv8_record_bytes(block_size, d)),
-          f"{what}: the cache must be uint8 [pages, {G}, {kv8_record_bytes(block_size, d)}] for {G} heads of {d} in pages of {block_size}")
+# (the checks below are made at every launch: what they say is put together only where one fails)
+def _kv8_records(cache, block_size, G, d, what) -> None:
+    record = _KV8_RECORDS.get((block_size, d))
+    if record is None:
+        record = _KV8_RECORDS[block_size, d] = kv8_record_bytes(block_size, d)
+    if cache.dtype != torch.uint8 or cache.dim() != 3 or cache.shape[1] != G or cache.shape[2] != record:
+        raise ValueError(f"{what}: the cache must be uint8 [pages, {G}, {record}] for {G} heads of {d} in pages of {block_size}")
 
 
-def _kv8_rows(x, T, n, dtype, what):
-    _need(x.dim() == 2 and x.shape == (T, n) and x.dtype == dtype and x.stride(1) == 1 and x.stride(0) >= n, f"{what} must be rows [T, {n}] of one type")
+_KV8_RECORDS = {}
+_KV8_TYPES = (torch.float32, torch.bfloat16)
 
 
-def _kv8_index(x, T, what):
-    _need(x.dtype == torch.int32 and x.dim() == 1 and x.shape[0] == T, f"{what} must be int32 [T]")
+def _kv8_rows(x, T, n, dtype, what) -> None:
+    if x.dim() != 2 or x.shape[0] != T or x.shape[1] != n or x.dtype != dtype or x.stride(1) != 1 or x.stride(0) < n:
+        raise ValueError(f"{what} must be rows [{T}, {n}] of one type")
+
+
+def _kv8_index(x, T, what) -> None:
+    if x.dtype != torch.int32 or x.dim() != 1 or x.shape[0] < T:
+        raise ValueError(f"{what} must be int32 [{T}]")
 
 
 def rope_kv8_write(qkv, cos_sin, n_rot, positions, slots, q_out, cache, H, G, d, block_size, pairing: str = "half") -> None:
@@ -357,44 +367,48 @@ def rope_kv8_write(qkv, cos_sin, n_rot, positions, slots, q_out, cache, H, G, d,
     wider rows), float32 or bfloat16; ``pairing``: the numbers (i, i + n_rot/2) turn together ("half") or (2i, 2i + 1)
     ("interleaved").  ``slots`` (int32 [T], or None: nothing is cached) names each token's place, page * block_size + row; below 0 the
     token is not cached.  No two tokens of a call may have the same slot."""
-    T = qkv.shape[0]
-    _need(qkv.dtype in (torch.float32, torch.bfloat16), "rope_kv8_write: rows are float32 or bfloat16")
-    _kv8_rows(qkv, T, (H + 2 * G) * d, qkv.dtype, "rope_kv8_write: q|k|v")
-    _need(q_out.shape == (T, H * d) and q_out.dtype == qkv.dtype, "rope_kv8_write: queries must be [T, H * d] of the rows' type")
-    _need(pairing in ("half", "interleaved"), "rope_kv8_write: pairing is 'half' or 'interleaved'")
-    _need(n_rot % 2 == 0 and 0 <= n_rot <= d, "rope_kv8_write: the rotated part is even and no longer than a head")
-    _need(n_rot == 0 or (cos_sin is not None and cos_sin.shape[1:] == (n_rot // 2, 2) and cos_sin.dtype == torch.float32),
-          "rope_kv8_write: cos/sin table must be float32 [positions, n_rot/2, 2]")
-    _kv8_ok(cache, block_size, G, d, "rope_kv8_write")
+    T, dtype = qkv.shape[0], qkv.dtype
+    if dtype not in _KV8_TYPES:
+        raise ValueError("rope_kv8_write: rows are float32 or bfloat16")
+    _kv8_rows(qkv, T, (H + 2 * G) * d, dtype, "rope_kv8_write: q|k|v")
+    if q_out.dim() != 2 or q_out.shape[0] != T or q_out.shape[1] != H * d or q_out.dtype != dtype:
+        raise ValueError("rope_kv8_write: queries must be [T, H * d] of the rows' type")
+    if pairing != "half" and pairing != "interleaved":
+        raise ValueError("rope_kv8_write: pairing is 'half' or 'interleaved'")
+    if n_rot % 2 or not 0 <= n_rot <= d:
+        raise ValueError("rope_kv8_write: the rotated part is even and no longer than a head")
     if n_rot:
+        if cos_sin is None or cos_sin.dim() != 3 or cos_sin.shape[1] != n_rot // 2 or cos_sin.shape[2] != 2 or cos_sin.dtype != torch.float32:
+            raise ValueError("rope_kv8_write: cos/sin table must be float32 [positions, n_rot/2, 2]")
         _kv8_index(positions, T, "rope_kv8_write: positions")
+    _kv8_records(cache, block_size, G, d, "rope_kv8_write")
     if slots is not None:
         _kv8_index(slots, T, "rope_kv8_write: slots")
-    backend().kv8_write(qkv[:, :H * d], qkv[:, H * d:(H + G) * d], qkv[:, (H + G) * d:], cos_sin if n_rot else None, int(n_rot), pairing,
-                        positions, slots, q_out, cache, int(H), int(G), int(d), int(block_size))
+    backend().kv8_write(qkv, None, cos_sin if n_rot else None, n_rot, pairing, positions, slots, q_out, cache, H, G, d, block_size)
 
 
 def kv8_write(k, v, slots, cache, G, d, block_size) -> None:
     """Keys and values [T, G * d] as they are into a cache in 8 bits (for layers whose own tails have made them)."""
     T = k.shape[0]
-    _need(k.dtype in (torch.float32, torch.bfloat16), "kv8_write: rows are float32 or bfloat16")
+    if k.dtype not in _KV8_TYPES:
+        raise ValueError("kv8_write: rows are float32 or bfloat16")
     _kv8_rows(k, T, G * d, k.dtype, "kv8_write: keys")
     _kv8_rows(v, T, G * d, k.dtype, "kv8_write: values")
-    _kv8_ok(cache, block_size, G, d, "kv8_write")
+    _kv8_records(cache, block_size, G, d, "kv8_write")
     _kv8_index(slots, T, "kv8_write: slots")
-    backend().kv8_write(None, k, v, None, 0, "half", None, slots, None, cache, 0, int(G), int(d), int(block_size))
+    backend().kv8_write(k, v, None, 0, "half", None, slots, None, cache, 0, G, d, block_size)
 
 
 def kv8_read(cache, pages, rows, k_out, v_out) -> None:
     """Keys and values [N, block, G, d] (float32 or bfloat16) of the pages ``pages`` (int32 [N]; below 0: no page) of a cache in 8 bits,
     as the values that their codes stand for; rows from ``rows[n]`` (int32 [N]) on are zeros."""
-    _need(k_out.dim() == 4 and k_out.shape == v_out.shape and k_out.dtype == v_out.dtype and k_out.dtype in (torch.float32, torch.bfloat16),
-          "kv8_read: keys and values must be [N, block, G, d], both float32 or bfloat16")
+    if k_out.dim() != 4 or k_out.shape != v_out.shape or k_out.dtype != v_out.dtype or k_out.dtype not in _KV8_TYPES:
+        raise ValueError("kv8_read: keys and values must be [N, block, G, d], both float32 or bfloat16")
     N, block_size, G, d = k_out.shape
-    _kv8_ok(cache, block_size, G, d, "kv8_read")
+    _kv8_records(cache, block_size, G, d, "kv8_read")
     _kv8_index(pages, N, "kv8_read: pages")
     _kv8_index(rows, N, "kv8_read: row counts")
-    backend().kv8_read(cache, pages, rows, k_out, v_out)
+    backend().kv8_read(cache, pages, rows, k_out, v_out, N, block_size, G, d)
 
 
 def kv8_head_groups(heads_per_group: int) -> int:
@@ -433,20 +447,27 @@ def paged_attention_kv8(q, cache, meta, ctx, H, G, d, window, scale, out, tiles=
     rows before the step's own positions were written before the kernel in front of this one was launched, so that they may be
     fetched while it still runs."""
     T = q.shape[0]
-    _need(q.dtype in (torch.float32, torch.bfloat16) and q.shape == (T, H * d) and out.shape == q.shape and out.dtype == q.dtype,
-          "paged_attention_kv8: queries and output must be [T, H * d], both float32 or bfloat16")
-    _need(G > 0 and H % G == 0, "paged_attention_kv8: %d heads over %d key/value heads" % (H, G))
-    _kv8_ok(cache, meta.block_size, G, d, "paged_attention_kv8")
-    _kv8_index(ctx.positions[:T], T, "paged_attention_kv8: positions")
-    _kv8_index(ctx.token_seq[:T], T, "paged_attention_kv8: the tokens' requests")
-    _need(meta.block_table.dtype == torch.int32 and meta.block_table.dim() == 2 and meta.block_table.shape[1] == meta.max_blocks,
-          "paged_attention_kv8: the block table must be int32 [requests, max_blocks]")
-    for name, x in (("sinks", sinks), ("slopes", slopes), ("head_scales", head_scales)):
-        _need(x is None or (x.shape == (H,) and x.dtype == torch.float32), f"paged_attention_kv8: {name} are float32 [H]")
-    _need(not (zero_sink and sinks is not None), "paged_attention_kv8: a learned sink or a sink of zero, not both")
-    _need(softcap >= 0, "paged_attention_kv8: softcap must be positive (0: none)")
-    backend().paged_attention_kv8(q, cache, meta, ctx, int(H), int(G), int(d), int(window), float(scale), out, tiles or {}, settled=bool(settled),
-                                  sinks=sinks, zero_sink=bool(zero_sink), slopes=slopes, head_scales=head_scales, softcap=float(softcap))
+    if q.dtype not in _KV8_TYPES or q.dim() != 2 or q.shape[1] != H * d or out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError("paged_attention_kv8: queries and output must be [T, H * d], both float32 or bfloat16")
+    if G < 1 or H % G:
+        raise ValueError("paged_attention_kv8: %d heads over %d key/value heads" % (H, G))
+    table = meta.block_table
+    _kv8_records(cache, meta.block_size, G, d, "paged_attention_kv8")
+    _kv8_index(ctx.positions, T, "paged_attention_kv8: positions")
+    _kv8_index(ctx.token_seq, T, "paged_attention_kv8: the tokens' requests")
+    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[1] != meta.max_blocks:
+        raise ValueError("paged_attention_kv8: the block table must be int32 [requests, max_blocks]")
+    options = ()
+    if sinks is not None or zero_sink or slopes is not None or head_scales is not None or softcap:
+        for name, x in (("sinks", sinks), ("slopes", slopes), ("head_scales", head_scales)):
+            if x is not None and (x.shape != (H,) or x.dtype != torch.float32):
+                raise ValueError(f"paged_attention_kv8: {name} are float32 [H]")
+        if zero_sink and sinks is not None:
+            raise ValueError("paged_attention_kv8: a learned sink or a sink of zero, not both")
+        if softcap < 0:
+            raise ValueError("paged_attention_kv8: softcap must be positive (0: none)")
+        options = dict(sinks=sinks, zero_sink=zero_sink, slopes=slopes, head_scales=head_scales, softcap=softcap)
+    backend().paged_attention_kv8(q, cache, meta, ctx, H, G, d, window, scale, out, tiles or {}, settled=settled, **dict(options))
 
 
 def swiglu(gu: torch.Tensor, out: torch.Tensor, interleaved: bool = False) -> None:

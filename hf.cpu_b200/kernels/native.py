@@ -12,7 +12,7 @@ from ctypes import c_float, c_int, c_int64, c_void_p
 
 import torch
 
-from . import FEW_TOKENS, Written, build as _build
+from . import FEW_TOKENS, Written, build as _build, kv8_head_groups
 
 HFB_ENOTSUP = 2          # status of csrc/hfb200.h: not a case for this kernel, nothing was launched
 
@@ -145,7 +145,11 @@ class NativeBackend:
         if self.lib.hfb_decay_chunk_tokens() != DECAY_CHUNK:
             raise KernelError("the library's chunks and the binding's are not of one length")
         self.decay_chunks = os.environ.get("HFB_DECAY_CHUNKS", "1") != "0"     # portions of a recurrence with scalar decays in chunks
-        self._kv8_counters = {}
+        self._kv8_counters, self._kv8_needs = {}, {}
+        self._kv8_few_tiles = self.lib.hfb_kv8_attention_few_tiles()
+        types = {"p": c_void_p, "i": c_int, "l": c_int64, "f": c_float, "z": ctypes.c_size_t}
+        for name, signature in self._KV8_SIGNATURES.items():
+            getattr(self.lib, name).argtypes = [types[c] for c in signature]
         # attention of few queries over the 8-bit cache: CTAs per SM by (heads of 128, more than 8 places a tile), fewest steps of a CTA
         self.kv8_ctas_per_sm, self.kv8_min_steps = {(False, False): 2, (False, True): 2, (True, False): 2, (True, True): 1}, 1
         self.kv8_tile_cost = 6                    # ... and what a tile's start and end are reckoned as, in steps
@@ -384,98 +388,107 @@ class NativeBackend:
                                                  c_int(v_row), *opt_args, self._stream()), "attention")
 
     # ---- the key/value cache in 8 bits ----------------------------------------------------------------------
-    @staticmethod
-    def _here(*ts):
-        """Tensors of the current device, whose current stream the launches go to."""
-        dev = _current_device()
-        for t in ts:
-            if t is not None and (not t.is_cuda or t.device.index != dev):
-                raise KernelError(f"kernel arguments must be tensors of the current CUDA device ({dev})")
+    # (These launches are few and short enough for the host's part to count: their functions know their arguments' types, so that plain
+    # numbers go in; the cache alone goes in as a pointer object, which a Recording tells from the numbers and replaces.)
+    _KV8_SIGNATURES = {
+        "hfb_kv8_write": "plplplipiiippppliiiiip", "hfb_kv8_read": "plppppiliiip", "hfb_kv8_attention_plain": "ppipippilifpiiiipippfp",
+        "hfb_kv8_attention_few": "pppippppiiiiiiilifppzpiiiipippfp", "hfb_kv8_attention_many": "pppippppiiiiilifppzpiiiipippfp"}
 
-    def kv8_write(self, q, k, v, cos_sin, n_rot, pairing, positions, slots, q_out, cache, H, G, d, block_size):
-        self._here(q, k, v, cos_sin, positions, slots, q_out, cache)
-        self._on_gpu(cos_sin, positions, slots, q_out, cache)
+    @staticmethod
+    def _here(tensors):
+        """Contiguous tensors of the current device, whose current stream the launches go to."""
+        dev = _current_device()
+        for t in tensors:
+            if t is not None and (t.get_device() != dev or not t.is_contiguous()):
+                raise KernelError(f"kernel arguments must be contiguous tensors of the current CUDA device ({dev})")
+        return dev
+
+    def kv8_write(self, rows, v, cos_sin, n_rot, pairing, positions, slots, q_out, cache, H, G, d, block_size):
+        """``rows`` are q|k|v, or keys with the values in ``v``."""
+        dev = self._here((cos_sin, positions, slots, q_out, cache))
+        if rows.get_device() != dev or (v is not None and v.get_device() != dev):
+            raise KernelError(f"kernel arguments must be tensors of the current CUDA device ({dev})")
+        size, stride = rows.element_size(), rows.stride(0)
+        q_at = rows.data_ptr() if v is None else 0
+        k_at = q_at + H * d * size if v is None else rows.data_ptr()
+        v_at = k_at + G * d * size if v is None else v.data_ptr()
         if slots is None:
             G = 0                                         # (nothing is cached: only the queries are turned)
         if H + G == 0:
             return
-        stride = lambda x: c_int64(x.stride(0) if x is not None else 0)
         self._check(self.lib.hfb_kv8_write(
-            _p(q), stride(q), _p(k), stride(k), _p(v), stride(v), c_int(_dt(k)), _p(cos_sin), c_int(n_rot),
-            c_int(cos_sin.shape[0] if cos_sin is not None else 0), c_int(1 if pairing == "interleaved" else 0), _p(positions), _p(slots),
-            _p(q_out), _p(cache), c_int64(cache.shape[0]), c_int(block_size), c_int(k.shape[0]), c_int(H), c_int(G), c_int(d),
-            self._stream()), "kv8_write")
+            q_at, stride, k_at, stride, v_at, stride if v is None else v.stride(0), _dt(rows), cos_sin.data_ptr() if n_rot else 0, n_rot,
+            cos_sin.shape[0] if n_rot else 0, pairing == "interleaved", positions.data_ptr() if n_rot else 0, slots.data_ptr() if G else 0,
+            q_out.data_ptr() if H else 0, _p(cache), cache.shape[0], block_size, rows.shape[0], H, G, d, _raw_stream(dev)), "kv8_write")
 
-    def kv8_read(self, cache, pages, rows, k_out, v_out):
-        self._here(cache, pages, rows, k_out, v_out)
-        self._on_gpu(cache, pages, rows, k_out, v_out)
-        N, block_size, G, d = k_out.shape
-        self._check(self.lib.hfb_kv8_read(_p(cache), c_int64(cache.shape[0]), _p(pages), _p(rows), _p(k_out), _p(v_out), c_int(_dt(k_out)),
-                                          c_int64(N), c_int(block_size), c_int(G), c_int(d), self._stream()), "kv8_read")
+    def kv8_read(self, cache, pages, rows, k_out, v_out, N, block_size, G, d):
+        dev = self._here((cache, pages, rows, k_out, v_out))
+        self._check(self.lib.hfb_kv8_read(_p(cache), cache.shape[0], pages.data_ptr(), rows.data_ptr(), k_out.data_ptr(), v_out.data_ptr(),
+                                          _dt(k_out), N, block_size, G, d, _raw_stream(dev)), "kv8_read")
 
     def paged_attention_kv8(self, q, cache, meta, ctx, H, G, d, window, scale, out, tiles, settled=False, sinks=None, zero_sink=False,
                             slopes=None, head_scales=None, softcap=0.0):
-        self._here(q, cache, meta.block_table, ctx.token_seq, ctx.positions, out, sinks, slopes, head_scales)
-        self._on_gpu(q, cache, meta.block_table, ctx.token_seq, ctx.positions, out, sinks, slopes, head_scales)
-        opt_args = (_p(sinks), c_int(1 if zero_sink else 0), _p(slopes), _p(head_scales), c_float(softcap))
-        if (self.attention == "fast" and ("few.seq" in tiles or "many.seq" in tiles) and q.dtype == torch.bfloat16 and d in (64, 128)
-                and meta.block_size in (8, 16, 32, 64) and scale > 0 and q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0):
-            if "many.seq" in tiles:
-                self._kv8_many(q, cache, meta, ctx, H, G, d, window, scale, out, tiles, settled, opt_args)
-            if "few.seq" in tiles:
-                self._kv8_few(q, cache, meta, ctx, H, G, d, window, scale, out, tiles, settled, opt_args)
+        table, positions, bs = meta.block_table, ctx.positions, meta.block_size
+        dev = self._here((q, cache, table, ctx.token_seq, positions, out, sinks, slopes, head_scales))
+        at = lambda t: 0 if t is None else t.data_ptr()
+        options = (at(sinks), 1 if zero_sink else 0, at(slopes), at(head_scales), softcap)
+        q_at, out_at, kept = q.data_ptr(), out.data_ptr(), _p(cache)
+        if (tiles and self.attention == "fast" and q.dtype == torch.bfloat16 and (d == 64 or d == 128) and bs in (8, 16, 32, 64) and scale > 0
+                and q_at % 16 == 0 and out_at % 16 == 0):
+            stream, capturing, r = _raw_stream(dev), torch.cuda.is_current_stream_capturing(), H // G
+            front = (q_at, kept, table.data_ptr(), meta.max_blocks, positions.data_ptr())
+            seq = tiles.get("many.seq")
+            if seq is not None:
+                n, ctas = seq.shape[0], self.sm_count
+                need = self._kv8_scratch(True, ctas, d)
+                counters = self._kv8_zeros(dev, stream, capturing, 2 * n * G)
+                self._check(self.lib.hfb_kv8_attention_many(
+                    *front, seq.data_ptr(), tiles["many.t0"].data_ptr(), tiles["many.nt"].data_ptr(), n, ctas, 1, settled, bs, cache.shape[0], window,
+                    scale, out_at, ctx.buf("kv8_scratch", (need,), torch.uint8).data_ptr(), need, counters.data_ptr(), counters.shape[0], H, G, d,
+                    *options, stream), "kv8_attention_many")
+            seq = tiles.get("few.seq")
+            if seq is not None:
+                share = 1 if r <= 16 else kv8_head_groups(r)
+                tile_tokens = 1 if share > 1 or ctx.max_q_len == 1 else 16 // r
+                ctas = self.kv8_ctas_per_sm[d == 128, tile_tokens * (r // share) > 8] * self.sm_count
+                need = self._kv8_scratch(False, ctas, d)
+                scratch = ctx.buf("kv8_scratch", (need,), torch.uint8).data_ptr()
+                for i in range(0, seq.shape[0], self._kv8_few_tiles):
+                    n = min(self._kv8_few_tiles, seq.shape[0] - i)
+                    counters = self._kv8_zeros(dev, stream, capturing, n * G * share)
+                    self._check(self.lib.hfb_kv8_attention_few(
+                        *front, seq.data_ptr() + 4 * i, tiles["few.t0"].data_ptr() + 4 * i, tiles["few.nt"].data_ptr() + 4 * i, n, tile_tokens, ctas,
+                        self.kv8_min_steps, self.kv8_tile_cost, settled, bs, cache.shape[0], window, scale, out_at, scratch, need, counters.data_ptr(),
+                        counters.shape[0], H, G, d, *options, stream), "kv8_attention_few")
             return
         self._check(self.lib.hfb_kv8_attention_plain(
-            _p(q), _p(cache), c_int(_dt(q)), _p(meta.block_table), c_int(meta.max_blocks), _p(ctx.token_seq), _p(ctx.positions),
-            c_int(meta.block_size), c_int64(cache.shape[0]), c_int(window), c_float(scale), _p(out), c_int(q.shape[0]), c_int(H), c_int(G),
-            c_int(d), *opt_args, self._stream()), "kv8_attention_plain")
+            q_at, kept, _dt(q), table.data_ptr(), meta.max_blocks, ctx.token_seq.data_ptr(), positions.data_ptr(), bs, cache.shape[0], window,
+            scale, out_at, q.shape[0], H, G, d, *options, _raw_stream(dev)), "kv8_attention_plain")
 
-    def _kv8_zeros(self, device, n):
+    def _kv8_scratch(self, many, ctas, d):
+        """Bytes of scratch; the library's answer depends on nothing else."""
+        need = self._kv8_needs.get((many, ctas, d))
+        if need is None:
+            ask = self.lib.hfb_kv8_attention_many_scratch if many else self.lib.hfb_kv8_attention_few_scratch
+            need = self._kv8_needs[many, ctas, d] = ask(c_int(ctas), c_int(d))
+        return need
+
+    def _kv8_zeros(self, dev, stream, capturing, n):
         """``n`` counters that are zero and that no launch uses which may run beside the one they are for: one set a stream, and for
         a launch that is being captured a set of its own, since its graph may be replayed beside anything."""
-        if torch.cuda.is_current_stream_capturing():
-            pool = self._kv8_counters.get(device)
+        if capturing:
+            pool = self._kv8_counters.get(dev)
             if pool is None or pool[1] + n > pool[0].numel():
-                return torch.zeros(n, dtype=torch.int32, device=device)       # (a part of the graph then)
+                return torch.zeros(n, dtype=torch.int32, device=dev)              # (a part of the graph then)
             pool[1] += n
             return pool[0][pool[1] - n:pool[1]]
-        if device not in self._kv8_counters:
-            self._kv8_counters[device] = [torch.zeros(1 << 20, dtype=torch.int32, device=device), 0]
-        key = device, _raw_stream(device.index)
-        have = self._kv8_counters.get(key)
-        if have is None or have.numel() < n:
-            have = self._kv8_counters[key] = torch.zeros(max(n, 4096), dtype=torch.int32, device=device)
+        have = self._kv8_counters.get((dev, stream))
+        if have is None or have.shape[0] < n:
+            if dev not in self._kv8_counters:
+                self._kv8_counters[dev] = [torch.zeros(1 << 20, dtype=torch.int32, device=dev), 0]
+                torch.cuda.current_stream().synchronize()                         # (other streams' captures take from it)
+            have = self._kv8_counters[dev, stream] = torch.zeros(max(n, 4096), dtype=torch.int32, device=dev)
         return have
-
-    def _kv8_many(self, q, cache, meta, ctx, H, G, d, window, scale, out, tiles, settled, opt_args):
-        seq, t0, nt = tiles["many.seq"], tiles["many.t0"], tiles["many.nt"]
-        n, ctas = seq.shape[0], self.sm_count
-        need = self.lib.hfb_kv8_attention_many_scratch(c_int(ctas), c_int(d))
-        scratch, counters = ctx.buf("kv8_scratch", (need,), torch.uint8), self._kv8_zeros(q.device, 2 * n * G)
-        self._check(self.lib.hfb_kv8_attention_many(
-            _p(q), _p(cache), _p(meta.block_table), c_int(meta.max_blocks), _p(ctx.positions), _p(seq), _p(t0), _p(nt), c_int(n), c_int(ctas),
-            c_int(1), c_int(1 if settled else 0), c_int(meta.block_size), c_int64(cache.shape[0]), c_int(window), c_float(scale), _p(out),
-            _p(scratch), ctypes.c_size_t(need), _p(counters), c_int(counters.numel()), c_int(H), c_int(G), c_int(d), *opt_args,
-            self._stream()), "kv8_attention_many")
-
-    def _kv8_few(self, q, cache, meta, ctx, H, G, d, window, scale, out, tiles, settled, opt_args):
-        from . import kv8_head_groups
-        seq, t0, nt = tiles["few.seq"], tiles["few.t0"], tiles["few.nt"]
-        r, most = H // G, self.lib.hfb_kv8_attention_few_tiles()
-        share = kv8_head_groups(r)
-        tile_tokens = 1 if share > 1 or ctx.max_q_len == 1 else max(1, 16 // r)
-        ctas = self.kv8_ctas_per_sm[d == 128, tile_tokens * (r // share) > 8] * self.sm_count
-        need = self.lib.hfb_kv8_attention_few_scratch(c_int(ctas), c_int(d))
-        scratch = ctx.buf("kv8_scratch", (need,), torch.uint8)
-        for i in range(0, seq.shape[0], most):
-            n = min(most, seq.shape[0] - i)
-            counters = self._kv8_zeros(q.device, n * G * share)
-            at = lambda x: c_void_p(x.data_ptr() + 4 * i)
-            self._check(self.lib.hfb_kv8_attention_few(
-                _p(q), _p(cache), _p(meta.block_table), c_int(meta.max_blocks), _p(ctx.positions), at(seq), at(t0), at(nt), c_int(n),
-                c_int(tile_tokens), c_int(ctas), c_int(self.kv8_min_steps), c_int(self.kv8_tile_cost), c_int(1 if settled else 0), c_int(meta.block_size),
-                c_int64(cache.shape[0]), c_int(window), c_float(scale), _p(out), _p(scratch), ctypes.c_size_t(need), _p(counters),
-                c_int(counters.numel()), c_int(H), c_int(G), c_int(d), *opt_args, self._stream()), "kv8_attention_few")
 
     def swiglu(self, gu, out, interleaved):
         self._on_gpu(gu, out)

@@ -111,8 +111,9 @@ def attention(q, cache, table, token_seq, positions, bs, H, G, d, mask, scale, s
 
 
 class EmuKv8(EmuBackend):
-    def kv8_write(self, q, k, v, cos_sin, n_rot, pairing, positions, slots, q_out, cache, H, G, d, block_size):
-        T = k.shape[0]
+    def kv8_write(self, rows, v, cos_sin, n_rot, pairing, positions, slots, q_out, cache, H, G, d, block_size):
+        T = rows.shape[0]
+        q, k, v = (None, rows, v) if v is not None else (rows[:, :H * d], rows[:, H * d:(H + G) * d], rows[:, (H + G) * d:])
         if H:
             q_out.copy_(rotated(q.float().reshape(T, H, d), cos_sin, positions, n_rot, pairing).reshape(T, H * d).to(q_out.dtype))
         if slots is None:
@@ -124,8 +125,7 @@ class EmuKv8(EmuBackend):
         vc[page, row], vs[page, row] = quantised(v.double().reshape(T, G, d)[ok])
         cache.copy_(pack(kc, ks, vc, vs))
 
-    def kv8_read(self, cache, pages, rows, k_out, v_out):
-        N, bs, G, d = k_out.shape
+    def kv8_read(self, cache, pages, rows, k_out, v_out, N, bs, G, d):
         used = (torch.arange(bs, device=cache.device)[None] < rows[:, None]) & (pages >= 0)[:, None]
         for out, x in zip((k_out, v_out), values(cache, bs, G, d)):
             out.copy_(torch.where(used[..., None, None], x[pages.long().clamp_min(0)], torch.zeros((), dtype=torch.float64, device=cache.device)))

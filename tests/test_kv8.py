@@ -189,3 +189,16 @@ def test_mixers_that_cannot_are_refused(emu):
     cfg = dict(TINY["A"], head_dim=24, num_attention_heads=4)
     with pytest.raises((UnsupportedError, ValueError)):
         Engine(random_model(config_from_dict(cfg), seed=3, dtype=torch.float32, device="cpu"), block_size=8, max_tokens=64, kv_dtype="int8")
+
+
+def test_argument_types_are_the_headers():
+    """The binding's argument types of the 8-bit cache's functions, against the C header."""
+    import os
+    import re
+    from hfcpu_b200.kernels import build
+    from hfcpu_b200.kernels.native import NativeBackend
+    header = open(os.path.join(build.CSRC, "hfb200.h")).read()
+    for name, signature in NativeBackend._KV8_SIGNATURES.items():
+        args = re.search(r"int %s\((.*?)\);" % name, header, re.S).group(1).split(",")
+        assert signature == "".join("p" if "*" in a or "hfb_stream" in a else "l" if "int64_t" in a else "z" if "size_t" in a else "f" if "float" in a else "i"
+                                    for a in args), name
