@@ -23,7 +23,7 @@ struct Kv8WriteParams {
     void *q_out;
     uint8_t *cache;
     long long cache_slots;
-    int n_rot, n_positions, interleaved, T, H, G, d, block_size, record, lanes;
+    int n_rot, n_positions, interleaved, T, H, G, d, block_size, record, lanes, turns;
 };
 
 template <typename T, int PER> struct alignas(sizeof(T) * PER) Kv8Pack { T e[PER]; };
@@ -87,30 +87,27 @@ kv8_write_kernel(Kv8WriteParams p, int *err)
     // the successor may start once the kernel in front of this one is done: then all that was written to the cache before
     // this step is there for it, and its own wait covers what this kernel writes
     pdl_sync();
-    const int lane = threadIdx.x & 31, per_warp = 32 / p.lanes, heads = p.H + 2 * p.G;
-    const long long rows = (long long)p.T * heads;
+    // a block takes a token's heads 4 * 32 / lanes at a time, `turns` times
+    const int lane = threadIdx.x & 31, per_warp = 32 / p.lanes, heads = p.H + 2 * p.G, t = blockIdx.x;
     const int sub = lane / p.lanes, l = lane % p.lanes, e0 = l * PER;
-    for (long long r0 = ((long long)blockIdx.x * 4 + (threadIdx.x >> 5)) * per_warp; r0 < rows; r0 += (long long)gridDim.x * 4 * per_warp) {
-        const long long r = r0 + sub;
-        const bool mine = r < rows && e0 < p.d;
-        const int t = mine ? (int)(r / heads) : 0, head = mine ? (int)(r % heads) : 0;
+    int slot = p.slots ? p.slots[t] : -1;
+    const float *cs = nullptr;
+    if (slot >= p.cache_slots) { if (threadIdx.x == 0) atomicOr(err, HFB_ERR_SLOT); slot = -1; }
+    if (p.n_rot > 0) {
+        int pos = p.positions[t];
+        if (pos < 0 || pos >= p.n_positions) { if (threadIdx.x == 0) atomicOr(err, HFB_ERR_POSITION); pos = 0; }
+        cs = p.cos_sin + (size_t)pos * p.n_rot;
+    }
+    const int in_page = slot >= 0 ? slot % p.block_size : 0;
+    uint8_t *page = p.cache + (size_t)(slot >= 0 ? slot / p.block_size : 0) * p.G * p.record;
+    for (int n = 0; n < p.turns; n++) {
+        const int head = ((blockIdx.y * p.turns + n) * 4 + (threadIdx.x >> 5)) * per_warp + sub;
         const bool is_q = head < p.H, is_k = !is_q && head < p.H + p.G;
-        long long slot = -1;
-        if (mine && !is_q) {
-            slot = p.slots ? p.slots[t] : -1;
-            if (slot >= p.cache_slots) { if (l == 0) atomicOr(err, HFB_ERR_SLOT); slot = -1; }
-        }
-        const bool work = mine && (is_q || slot >= 0);
+        const bool work = head < heads && e0 < p.d && (is_q || slot >= 0);
         float x[PER], y[PER], c[PER], s[PER];
         unsigned second = 0, turned = 0;
         if (work) {
-            const float *cs = nullptr;
             const bool rotate = p.n_rot > 0 && (is_q || is_k);
-            if (rotate) {
-                int pos = p.positions[t];
-                if (pos < 0 || pos >= p.n_positions) { if (l == 0) atomicOr(err, HFB_ERR_POSITION); pos = 0; }
-                cs = p.cos_sin + (size_t)pos * p.n_rot;
-            }
             const T *row = is_q ? (const T *)p.q + t * p.q_stride + (size_t)head * p.d
                          : is_k ? (const T *)p.k + t * p.k_stride + (size_t)(head - p.H) * p.d
                                 : (const T *)p.v + t * p.v_stride + (size_t)(head - p.H - p.G) * p.d;
@@ -164,11 +161,10 @@ kv8_write_kernel(Kv8WriteParams p, int *err)
                 else codes[i / 4] |= b << (8 * (i % 4));
             }
             const int g = is_k ? head - p.H : head - p.H - p.G;
-            const int in_page = (int)(slot % p.block_size);
-            uint8_t *rec = p.cache + ((size_t)(slot / p.block_size) * p.G + g) * p.record;
+            uint8_t *rec = page + (size_t)g * p.record;
             uint8_t *dst = rec + (is_k ? 0 : p.block_size * p.d) + in_page * p.d + kv8_piece(in_page, e0 >> 4, p.d) * 16 + (e0 & 15);
-#pragma unroll
-            for (int i = 0; i < PER / 4; i++) ((uint32_t *)dst)[i] = codes[i];
+            if (PER == 8) *(uint2 *)dst = make_uint2(codes[0], codes[PER / 4 - 1]);
+            else *(uint32_t *)dst = codes[0];
             if (l == 0) ((float *)(rec + 2 * p.block_size * p.d))[(is_k ? 0 : p.block_size) + in_page] = scale;
         }
     }
@@ -181,45 +177,62 @@ __device__ __forceinline__ float kv8_value(uint32_t word, int i, float scale)
     return (float)((int)(word >> (8 * i) & 255u) - 128) * scale;
 }
 
+// A block takes as many records at once as its threads have pieces for, and four times that many before it stores any: a thread has the same
+// piece of each.
+constexpr int KV8_READ_THREADS = 256, KV8_READ_AHEAD = 4;
+
 template <typename T>
-__global__ void __launch_bounds__(256)
-kv8_read_kernel(const uint8_t *cache, long long num_pages, const int32_t *pages, const int32_t *used, T *k_out, T *v_out, long long N,
+__global__ void __launch_bounds__(KV8_READ_THREADS)
+kv8_read_kernel(const uint8_t *cache, long long num_pages, const int32_t *pages, const int32_t *used, T *k_out, T *v_out, int records,
                 int block_size, int G, int d, int record, int *err)
 {
     pdl_sync();
-    const int pieces = d / 16;
-    const long long items = N * G * 2 * block_size * pieces;
-    for (long long it = (long long)blockIdx.x * blockDim.x + threadIdx.x; it < items; it += (long long)gridDim.x * blockDim.x) {
-        const int c = (int)(it % pieces);
-        long long rest = it / pieces;
-        const int row = (int)(rest % block_size);
-        rest /= block_size;
-        const int kv = (int)(rest & 1);
-        rest >>= 1;
-        const int g = (int)(rest % G);
-        const long long n = rest / G;
-        const long long page = pages[n];
-        uint4 codes = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-        float scale = 0.f;
-        if (page >= num_pages) { if (c == 0 && row == 0) atomicOr(err, HFB_ERR_PAGE); }
-        else if (page >= 0 && row < used[n]) {
-            const uint8_t *rec = cache + ((size_t)page * G + g) * record;
-            codes = *(const uint4 *)(rec + (kv ? block_size * d : 0) + row * d + kv8_piece(row, c, d) * 16);
-            scale = ((const float *)(rec + 2 * block_size * d))[kv * block_size + row];
+    const int row_pieces = d / 16, pieces = 2 * block_size * row_pieces, at_once = max(1, KV8_READ_THREADS / pieces);
+    const int mine = threadIdx.x / pieces;                       // of the records at once (more pieces than threads: always 0)
+    if (mine >= at_once) return;
+    for (int i = threadIdx.x % pieces; i < pieces; i += KV8_READ_THREADS) {
+        const int kv = i / (pieces / 2), in_kv = i % (pieces / 2), row = in_kv / row_pieces, c = in_kv % row_pieces;
+        const size_t from = (size_t)(kv ? block_size * d : 0) + row * d + kv8_piece(row, c, d) * 16, scale_from = (size_t)2 * block_size * d + 4 * (kv * block_size + row);
+        T *out = (kv ? v_out : k_out) + (size_t)row * G * d + c * 16;
+        for (int r0 = blockIdx.x * at_once + mine; r0 < records; r0 += gridDim.x * at_once * KV8_READ_AHEAD) {
+            uint4 codes[KV8_READ_AHEAD];
+            float scale[KV8_READ_AHEAD];
+            int n[KV8_READ_AHEAD], g[KV8_READ_AHEAD];
+#pragma unroll
+            for (int u = 0; u < KV8_READ_AHEAD; u++) {
+                const int r = r0 + u * gridDim.x * at_once;
+                n[u] = r < records ? r / G : -1;
+                g[u] = r - n[u] * G;
+                codes[u] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+                scale[u] = 0.f;
+                if (n[u] < 0) continue;
+                const long long page = pages[n[u]];
+                if (page >= num_pages) { if (i == 0) atomicOr(err, HFB_ERR_PAGE); }
+                else if (page >= 0 && row < used[n[u]]) {
+                    const uint8_t *rec = cache + ((size_t)page * G + g[u]) * record;
+                    codes[u] = *(const uint4 *)(rec + from);
+                    scale[u] = *(const float *)(rec + scale_from);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < KV8_READ_AHEAD; u++) {
+                if (n[u] < 0) continue;
+                const uint32_t w[4] = {codes[u].x, codes[u].y, codes[u].z, codes[u].w};
+                T o[16];
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[e] = from_f32<T>(kv8_value(w[e >> 2], e & 3, scale[u]));
+                uint4 *dst = (uint4 *)(out + ((size_t)n[u] * block_size * G + g[u]) * d);
+#pragma unroll
+                for (int e = 0; e < (int)sizeof(T); e++) dst[e] = ((const uint4 *)o)[e];
+            }
         }
-        T o[16];
-#pragma unroll
-        for (int i = 0; i < 16; i++) o[i] = from_f32<T>(kv8_value(i < 4 ? codes.x : i < 8 ? codes.y : i < 12 ? codes.z : codes.w, i & 3, scale));
-        uint4 *dst = (uint4 *)((kv ? v_out : k_out) + ((n * block_size + row) * G + g) * d + c * 16);
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(T); i++) dst[i] = ((const uint4 *)o)[i];
     }
 }
 
 // ---- attention, plain kernel ---------------------------------------------------------------------------------------------
 // One block per (token, head); any head size, page size and mask, float32 throughout, for the float32 run and for what the
 // tiled kernels don't take.  s_j = scale (q . code_j) ks_j, softmax, out = sum_j p_j vs_j code'_j / sum_j p_j.  The warps take
-// groups of eight keys in turn and keep a maximum and sums each, merged in warp order at the end: the result depends only on the keys
+// groups of eight keys in turn (all of a group's reads in flight together) and keep a maximum and sums each, merged in warp order at the end: the result depends only on the keys
 // seen, never on the rest of the batch.  A lane holds four numbers of a row (WORDS times), as one word of codes.
 constexpr int KV8_WARPS = 8, KV8_KEYS = 8;
 
@@ -246,59 +259,80 @@ kv8_attention_plain_kernel(Kv8Params p, const int32_t *token_seq, int d, int *er
     const float scale = p.head_scales ? p.scale * p.head_scales[h] : p.scale;
     float m = -INFINITY, l = 0.f;
     for (int j0 = lo + warp * KV8_KEYS; j0 <= pos; j0 += KV8_WARPS * KV8_KEYS) {
-        float s[KV8_KEYS], vs[KV8_KEYS];
-        uint32_t vc[KV8_KEYS][WORDS];
+        // a key a lane: where its record and its row lie (-1: beyond the query, or no page), and its scales
+        long long at = -1;
+        float ks = 0.f, vs = 0.f;
+        const int j = j0 + (lane & (KV8_KEYS - 1)), row = j % bs;
+        if (j <= pos) {
+            const int blk = j / bs;
+            const long long page = blk < p.max_blocks ? table[blk] : -1;
+            if (page < 0 || page >= p.num_pages) { if (lane < KV8_KEYS) atomicOr(err, HFB_ERR_PAGE); }
+            else {
+                at = (page * p.G + g) * p.record;
+                const float *sc = (const float *)(p.cache + at + 2 * bs * d) + row;
+                ks = sc[0]; vs = sc[bs];
+            }
+        }
+        if (!__any_sync(0xffffffffu, at >= 0)) continue;
+        float dot[KV8_KEYS];
+        uint32_t kc[KV8_KEYS][WORDS], vc[KV8_KEYS][WORDS];
 #pragma unroll
         for (int k = 0; k < KV8_KEYS; k++) {
-            const int j = j0 + k, blk = j / bs, row = j % bs;
-            const long long page = j <= pos && blk < p.max_blocks ? table[blk] : -1;
-            const bool there = page >= 0 && page < p.num_pages;
-            if (j <= pos && !there && lane == 0) atomicOr(err, HFB_ERR_PAGE);
-            const uint8_t *rec = p.cache + ((size_t)(there ? page : 0) * p.G + g) * p.record;
-            float x = 0.f;
+            const long long its = __shfl_sync(0xffffffffu, at, k);
+            const int r = __shfl_sync(0xffffffffu, row, k);
 #pragma unroll
             for (int w = 0; w < WORDS; w++) {
                 const int e = 4 * (lane + 32 * w);
-                vc[k][w] = 0x80808080u;
-                if (there && e < d) {
-                    const int at = row * d + kv8_piece(row, e >> 4, d) * 16 + (e & 15);
-                    const uint32_t kc = *(const uint32_t *)(rec + at);
-                    vc[k][w] = *(const uint32_t *)(rec + bs * d + at);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) x = fmaf(q[w][i], kv8_value(kc, i, 1.f), x);
+                kc[k][w] = vc[k][w] = 0x80808080u;
+                if (its >= 0 && e < d) {
+                    const uint8_t *src = p.cache + its + r * d + kv8_piece(r, e >> 4, d) * 16 + (e & 15);
+                    kc[k][w] = *(const uint32_t *)src;
+                    vc[k][w] = *(const uint32_t *)(src + bs * d);
                 }
             }
-            const float *sc = (const float *)(rec + 2 * bs * d);
-            vs[k] = there ? sc[bs + row] : 0.f;
-            x = warp_sum(x) * (there ? sc[row] : 0.f) * scale;
-            if (p.softcap > 0.f) x = p.softcap * tanhf(x / p.softcap);
-            x -= slope * (float)(pos - j);
-            s[k] = there ? x : -INFINITY;
         }
-        float top = m;
 #pragma unroll
-        for (int k = 0; k < KV8_KEYS; k++) top = fmaxf(top, s[k]);
-        if (top == -INFINITY) {
-            bool any = false;                                            // (a key of which nothing is a number counts)
+        for (int k = 0; k < KV8_KEYS; k++) {
+            dot[k] = 0.f;
 #pragma unroll
-            for (int k = 0; k < KV8_KEYS; k++) any |= s[k] != s[k];
-            if (!any) continue;
+            for (int w = 0; w < WORDS; w++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) dot[k] = fmaf(q[w][i], kv8_value(kc[k][w], i, 1.f), dot[k]);
         }
-        const float corr = m == -INFINITY ? 0.f : expf(m - top);
-        l *= corr;
+        // the keys' sums over the lanes, all at once: key k ends up in the lanes whose number is k modulo 8
+#pragma unroll
+        for (int o = 1; o < KV8_KEYS; o <<= 1)
+#pragma unroll
+            for (int k = 0; k < KV8_KEYS; k += 2 * o)
+                dot[k] = (lane & o ? dot[k + o] : dot[k]) + __shfl_xor_sync(0xffffffffu, lane & o ? dot[k] : dot[k + o], o);
+        float x = dot[0];
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        x = x * ks * scale;
+        if (p.softcap > 0.f) x = p.softcap * tanhf(x / p.softcap);
+        x -= slope * (float)(pos - j);
+        if (at < 0) x = -INFINITY;
+        float top = fmaxf(m, x);
+#pragma unroll
+        for (int o = 1; o < KV8_KEYS; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const bool none = top == -INFINITY;                              // (keys of which nothing is a number)
+        const float corr = m == -INFINITY ? 0.f : expf(m - top), e = x == -INFINITY ? 0.f : expf(x - (none ? 0.f : top));
+        const float f = x == -INFINITY ? 0.f : e * vs;
+        float sum = e;
+#pragma unroll
+        for (int o = 1; o < KV8_KEYS; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        l = (l == 0.f ? 0.f : l * (none ? 1.f : corr)) + sum;
 #pragma unroll
         for (int w = 0; w < WORDS; w++)
 #pragma unroll
             for (int i = 0; i < 4; i++) acc[w][i] *= corr;
 #pragma unroll
         for (int k = 0; k < KV8_KEYS; k++) {
-            const float e = s[k] == -INFINITY ? 0.f : expf(s[k] - top);
-            l += e;
-            const float f = s[k] == -INFINITY ? 0.f : e * vs[k];
+            const float fk = __shfl_sync(0xffffffffu, f, k);
 #pragma unroll
             for (int w = 0; w < WORDS; w++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) acc[w][i] = fmaf(f, kv8_value(vc[k][w], i, 1.f), acc[w][i]);
+                for (int i = 0; i < 4; i++) acc[w][i] = fmaf(fk, kv8_value(vc[k][w], i, 1.f), acc[w][i]);
         }
         m = top;
     }
@@ -351,18 +385,23 @@ extern "C" int hfb_kv8_write(const void *q, int64_t q_stride, const void *k, int
     p.cache_slots = num_pages * block_size;
     p.n_rot = n_rot; p.n_positions = n_positions; p.interleaved = interleaved; p.T = T; p.H = H; p.G = G; p.d = d;
     p.block_size = block_size; p.record = kv8_record_bytes(block_size, d);
-    const int per = d > 128 ? 8 : 4;
-    p.lanes = 1;
-    while (p.lanes * per < d) p.lanes *= 2;
-    const long long rows = (long long)T * (H + 2 * G), blocks = (rows + 4 * (32 / p.lanes) - 1) / (4 * (32 / p.lanes));
-    const int grid = (int)(blocks < (1 << 20) ? blocks : (1 << 20));
-    // wide accesses where rows, table and rotated part allow them
+    // Wide accesses where rows, table and rotated part allow them; bfloat16 rows then go eight numbers a lane (16 bytes), others four (above
+    // 128 numbers a head eight).  A block takes as many turns as leave two rounds of blocks on the SMs.
     const uintptr_t all = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out | (uintptr_t)(n_rot ? cos_sin : nullptr);
     const long long strides = (H ? q_stride : 0) | (G ? k_stride | v_stride : 0);
-    const bool vec = !(all & 31 & (dt == HFB_F32 ? 4 * per - 1 : (2 * per - 1) | 15)) && strides % per == 0 && n_rot % (interleaved ? per : 2 * per) == 0;
+    auto wide = [&](int n) { return !(all & (dt == HFB_F32 && n == 8 ? 31 : 15)) && strides % n == 0 && n_rot % (interleaved ? n : 2 * n) == 0; };
+    const int per = d > 128 || (dt == HFB_BF16 && wide(8)) ? 8 : 4;
+    const bool vec = wide(per);
+    p.lanes = 1;
+    while (p.lanes * per < d) p.lanes *= 2;
+    const int at_once = 4 * (32 / p.lanes), parts = (H + 2 * G + at_once - 1) / at_once;
+    const long long spare = (long long)T * parts / (2 * 148 * 12);
+    p.turns = (int)(spare < 1 ? 1 : spare > parts ? parts : spare);
+    const dim3 grid(T, (parts + p.turns - 1) / p.turns);
+    if (grid.y > 65535) return fail(HFB_ENOTSUP, "kv8_write: %d heads exceed the grid limit", H + 2 * G);
 #define HFB_KV8_WRITE(TY, PER) \
-    g_launch_err = vec ? launch_pdl(kv8_write_kernel<TY, PER, true>, dim3(grid), dim3(128), 0, (cudaStream_t)s, p, error_word()) \
-                       : launch_pdl(kv8_write_kernel<TY, PER, false>, dim3(grid), dim3(128), 0, (cudaStream_t)s, p, error_word())
+    g_launch_err = vec ? launch_pdl(kv8_write_kernel<TY, PER, true>, grid, dim3(128), 0, (cudaStream_t)s, p, error_word()) \
+                       : launch_pdl(kv8_write_kernel<TY, PER, false>, grid, dim3(128), 0, (cudaStream_t)s, p, error_word())
     if (dt == HFB_F32) { if (per == 8) HFB_KV8_WRITE(float, 8); else HFB_KV8_WRITE(float, 4); }
     else { if (per == 8) HFB_KV8_WRITE(__nv_bfloat16, 8); else HFB_KV8_WRITE(__nv_bfloat16, 4); }
 #undef HFB_KV8_WRITE
@@ -377,15 +416,17 @@ extern "C" int hfb_kv8_read(const void *cache, int64_t num_pages, const int32_t 
         return fail(HFB_EINVAL, "kv8_read: bad arguments (G=%d)", G);
     if (!kv8_sizes(block_size, d)) return fail(HFB_ENOTSUP, "kv8_read: head size %d or page of %d tokens (multiples of 16 up to 256, 1..1024)", d, block_size);
     if (((uintptr_t)cache | (uintptr_t)k_out | (uintptr_t)v_out) & 15) return fail(HFB_EINVAL, "kv8_read: arrays must be 16-byte aligned");
-    const long long items = N * G * 2 * block_size * (d / 16), blocks = (items + 255) / 256;
-    const int grid = (int)(blocks < (1 << 20) ? blocks : (1 << 20));
+    const int pieces = 2 * block_size * (d / 16), at_once = pieces < KV8_READ_THREADS ? KV8_READ_THREADS / pieces : 1;
+    if (N * G >= (1ll << 31) - (1 << 24)) return fail(HFB_ENOTSUP, "kv8_read: %lld pages of %d heads", (long long)N, G);
+    const long long blocks = (N * G + at_once - 1) / at_once;
+    const int grid = (int)(blocks < 148 * 8 ? blocks : 148 * 8);          // (as many as are resident)
     const int record = kv8_record_bytes(block_size, d);
     if (out_dt == HFB_F32)
-        g_launch_err = launch_pdl(kv8_read_kernel<float>, dim3(grid), dim3(256), 0, (cudaStream_t)s, (const uint8_t *)cache, (long long)num_pages,
-                                  pages, used, (float *)k_out, (float *)v_out, (long long)N, block_size, G, d, record, error_word());
+        g_launch_err = launch_pdl(kv8_read_kernel<float>, dim3(grid), dim3(KV8_READ_THREADS), 0, (cudaStream_t)s, (const uint8_t *)cache, (long long)num_pages,
+                                  pages, used, (float *)k_out, (float *)v_out, (int)(N * G), block_size, G, d, record, error_word());
     else
-        g_launch_err = launch_pdl(kv8_read_kernel<__nv_bfloat16>, dim3(grid), dim3(256), 0, (cudaStream_t)s, (const uint8_t *)cache, (long long)num_pages,
-                                  pages, used, (__nv_bfloat16 *)k_out, (__nv_bfloat16 *)v_out, (long long)N, block_size, G, d, record, error_word());
+        g_launch_err = launch_pdl(kv8_read_kernel<__nv_bfloat16>, dim3(grid), dim3(KV8_READ_THREADS), 0, (cudaStream_t)s, (const uint8_t *)cache, (long long)num_pages,
+                                  pages, used, (__nv_bfloat16 *)k_out, (__nv_bfloat16 *)v_out, (int)(N * G), block_size, G, d, record, error_word());
     return check_pdl_launch(g_launch_err, "kv8_read");
 }
 
