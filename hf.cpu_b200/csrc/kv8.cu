@@ -1,18 +1,26 @@
 // The key/value cache in 8 bits (kv8.cuh): rows written to it, pages read back, and attention over it, plain kernel.
 #include "kv8.cuh"
+#include "tc_ptx.cuh"
 
 static thread_local cudaError_t g_launch_err = cudaSuccess;      // what the last launch_pdl returned
 
 namespace hfb {
 int *error_word();
 
+// Code i of a word as a number: the byte under 2^23's exponent is 2^23 + code + 128.  (Conversions between whole numbers and floats run at a
+// quarter of the additions' rate.)
+__device__ __forceinline__ float kv8_number(uint32_t word, int i)
+{
+    return __uint_as_float(__byte_perm(word, 0x4b000000u, 0x7440u + i)) - 8388736.f;
+}
+
 // ---- write ---------------------------------------------------------------------------------------------------------------
 // Rows q | k | v of a step: queries and keys are rotated; queries go out in the run's type, keys and values into the cache.
 //
-// A key is rotated in float64 and a value next to a border between two codes is divided in float64: the products of a 24-bit
-// number with the table's float32 are exact there, so that the codes are those of the definition and a row's codes don't
-// depend on the kernel that made them.  (float32 would move about one code in 10^5 to its neighbour.)  Queries are rotated as
-// the other kernels rotate them.
+// A key is rotated to twice float32's precision and a value next to a border between two codes is made and divided again in float64: the
+// products of a 24-bit number with the table's float32 are exact there, so that the codes are those of the definition and a row's
+// codes don't depend on the kernel that made them.  (Plain float32 would move about one code in 10^5 to its neighbour.)  Queries are
+// rotated as the other kernels rotate them.
 //
 // A row belongs to `lanes` (a power of two) neighbouring lanes, each with PER consecutive numbers of it.
 struct Kv8WriteParams {
@@ -28,58 +36,26 @@ struct Kv8WriteParams {
 
 template <typename T, int PER> struct alignas(sizeof(T) * PER) Kv8Pack { T e[PER]; };
 
-// (cos, sin) of the pairs that PER numbers from e0 on belong to, and whether each number is its pair's second.
-template <typename T, int PER, bool VEC>
-__device__ __forceinline__ void kv8_load(const T *row, int e0, const Kv8WriteParams &p, bool rotate, const float *cs, float (&x)[PER],
-                                         float (&y)[PER], float (&c)[PER], float (&s)[PER], unsigned &second, unsigned &turned)
+// x c + y s in float64: exact products, one rounding.  (A pair's first number is turned with -s, its second with s; a number that is not
+// turned has c = 1, s = y = 0.)
+__device__ __forceinline__ double kv8_turned(float x, float y, float c, float s) { return fma((double)x, (double)c, (double)y * s); }
+// The same in float32, rounded once from a sum of twice the precision (products and their errors, the sum and its error).
+__device__ __forceinline__ float kv8_turned_f32(float x, float y, float c, float s)
 {
-    // x: the numbers; y: their partners; bit i of `turned`: number i is rotated; of `second`: it is its pair's second
-    second = turned = 0;
-    const int half = p.n_rot / 2;
-    if (VEC) {
-        const Kv8Pack<T, PER> a = *(const Kv8Pack<T, PER> *)(row + e0);
-#pragma unroll
-        for (int i = 0; i < PER; i++) x[i] = to_f32(a.e[i]);
-        if (rotate && e0 < p.n_rot) {                    // (a lane's numbers are all rotated or all not, and all first or all second)
-            turned = (1u << PER) - 1u;
-            if (p.interleaved) {
-#pragma unroll
-                for (int i = 0; i < PER; i += 2) {
-                    y[i] = x[i + 1]; y[i + 1] = x[i];
-                    const float2 t = *(const float2 *)(cs + e0 + i);
-                    c[i] = c[i + 1] = t.x; s[i] = s[i + 1] = t.y;
-                    second |= 2u << i;
-                }
-            } else {
-                const bool up = e0 >= half;
-                const int i0 = up ? e0 - half : e0;
-                const Kv8Pack<T, PER> b = *(const Kv8Pack<T, PER> *)(row + (up ? i0 : e0 + half));
-                if (up) second = turned;
-#pragma unroll
-                for (int i = 0; i < PER; i += 2) {
-                    const float4 t = *(const float4 *)(cs + 2 * (i0 + i));
-                    c[i] = t.x; s[i] = t.y; c[i + 1] = t.z; s[i + 1] = t.w;
-                    y[i] = to_f32(b.e[i]); y[i + 1] = to_f32(b.e[i + 1]);
-                }
-            }
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const int e = e0 + i;
-            x[i] = to_f32(row[e]);
-            if (rotate && e < p.n_rot) {
-                const int pair = p.interleaved ? e >> 1 : (e < half ? e : e - half);
-                const bool up = p.interleaved ? e & 1 : e >= half;
-                y[i] = to_f32(row[p.interleaved ? e ^ 1 : (up ? e - half : e + half)]);
-                c[i] = cs[2 * pair]; s[i] = cs[2 * pair + 1];
-                turned |= 1u << i;
-                if (up) second |= 1u << i;
-            }
-        }
-    }
+    const float p = __fmul_rn(x, c), q = __fmul_rn(y, s), pe = __fmaf_rn(x, c, -p), qe = __fmaf_rn(y, s, -q);
+    const float sum = __fadd_rn(p, q), part = __fsub_rn(sum, p);
+    const float err = __fadd_rn(__fsub_rn(p, __fsub_rn(sum, part)), __fsub_rn(q, part));
+    return __fadd_rn(sum, __fadd_rn(err, __fadd_rn(pe, qe)));
 }
+// What few numbers need stays out of the way of the others.  The whole number is read off the low bits (code + 1.5 * 2^23).
+__device__ __noinline__ float kv8_code_at_border(float x, float y, float c, float s, float scale)
+{
+    return (float)rint(kv8_turned(x, y, c, s) / (double)scale) + 12582912.f;
+}
+__device__ __noinline__ float kv8_turned_tiny(float x, float y, float c, float s) { return (float)kv8_turned(x, y, c, s); }
 
+// Every head of a token is turned by the same table row, so that a lane reads its (cos, sin) once; a block takes 4 * 32 / lanes heads at a
+// time, `turns` times, with the next ones' rows on their way.
 template <typename T, int PER, bool VEC>
 __global__ void __launch_bounds__(128)
 kv8_write_kernel(Kv8WriteParams p, int *err)
@@ -87,79 +63,141 @@ kv8_write_kernel(Kv8WriteParams p, int *err)
     // the successor may start once the kernel in front of this one is done: then all that was written to the cache before
     // this step is there for it, and its own wait covers what this kernel writes
     pdl_sync();
-    // a block takes a token's heads 4 * 32 / lanes at a time, `turns` times
     const int lane = threadIdx.x & 31, per_warp = 32 / p.lanes, heads = p.H + 2 * p.G, t = blockIdx.x;
-    const int sub = lane / p.lanes, l = lane % p.lanes, e0 = l * PER;
+    const int sub = lane / p.lanes, l = lane % p.lanes, e0 = l * PER, half = p.n_rot / 2;
+    // where the numbers' partners are; which numbers are turned, and which are their pairs' second (VEC: all of a lane's are turned or none)
+    const int partner = p.interleaved ? e0 : e0 < half ? e0 + half : e0 - half;
+    auto turned = [&](int i) { return (VEC ? e0 : e0 + i) < p.n_rot; };
+    auto second = [&](int i) { return p.interleaved ? (i & 1) != 0 : (VEC ? e0 : e0 + i) >= half; };
+    const int first_head = blockIdx.y * p.turns * 4 * per_warp + (threadIdx.x >> 5) * per_warp + sub, step = 4 * per_warp;
+    Kv8Pack<T, PER> a, b;                                    // the coming row's numbers and their partners
+    auto load = [&](int head) {
+        if (head >= heads || e0 >= p.d) return;
+        const T *row = head < p.H ? (const T *)p.q + t * p.q_stride + (size_t)head * p.d
+                     : head < p.H + p.G ? (const T *)p.k + t * p.k_stride + (size_t)(head - p.H) * p.d
+                                        : (const T *)p.v + t * p.v_stride + (size_t)(head - p.H - p.G) * p.d;
+        const bool rotate = e0 < p.n_rot && head < p.H + p.G;
+        if (VEC) {                                           // (all of a lane's numbers are turned or none, all are first or all second)
+            a = *(const Kv8Pack<T, PER> *)(row + e0);
+            if (rotate && !p.interleaved) b = *(const Kv8Pack<T, PER> *)(row + partner);
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                a.e[i] = row[e0 + i];
+                if (rotate && turned(i)) b.e[i] = row[p.interleaved ? (e0 + i) ^ 1 : second(i) ? e0 + i - half : e0 + i + half];
+            }
+        }
+    };
+    load(first_head);
     int slot = p.slots ? p.slots[t] : -1;
-    const float *cs = nullptr;
-    if (slot >= p.cache_slots) { if (threadIdx.x == 0) atomicOr(err, HFB_ERR_SLOT); slot = -1; }
+    float c[PER], s[PER];                                    // (s: of a pair's first number with the sign turned)
+#pragma unroll
+    for (int i = 0; i < PER; i++) { c[i] = 1.f; s[i] = 0.f; }
     if (p.n_rot > 0) {
         int pos = p.positions[t];
         if (pos < 0 || pos >= p.n_positions) { if (threadIdx.x == 0) atomicOr(err, HFB_ERR_POSITION); pos = 0; }
-        cs = p.cos_sin + (size_t)pos * p.n_rot;
+        const float2 *cs = (const float2 *)(p.cos_sin + (size_t)pos * p.n_rot);
+        if (VEC) {
+            if (e0 < p.n_rot) {
+                cs += p.interleaved ? e0 / 2 : e0 < half ? e0 : e0 - half;
+#pragma unroll
+                for (int i = 0; i < PER; i += 2) {
+                    if (p.interleaved) { const float2 v = cs[i / 2]; c[i] = c[i + 1] = v.x; s[i] = -v.y; s[i + 1] = v.y; }
+                    else {
+                        const float4 v = *(const float4 *)(cs + i);
+                        c[i] = v.x; c[i + 1] = v.z;
+                        s[i] = e0 < half ? -v.y : v.y; s[i + 1] = e0 < half ? -v.w : v.w;
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER; i++)
+                if (turned(i)) {
+                    const float2 v = cs[p.interleaved ? (e0 + i) / 2 : second(i) ? e0 + i - half : e0 + i];
+                    c[i] = v.x;
+                    s[i] = second(i) ? v.y : -v.y;
+                }
+        }
     }
+    if (slot >= p.cache_slots) { if (threadIdx.x == 0) atomicOr(err, HFB_ERR_SLOT); slot = -1; }
     const int in_page = slot >= 0 ? slot % p.block_size : 0;
     uint8_t *page = p.cache + (size_t)(slot >= 0 ? slot / p.block_size : 0) * p.G * p.record;
     for (int n = 0; n < p.turns; n++) {
-        const int head = ((blockIdx.y * p.turns + n) * 4 + (threadIdx.x >> 5)) * per_warp + sub;
+        const int head = first_head + n * step;
         const bool is_q = head < p.H, is_k = !is_q && head < p.H + p.G;
         const bool work = head < heads && e0 < p.d && (is_q || slot >= 0);
-        float x[PER], y[PER], c[PER], s[PER];
-        unsigned second = 0, turned = 0;
-        if (work) {
-            const bool rotate = p.n_rot > 0 && (is_q || is_k);
-            const T *row = is_q ? (const T *)p.q + t * p.q_stride + (size_t)head * p.d
-                         : is_k ? (const T *)p.k + t * p.k_stride + (size_t)(head - p.H) * p.d
-                                : (const T *)p.v + t * p.v_stride + (size_t)(head - p.H - p.G) * p.d;
-            kv8_load<T, PER, VEC>(row, e0, p, rotate, cs, x, y, c, s, second, turned);
-        }
-        if (work && is_q) {
-            T o[PER];
+        const bool rotate = p.n_rot > 0 && (is_q || is_k);
+        float x[PER], y[PER];
 #pragma unroll
-            for (int i = 0; i < PER; i++) {
-                float lo = x[i], hi = x[i];
-                const bool up = second >> i & 1;
-                if (turned >> i & 1) rope_pair(up ? y[i] : x[i], up ? x[i] : y[i], c[i], s[i], lo, hi);
-                o[i] = from_f32<T>(up ? hi : lo);
-            }
+        for (int i = 0; i < PER; i++) {
+            x[i] = to_f32(a.e[i]);
+            y[i] = VEC && p.interleaved ? to_f32(a.e[i ^ 1]) : to_f32(b.e[i]);
+        }
+        if (n + 1 < p.turns) load(head + step);
+        if (work && is_q) {
+            Kv8Pack<T, PER> o;
+#pragma unroll
+            for (int i = 0; i < PER; i++)                    // (the arithmetic of rope_pair)
+                o.e[i] = from_f32<T>(rotate && turned(i) ? __fadd_rn(__fmul_rn(x[i], c[i]), __fmul_rn(y[i], s[i])) : x[i]);
             T *dst = (T *)p.q_out + ((size_t)t * p.H + head) * p.d + e0;
-            if (VEC) *(Kv8Pack<T, PER> *)dst = *(Kv8Pack<T, PER> *)o;
+            if (VEC) *(Kv8Pack<T, PER> *)dst = o;
             else
 #pragma unroll
-                for (int i = 0; i < PER; i++) dst[i] = o[i];
+                for (int i = 0; i < PER; i++) dst[i] = o.e[i];
         }
+        if (!__any_sync(0xffffffffu, work && !is_q)) continue;
         // keys and values: every lane of the row takes part in finding its largest magnitude (as bits: NaN > inf > finite)
-        double xd[PER];
+        float z[PER];
         unsigned top = 0;
         if (work && !is_q) {
 #pragma unroll
             for (int i = 0; i < PER; i++) {
-                xd[i] = x[i];
-                if (turned >> i & 1) {
-                    // first: x c - y s; second: y s + x c with y the pair's first
-                    const double a = (double)y[i] * s[i];
-                    xd[i] = fma((double)x[i], (double)c[i], second >> i & 1 ? a : -a);
-                }
-                x[i] = (float)xd[i];
-                top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+                if (!(rotate && turned(i))) y[i] = 0.f;
+                z[i] = rotate && turned(i) ? kv8_turned_f32(x[i], y[i], c[i], s[i]) : x[i];
+                top = max(top, __float_as_uint(z[i]) & 0x7fffffffu);
             }
         }
         for (int o = p.lanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        // (rows below 2^-80: the products' errors leave float32's range; above 2^120 their sums may)
+        const bool wild = work && is_k && rotate && (top < (47u << 23) || top > (247u << 23));
+        if (__any_sync(0xffffffffu, wild)) {
+            if (wild) {
+                top = 0;
+#pragma unroll
+                for (int i = 0; i < PER; i++) {
+                    if (turned(i)) z[i] = kv8_turned_tiny(x[i], y[i], c[i], s[i]);
+                    top = max(top, __float_as_uint(z[i]) & 0x7fffffffu);
+                }
+            }
+            for (int o = p.lanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        }
         if (work && !is_q) {
             const bool finite = top < 0x7f800000u;
             const float scale = finite ? fmaxf(__fdiv_rn(__uint_as_float(top), 127.f), 1.17549435e-38f) : __uint_as_float(0x7fc00000u);
             const float inv = finite ? 1.0f / scale : 0.f;
-            uint32_t codes[PER / 4];
+            float r[PER];
+            bool border = false;
 #pragma unroll
             for (int i = 0; i < PER; i++) {
-                const float u = x[i] * inv;
-                float code = rintf(u);
-                // (u is off by at most 127 * 3 * 2^-24 = 2.3e-5)
-                if (fabsf(fabsf(u - code) - 0.5f) < 1e-4f) code = (float)rint(xd[i] / (double)scale);
-                const uint32_t b = finite ? (uint32_t)((int)code + 128) : 128u;
-                if (i % 4 == 0) codes[i / 4] = b;
-                else codes[i / 4] |= b << (8 * (i % 4));
+                // (1.5 * 2^23 added: rounded to a whole number; u is off by at most 127 * 3 * 2^-24 = 2.3e-5)
+                const float u = finite ? z[i] * inv : 0.f;
+                r[i] = u + 12582912.f;
+                border |= fabsf(u - (r[i] - 12582912.f)) > 0.4999f;
             }
+            if (border) {
+#pragma unroll
+                for (int i = 0; i < PER; i++)
+                    if (fabsf(z[i] * inv - (r[i] - 12582912.f)) > 0.4999f) {
+                        const bool t2 = rotate && turned(i);
+                        r[i] = kv8_code_at_border(x[i], y[i], t2 ? c[i] : 1.f, t2 ? s[i] : 0.f, scale);
+                    }
+            }
+            uint32_t codes[PER / 4];
+#pragma unroll
+            for (int i = 0; i < PER; i += 4)                 // the low bytes, plus 128
+                codes[i / 4] = __byte_perm(__byte_perm(__float_as_uint(r[i]), __float_as_uint(r[i + 1]), 0x0040),
+                                           __byte_perm(__float_as_uint(r[i + 2]), __float_as_uint(r[i + 3]), 0x0040), 0x5410) ^ 0x80808080u;
             const int g = is_k ? head - p.H : head - p.H - p.G;
             uint8_t *rec = page + (size_t)g * p.record;
             uint8_t *dst = rec + (is_k ? 0 : p.block_size * p.d) + in_page * p.d + kv8_piece(in_page, e0 >> 4, p.d) * 16 + (e0 & 15);
@@ -171,15 +209,100 @@ kv8_write_kernel(Kv8WriteParams p, int *err)
 }
 
 // ---- read ----------------------------------------------------------------------------------------------------------------
-// The rows of some pages as the values that they stand for, [N, block, G, d] keys and values.  A thread takes 16 codes.
-__device__ __forceinline__ float kv8_value(uint32_t word, int i, float scale)
+// The rows of some pages as the values that they stand for, [N, block, G, d] keys and values.  A thread makes 16 bytes of the output at a
+// time, neighbouring threads neighbouring ones (32 a thread, in two stores, reached 3.9 of 6.5 TB/s).  A block takes as many records
+// at once as its threads have pieces for, and four times that many before it stores any: a thread has the same pieces of each.
+__device__ __forceinline__ void kv8_store(float *dst, const float (&v)[4]) { *(float4 *)dst = make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void kv8_store(__nv_bfloat16 *dst, const float (&v)[8])
 {
-    return (float)((int)(word >> (8 * i) & 255u) - 128) * scale;
+    const __nv_bfloat162 h[4] = {__floats2bfloat162_rn(v[0], v[1]), __floats2bfloat162_rn(v[2], v[3]), __floats2bfloat162_rn(v[4], v[5]),
+                                 __floats2bfloat162_rn(v[6], v[7])};
+    *(uint4 *)dst = *(const uint4 *)h;
 }
 
-// A block takes as many records at once as its threads have pieces for, and four times that many before it stores any: a thread has the same
-// piece of each.
-constexpr int KV8_READ_THREADS = 256, KV8_READ_AHEAD = 4;
+constexpr int KV8_READ_THREADS = 256, KV8_READ_AHEAD = 4, KV8_READ_STAGES = 4;
+
+// Records of up to 24 KB: brought whole by bulk copies, four ahead, by one thread; where a thread's pieces come from and go to is looked up
+// in a table that the block makes once (worked out for every piece it took three times the instructions).
+template <typename T>
+__global__ void __launch_bounds__(KV8_READ_THREADS)
+kv8_read_bulk_kernel(const uint8_t *cache, long long num_pages, const int32_t *pages, const int32_t *used, T *k_out, T *v_out, int records,
+                     int block_size, int G, int d, int record, int *err)
+{
+    constexpr int PER = 16 / sizeof(T);
+    extern __shared__ __align__(128) uint8_t kv8_smem[];
+    const int row_pieces = d / PER, pieces = 2 * block_size * row_pieces;
+    uint4 *table = (uint4 *)(kv8_smem + KV8_READ_STAGES * record);       // from, scale from, row, to (element; values' from the keys' end on)
+    const uint32_t bars = smem_u32(table + pieces), stages = smem_u32(kv8_smem);
+    volatile int *abort_flag = (volatile int *)((uint8_t *)(table + pieces) + 8 * KV8_READ_STAGES), *there = abort_flag + 1;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < KV8_READ_STAGES; s++) mbar_init(bars + 8 * s, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    for (int i = threadIdx.x; i < pieces; i += KV8_READ_THREADS) {
+        const int kv = i / (pieces / 2), in_kv = i % (pieces / 2), row = in_kv / row_pieces, c = in_kv % row_pieces * PER;
+        table[i] = make_uint4((kv ? block_size * d : 0) + row * d + kv8_piece(row, c >> 4, d) * 16 + (c & 15), 2 * block_size * d + 4 * (kv * block_size + row),
+                              row, row * G * d + c);
+    }
+    pdl_sync();
+    // (called by thread 0: `page` is that of record r)
+    auto ask = [&](int r, int page, int s) {
+        const bool is = page >= 0 && page < num_pages;
+        if (page >= num_pages) atomicOr(err, HFB_ERR_PAGE);
+        there[s] = is;
+        mbar_arrive_expect_tx(bars + 8 * s, is ? record : 0);
+        if (is)
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                         ::"r"(stages + s * record), "l"(cache + ((size_t)page * G + r % G) * record), "r"(record), "r"(bars + 8 * s) : "memory");
+    };
+    int coming = -1;                                             // page of the record that is asked for next
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < KV8_READ_STAGES; s++) {
+            const int r = blockIdx.x + s * gridDim.x;
+            if (r < records) ask(r, pages[r / G], s);
+        }
+        const int r = blockIdx.x + KV8_READ_STAGES * gridDim.x;
+        if (r < records) coming = pages[r / G];
+    }
+    __syncthreads();
+    int s = 0, phase = 0;
+    for (int r0 = blockIdx.x; r0 < records; r0 += gridDim.x) {
+        const bool ok = mbar_wait(bars + 8 * s, phase, abort_flag, err);
+        if (__syncthreads_or(!ok)) break;
+        const int n = r0 / G, g = r0 % G, rows = there[s] ? used[n] : 0;
+        const uint8_t *rec = kv8_smem + s * record;
+        const size_t to = ((size_t)n * block_size * G + g) * d;
+        for (int i = threadIdx.x; i < pieces; i += KV8_READ_THREADS) {
+            const uint4 e = table[i];
+            float v[PER];
+            if ((int)e.z < rows) {
+                const float scale = *(const float *)(rec + e.y);
+                uint32_t w[PER / 4];
+                if (PER == 8) { const uint2 c = *(const uint2 *)(rec + e.x); w[0] = c.x; w[PER / 4 - 1] = c.y; }
+                else w[0] = *(const uint32_t *)(rec + e.x);
+#pragma unroll
+                for (int u = 0; u < PER; u++) v[u] = kv8_number(w[u >> 2], u & 3) * scale;
+            } else {
+#pragma unroll
+                for (int u = 0; u < PER; u++) v[u] = 0.f;
+            }
+            kv8_store((i < pieces / 2 ? k_out : v_out) + to + e.w, v);
+        }
+        __syncthreads();                                         // the stage has been read
+        if (threadIdx.x == 0) {
+            const int r = r0 + KV8_READ_STAGES * gridDim.x, after = r + gridDim.x;
+            if (r < records) ask(r, coming, s);
+            if (after < records && after > r) coming = pages[after / G];
+        }
+        if (++s == KV8_READ_STAGES) { s = 0; phase ^= 1; }
+    }
+    __syncthreads();
+    if (*abort_flag != 0 && threadIdx.x == 0)                    // a wait ran out: copies still in flight land before the shared memory goes away
+        for (int i = 0; i < 2000; i++) __nanosleep(1000);
+    __syncthreads();
+}
 
 template <typename T>
 __global__ void __launch_bounds__(KV8_READ_THREADS)
@@ -187,15 +310,17 @@ kv8_read_kernel(const uint8_t *cache, long long num_pages, const int32_t *pages,
                 int block_size, int G, int d, int record, int *err)
 {
     pdl_sync();
-    const int row_pieces = d / 16, pieces = 2 * block_size * row_pieces, at_once = max(1, KV8_READ_THREADS / pieces);
+    constexpr int PER = 16 / sizeof(T);                          // codes of a piece: 8 or 4
+    const int row_pieces = d / PER, pieces = 2 * block_size * row_pieces, at_once = max(1, KV8_READ_THREADS / pieces);
     const int mine = threadIdx.x / pieces;                       // of the records at once (more pieces than threads: always 0)
     if (mine >= at_once) return;
     for (int i = threadIdx.x % pieces; i < pieces; i += KV8_READ_THREADS) {
-        const int kv = i / (pieces / 2), in_kv = i % (pieces / 2), row = in_kv / row_pieces, c = in_kv % row_pieces;
-        const size_t from = (size_t)(kv ? block_size * d : 0) + row * d + kv8_piece(row, c, d) * 16, scale_from = (size_t)2 * block_size * d + 4 * (kv * block_size + row);
-        T *out = (kv ? v_out : k_out) + (size_t)row * G * d + c * 16;
+        const int kv = i / (pieces / 2), in_kv = i % (pieces / 2), row = in_kv / row_pieces, c = in_kv % row_pieces * PER;
+        const size_t from = (size_t)(kv ? block_size * d : 0) + row * d + kv8_piece(row, c >> 4, d) * 16 + (c & 15);
+        const size_t scale_from = (size_t)2 * block_size * d + 4 * (kv * block_size + row);
+        T *out = (kv ? v_out : k_out) + (size_t)row * G * d + c;
         for (int r0 = blockIdx.x * at_once + mine; r0 < records; r0 += gridDim.x * at_once * KV8_READ_AHEAD) {
-            uint4 codes[KV8_READ_AHEAD];
+            uint32_t codes[KV8_READ_AHEAD][PER / 4];
             float scale[KV8_READ_AHEAD];
             int n[KV8_READ_AHEAD], g[KV8_READ_AHEAD];
 #pragma unroll
@@ -203,27 +328,26 @@ kv8_read_kernel(const uint8_t *cache, long long num_pages, const int32_t *pages,
                 const int r = r0 + u * gridDim.x * at_once;
                 n[u] = r < records ? r / G : -1;
                 g[u] = r - n[u] * G;
-                codes[u] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+#pragma unroll
+                for (int w = 0; w < PER / 4; w++) codes[u][w] = 0x80808080u;
                 scale[u] = 0.f;
                 if (n[u] < 0) continue;
                 const long long page = pages[n[u]];
                 if (page >= num_pages) { if (i == 0) atomicOr(err, HFB_ERR_PAGE); }
                 else if (page >= 0 && row < used[n[u]]) {
                     const uint8_t *rec = cache + ((size_t)page * G + g[u]) * record;
-                    codes[u] = *(const uint4 *)(rec + from);
+                    if (PER == 8) { const uint2 v = *(const uint2 *)(rec + from); codes[u][0] = v.x; codes[u][PER / 4 - 1] = v.y; }
+                    else codes[u][0] = *(const uint32_t *)(rec + from);
                     scale[u] = *(const float *)(rec + scale_from);
                 }
             }
 #pragma unroll
             for (int u = 0; u < KV8_READ_AHEAD; u++) {
                 if (n[u] < 0) continue;
-                const uint32_t w[4] = {codes[u].x, codes[u].y, codes[u].z, codes[u].w};
-                T o[16];
+                float v[PER];
 #pragma unroll
-                for (int e = 0; e < 16; e++) o[e] = from_f32<T>(kv8_value(w[e >> 2], e & 3, scale[u]));
-                uint4 *dst = (uint4 *)(out + ((size_t)n[u] * block_size * G + g[u]) * d);
-#pragma unroll
-                for (int e = 0; e < (int)sizeof(T); e++) dst[e] = ((const uint4 *)o)[e];
+                for (int e = 0; e < PER; e++) v[e] = kv8_number(codes[u][e >> 2], e & 3) * scale[u];
+                kv8_store(out + ((size_t)n[u] * block_size * G + g[u]) * d, v);
             }
         }
     }
@@ -297,7 +421,7 @@ kv8_attention_plain_kernel(Kv8Params p, const int32_t *token_seq, int d, int *er
 #pragma unroll
             for (int w = 0; w < WORDS; w++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) dot[k] = fmaf(q[w][i], kv8_value(kc[k][w], i, 1.f), dot[k]);
+                for (int i = 0; i < 4; i++) dot[k] = fmaf(q[w][i], kv8_number(kc[k][w], i), dot[k]);
         }
         // the keys' sums over the lanes, all at once: key k ends up in the lanes whose number is k modulo 8
 #pragma unroll
@@ -332,7 +456,7 @@ kv8_attention_plain_kernel(Kv8Params p, const int32_t *token_seq, int d, int *er
 #pragma unroll
             for (int w = 0; w < WORDS; w++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) acc[w][i] = fmaf(fk, kv8_value(vc[k][w], i, 1.f), acc[w][i]);
+                for (int i = 0; i < 4; i++) acc[w][i] = fmaf(fk, kv8_number(vc[k][w], i), acc[w][i]);
         }
         m = top;
     }
@@ -416,11 +540,31 @@ extern "C" int hfb_kv8_read(const void *cache, int64_t num_pages, const int32_t 
         return fail(HFB_EINVAL, "kv8_read: bad arguments (G=%d)", G);
     if (!kv8_sizes(block_size, d)) return fail(HFB_ENOTSUP, "kv8_read: head size %d or page of %d tokens (multiples of 16 up to 256, 1..1024)", d, block_size);
     if (((uintptr_t)cache | (uintptr_t)k_out | (uintptr_t)v_out) & 15) return fail(HFB_EINVAL, "kv8_read: arrays must be 16-byte aligned");
-    const int pieces = 2 * block_size * (d / 16), at_once = pieces < KV8_READ_THREADS ? KV8_READ_THREADS / pieces : 1;
+    const int pieces = 2 * block_size * (d / (out_dt == HFB_F32 ? 4 : 8)), at_once = pieces < KV8_READ_THREADS ? KV8_READ_THREADS / pieces : 1;
     if (N * G >= (1ll << 31) - (1 << 24)) return fail(HFB_ENOTSUP, "kv8_read: %lld pages of %d heads", (long long)N, G);
+    const int record = kv8_record_bytes(block_size, d);
+    if (record <= 24 * 1024) {
+        const int smem = KV8_READ_STAGES * record + pieces * 16 + 8 * KV8_READ_STAGES + 4 + 4 * KV8_READ_STAGES;
+        static bool configured[64] = {false};                             // (the opt-in is a property of the function on one device)
+        if (!configured[current_device()]) {
+            cudaError_t e = cudaFuncSetAttribute(kv8_read_bulk_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+            if (e == cudaSuccess) e = cudaFuncSetAttribute(kv8_read_bulk_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+            if (e != cudaSuccess) return fail(HFB_ECUDA, "kv8_read: cannot opt in to shared memory: %s", cudaGetErrorString(e));
+            configured[current_device()] = true;
+        }
+        const int resident = 148 * (smem > 110 * 1024 ? 1 : smem > 74 * 1024 ? 2 : smem > 55 * 1024 ? 3 : smem > 36 * 1024 ? 4 : 6);
+        const int grid = (int)(N * G < resident ? N * G : resident);
+        if (out_dt == HFB_F32)
+            g_launch_err = launch_pdl(kv8_read_bulk_kernel<float>, dim3(grid), dim3(KV8_READ_THREADS), smem, (cudaStream_t)s, (const uint8_t *)cache,
+                                      (long long)num_pages, pages, used, (float *)k_out, (float *)v_out, (int)(N * G), block_size, G, d, record, error_word());
+        else
+            g_launch_err = launch_pdl(kv8_read_bulk_kernel<__nv_bfloat16>, dim3(grid), dim3(KV8_READ_THREADS), smem, (cudaStream_t)s, (const uint8_t *)cache,
+                                      (long long)num_pages, pages, used, (__nv_bfloat16 *)k_out, (__nv_bfloat16 *)v_out, (int)(N * G), block_size, G, d, record,
+                                      error_word());
+        return check_pdl_launch(g_launch_err, "kv8_read");
+    }
     const long long blocks = (N * G + at_once - 1) / at_once;
     const int grid = (int)(blocks < 148 * 8 ? blocks : 148 * 8);          // (as many as are resident)
-    const int record = kv8_record_bytes(block_size, d);
     if (out_dt == HFB_F32)
         g_launch_err = launch_pdl(kv8_read_kernel<float>, dim3(grid), dim3(KV8_READ_THREADS), 0, (cudaStream_t)s, (const uint8_t *)cache, (long long)num_pages,
                                   pages, used, (float *)k_out, (float *)v_out, (int)(N * G), block_size, G, d, record, error_word());
