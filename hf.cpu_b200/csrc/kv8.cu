@@ -54,10 +54,12 @@ __device__ __noinline__ float kv8_code_at_border(float x, float y, float c, floa
 }
 __device__ __noinline__ float kv8_turned_tiny(float x, float y, float c, float s) { return (float)kv8_turned(x, y, c, s); }
 
-// Every head of a token is turned by the same table row, so that a lane reads its (cos, sin) once; a block takes 4 * 32 / lanes heads at a
+// Every head of a token is turned by the same table row, so that a lane reads its (cos, sin) once; a block takes 8 * 32 / lanes heads at a
 // time, `turns` times, with the next ones' rows on their way.
+constexpr int KV8_WRITE_THREADS = 256, KV8_WRITE_WARPS = KV8_WRITE_THREADS / 32;
+
 template <typename T, int PER, bool VEC>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(KV8_WRITE_THREADS)
 kv8_write_kernel(Kv8WriteParams p, int *err)
 {
     // the successor may start once the kernel in front of this one is done: then all that was written to the cache before
@@ -69,7 +71,7 @@ kv8_write_kernel(Kv8WriteParams p, int *err)
     const int partner = p.interleaved ? e0 : e0 < half ? e0 + half : e0 - half;
     auto turned = [&](int i) { return (VEC ? e0 : e0 + i) < p.n_rot; };
     auto second = [&](int i) { return p.interleaved ? (i & 1) != 0 : (VEC ? e0 : e0 + i) >= half; };
-    const int first_head = blockIdx.y * p.turns * 4 * per_warp + (threadIdx.x >> 5) * per_warp + sub, step = 4 * per_warp;
+    const int first_head = (blockIdx.y * p.turns * KV8_WRITE_WARPS + (threadIdx.x >> 5)) * per_warp + sub, step = KV8_WRITE_WARPS * per_warp;
     Kv8Pack<T, PER> a, b;                                    // the coming row's numbers and their partners
     auto load = [&](int head) {
         if (head >= heads || e0 >= p.d) return;
@@ -510,22 +512,22 @@ extern "C" int hfb_kv8_write(const void *q, int64_t q_stride, const void *k, int
     p.n_rot = n_rot; p.n_positions = n_positions; p.interleaved = interleaved; p.T = T; p.H = H; p.G = G; p.d = d;
     p.block_size = block_size; p.record = kv8_record_bytes(block_size, d);
     // Wide accesses where rows, table and rotated part allow them; bfloat16 rows then go eight numbers a lane (16 bytes), others four (above
-    // 128 numbers a head eight).  A block takes as many turns as leave two rounds of blocks on the SMs.
+    // 128 numbers a head eight).  A block takes as many turns as leave a round of blocks on the SMs.
     const uintptr_t all = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out | (uintptr_t)(n_rot ? cos_sin : nullptr);
     const long long strides = (H ? q_stride : 0) | (G ? k_stride | v_stride : 0);
     auto wide = [&](int n) { return !(all & (dt == HFB_F32 && n == 8 ? 31 : 15)) && strides % n == 0 && n_rot % (interleaved ? n : 2 * n) == 0; };
-    const int per = d > 128 || (dt == HFB_BF16 && wide(8)) ? 8 : 4;
+    const int per = d > 128 ? 8 : 4;
     const bool vec = wide(per);
     p.lanes = 1;
     while (p.lanes * per < d) p.lanes *= 2;
-    const int at_once = 4 * (32 / p.lanes), parts = (H + 2 * G + at_once - 1) / at_once;
-    const long long spare = (long long)T * parts / (2 * 148 * 12);
+    const int at_once = KV8_WRITE_WARPS * (32 / p.lanes), parts = (H + 2 * G + at_once - 1) / at_once;
+    const long long spare = (long long)T * parts / (148 * 4);
     p.turns = (int)(spare < 1 ? 1 : spare > parts ? parts : spare);
     const dim3 grid(T, (parts + p.turns - 1) / p.turns);
     if (grid.y > 65535) return fail(HFB_ENOTSUP, "kv8_write: %d heads exceed the grid limit", H + 2 * G);
 #define HFB_KV8_WRITE(TY, PER) \
-    g_launch_err = vec ? launch_pdl(kv8_write_kernel<TY, PER, true>, grid, dim3(128), 0, (cudaStream_t)s, p, error_word()) \
-                       : launch_pdl(kv8_write_kernel<TY, PER, false>, grid, dim3(128), 0, (cudaStream_t)s, p, error_word())
+    g_launch_err = vec ? launch_pdl(kv8_write_kernel<TY, PER, true>, grid, dim3(KV8_WRITE_THREADS), 0, (cudaStream_t)s, p, error_word()) \
+                       : launch_pdl(kv8_write_kernel<TY, PER, false>, grid, dim3(KV8_WRITE_THREADS), 0, (cudaStream_t)s, p, error_word())
     if (dt == HFB_F32) { if (per == 8) HFB_KV8_WRITE(float, 8); else HFB_KV8_WRITE(float, 4); }
     else { if (per == 8) HFB_KV8_WRITE(__nv_bfloat16, 8); else HFB_KV8_WRITE(__nv_bfloat16, 4); }
 #undef HFB_KV8_WRITE
