@@ -210,9 +210,11 @@ kv8_write_kernel(Kv8WriteParams p, int *err)
     }
 }
 
+// Measured: 2,048 tokens, 28 heads of 128 on 4, 21 us: the instructions per row (about 180 a warp) bound it, not the 37 MB.
+
 // ---- read ----------------------------------------------------------------------------------------------------------------
 // The rows of some pages as the values that they stand for, [N, block, G, d] keys and values.  A thread makes 16 bytes of the output at a
-// time, neighbouring threads neighbouring ones (32 a thread, in two stores, reached 3.9 of 6.5 TB/s).  A block takes as many records
+// time, neighbouring threads neighbouring ones.  A block takes as many records
 // at once as its threads have pieces for, and four times that many before it stores any: a thread has the same pieces of each.
 __device__ __forceinline__ void kv8_store(float *dst, const float (&v)[4]) { *(float4 *)dst = make_float4(v[0], v[1], v[2], v[3]); }
 __device__ __forceinline__ void kv8_store(__nv_bfloat16 *dst, const float (&v)[8])
@@ -225,7 +227,8 @@ __device__ __forceinline__ void kv8_store(__nv_bfloat16 *dst, const float (&v)[8
 constexpr int KV8_READ_THREADS = 256, KV8_READ_AHEAD = 4, KV8_READ_STAGES = 4;
 
 // Records of up to 24 KB: brought whole by bulk copies, four ahead, by one thread; where a thread's pieces come from and go to is looked up
-// in a table that the block makes once (worked out for every piece it took three times the instructions).
+// in a table that the block makes once (worked out for every piece it took three times the instructions).  81,936 tokens of 4 heads of
+// 128 into bfloat16: 45 us of the kernel's own (61 with plain loads), 52 us a pass among others, 0.60 of the measured bandwidth.
 template <typename T>
 __global__ void __launch_bounds__(KV8_READ_THREADS)
 kv8_read_bulk_kernel(const uint8_t *cache, long long num_pages, const int32_t *pages, const int32_t *used, T *k_out, T *v_out, int records,
@@ -511,8 +514,9 @@ extern "C" int hfb_kv8_write(const void *q, int64_t q_stride, const void *k, int
     p.cache_slots = num_pages * block_size;
     p.n_rot = n_rot; p.n_positions = n_positions; p.interleaved = interleaved; p.T = T; p.H = H; p.G = G; p.d = d;
     p.block_size = block_size; p.record = kv8_record_bytes(block_size, d);
-    // Wide accesses where rows, table and rotated part allow them; bfloat16 rows then go eight numbers a lane (16 bytes), others four (above
-    // 128 numbers a head eight).  A block takes as many turns as leave a round of blocks on the SMs.
+    // Wide accesses where rows, table and rotated part allow them.  Four numbers a lane (above 128 numbers a head eight): with eight, half
+    // as many lanes share a row's fixed work, but half as many warps fit (2,048 rows of 36 heads of 128: 21.3 us with four, 25.7 with
+    // eight).  A block takes as many turns as leave a round of blocks on the SMs.
     const uintptr_t all = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out | (uintptr_t)(n_rot ? cos_sin : nullptr);
     const long long strides = (H ? q_stride : 0) | (G ? k_stride | v_stride : 0);
     auto wide = [&](int n) { return !(all & (dt == HFB_F32 && n == 8 ? 31 : 15)) && strides % n == 0 && n_rot % (interleaved ? n : 2 * n) == 0; };

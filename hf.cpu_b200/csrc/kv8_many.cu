@@ -7,8 +7,8 @@
 //   each of a tile of 128, while the softmax of the tile before runs.  The reference is the power of two above the largest scale of the 32
 //   keys, which is left to the softmax as one factor for 32 columns.  A number is rounded once to 11 bits (keys; their scale goes in as
 //   a sum of two float16) or, with its scale, twice (values); half a step is 2^-11 of the number, an eighth of what bfloat16 keys and
-//   values lose.  (Scales applied to scores and weights in float32 instead took two reads of shared memory for every four scores: each
-//   brings a thread 16 bytes, 512 a warp, and those reads alone were 4,700 of 9,400 cycles a step: 436 us where this takes ###.)
+//   values lose.  (Scales applied to scores and weights in float32 by the softmax's threads: two reads of shared memory and
+//   two multiplications for every four scores, 3 % of the time.)
 // * each of these warps asks for its keys' codes of the next tile as soon as it has converted the last ones, and both operands have two
 //   places, so that the conversion runs a tile ahead of the products.
 // * a row whose key or value is no number makes its scores so and leaves its values zero: a weight of zero stays zero in the sums of the
@@ -24,6 +24,8 @@
 // * work is cut evenly (as in kv8_few.cu): a step is a tile of keys of one double tile and key/value head, CTA c of C walks steps c N / C to
 //   (c + 1) N / C.  What a CTA has of a double tile that others share goes to scratch, and whoever brings its last piece merges them, in
 //   the order of the keys.  (Whole double tiles a CTA: 228 items of 2,048 tokens and 28 heads are two rounds on 148 SMs where 1.5 would do.)
+// Measured: 2,048 tokens behind 6,144, 28 heads of 128 on 4: 316 us, 666 TFLOP/s, 0.41 of the measured bf16 rate; the bfloat16 cache's kernel
+// takes 288 us.  Steps without the conversion take 268: its instructions and the softmax's share the issue slots.
 // Barrier waits are bounded (HFB_ERR_WAIT, TMEM freed; tc_ptx.cuh).
 #include <cuda_fp16.h>
 
@@ -464,7 +466,7 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                 const bool open = __all_sync(0xffffffffu, !valid || (key0 + KM_KEYS - 1 <= pos && key0 >= lo)) && full && !finished;
                 const float b0 = slope2 * (float)(key0 - pos), by_head = unit * hscale;
                 // (loops over the quarters of a tile stay loops: eight warps of these run beside four that convert, and unrolled their
-                // instructions do not stay in the caches: ### us)
+                // instructions do not stay in the caches: 410 us for the portion named above, 358 so)
                 auto load32 = [&](int q, uint32_t (&raw)[32]) { tmem_ld16(tS + 32 * q, raw); tmem_ld16(tS + 32 * q + 16, raw + 16); };
                 auto k_ref = [&](int q) { return km_load1(s_at + 4u * q); };
                 auto v_log = [&](int q) { return km_load1(s_at + 16u + 4u * q); };

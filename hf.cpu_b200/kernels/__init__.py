@@ -416,7 +416,7 @@ def kv8_head_groups(heads_per_group: int) -> int:
     return next(s for s in range(1, heads_per_group + 1) if heads_per_group <= 16 * s and heads_per_group % s == 0)
 
 
-KV8_MANY = 64               # query rows (tokens times heads on a key/value head) of a request from which its portion is a prompt's
+KV8_MANY = 64               # query rows (tokens times heads on a key/value head) above which a request's portion goes to the prompts' kernel
 
 
 def kv8_step_arrays(q_lens, heads_per_group: int):

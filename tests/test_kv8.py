@@ -202,3 +202,28 @@ def test_argument_types_are_the_headers():
         args = re.search(r"int %s\((.*?)\);" % name, header, re.S).group(1).split(",")
         assert signature == "".join("p" if "*" in a or "hfb_stream" in a else "l" if "int64_t" in a else "z" if "size_t" in a else "f" if "float" in a else "i"
                                     for a in args), name
+
+
+@pytest.mark.parametrize("arch", ["manapel", "tupalorn"])
+def test_other_architectures_plain_layers(emu, arch):
+    """Layers with head norms, a norm over the row, caches that other layers read: on 8 bits near the plain cache, and forks too."""
+    import importlib
+    cfg = config_from_dict(importlib.import_module(arch + "_util").WIDE)
+    got = {}
+    for kv in ("auto", "int8"):
+        model = random_model(cfg, seed=3, dtype=torch.float32, device="cpu", std=0.05)
+        eng = Engine(model, block_size=16, max_tokens=512, max_requests=2, ctx_max=256, kv_dtype=kv)
+        ids = [int(x) for x in torch.randint(0, model.plan.vocab_size, (50,), generator=torch.Generator().manual_seed(1))]
+        eng.add_request("r")
+        eng.step([StepEntry("r", ids[:30], [29])])
+        got[kv] = eng.step([StepEntry("r", ids[30:], [19])]).clone()
+    assert not torch.equal(got["auto"], got["int8"])
+    assert float((got["auto"] - got["int8"]).abs().max() / got["auto"].abs().max()) < 0.05
+
+
+@pytest.mark.parametrize("arch", ["peludra", "mokisun", "silupel", "birizen"])
+def test_latent_and_other_mixers_are_refused(emu, arch):
+    import importlib
+    model = random_model(config_from_dict(importlib.import_module(arch + "_util").WIDE), seed=3, dtype=torch.float32, device="cpu", std=0.05)
+    with pytest.raises(UnsupportedError, match="8 bits"):
+        Engine(model, block_size=16, max_tokens=512, max_requests=2, ctx_max=128, kv_dtype="int8")
