@@ -47,6 +47,11 @@ from ..weights.loader import TensorSpec, fused_rows, pad_rows
 from .base import CacheSpec, Mixer, register_part
 
 
+def _records(cache):
+    """The records of a cache in 8 bits; None of any other."""
+    return getattr(cache, "kv8", None)
+
+
 class OutputProduct:
     """What mixers that end in one product over the concatenated heads share: ``self._attend(ctx, xn, cache,
     write_cache)`` gives the heads' outputs, ``self.w_o`` / ``self.b_o`` carry them back to the stream."""
@@ -310,7 +315,7 @@ class PagedAttention(OutputProduct, Mixer):
         T, meta = x.shape[0], ctx.group_meta(cache.group)
         q = ctx.buf("attn_q", (T, self.QD), ctx.run_dtype)
         with kernels.phase("qkv"):
-            if cache.kv8 is not None:
+            if _records(cache) is not None:
                 qkv = ctx.buf("attn_qkv", (T, self.QD + 2 * self.KD), ctx.run_dtype)
                 kernels.few_linear(x, norm, self.w_qkv, self.b_qkv, qkv, False)
                 kernels.rope_kv8_write(qkv, self.rotary.cos_sin, self.rotary.n_rot, ctx.positions, meta.slots if write_cache else None, q, cache.kv8,
@@ -338,7 +343,7 @@ class PagedAttention(OutputProduct, Mixer):
 
     def _softmax_attention(self, ctx, q, cache, meta):
         att = ctx.buf("attn_out", (q.shape[0], self.OD), q.dtype)
-        if cache.kv8 is not None:
+        if _records(cache) is not None:
             # (all that lies before the step's tokens was written by earlier steps)
             with kernels.phase("attn"):
                 kernels.paged_attention_kv8(q, cache.kv8, meta, ctx, self.H, self.G, self.d, self.mask, self.scale, att,
@@ -355,14 +360,14 @@ class PagedAttention(OutputProduct, Mixer):
     def _kv_places(self, ctx, T, G, cache, meta, write_cache):
         """Where a tail that makes keys and values puts them: the cache at the step's slots, or, in front of a cache in 8 bits, rows of
         the step's own, one behind the other."""
-        if cache.kv8 is None:
+        if _records(cache) is None:
             return cache.k, None if self.values_are_keys else cache.v, meta.slots if write_cache else None
         shape = (T, 1, max(G, 1), self.d)
         k, v = (ctx.buf(name, shape, ctx.run_dtype) for name in ("attn_new_k", "attn_new_v"))
         return k, v, ctx.engine.places(T) if write_cache else None
 
     def _kv_to_8bits(self, T, k, v, cache, meta, slots):
-        if cache.kv8 is not None and slots is not None:
+        if _records(cache) is not None and slots is not None:
             kernels.kv8_write(k.view(T, self.KD), v.view(T, self.KD), meta.slots, cache.kv8, self.G, self.d, meta.block_size)
 
     def _attend(self, ctx, xn, cache, write_cache):
@@ -392,7 +397,7 @@ class PagedAttention(OutputProduct, Mixer):
                                             self.H, G, self.d, dv_row, self.qk_norm_eps, norm_weights=self.norm_w, value_mix=mix,
                                             pairing=self.pairing)
                 self._kv_to_8bits(T, k, v, cache, meta, slots)
-        elif cache.kv8 is not None:
+        elif _records(cache) is not None:
             qkv = ctx.buf("attn_qkv", (T, self.QD + 2 * self.KD), xn.dtype)
             with kernels.phase("qkv"):
                 kernels.linear(xn, self.w_qkv, self.b_qkv, qkv, accumulate=False)
