@@ -40,6 +40,9 @@ namespace hfb {
 int *error_word();
 
 constexpr int KM_ROWS = 128, KM_KEYS = 128, KM_THREADS = 416, KM_TMEM_COLS = 512;
+// Fewest steps that are worth a CTA of their own: a piece costs its merge 64 KB or 128 KB of reads by one CTA.  Four requests of 1,024 tokens,
+// 28 heads of 128 on 4: 43, 57, 64 us with 3, 6, 10; one of 8,192: 92, 70, 71, where the kernel of few queries is taken anyway.
+constexpr int KM_MIN_STEPS = 3;
 constexpr uint32_t KM_SUB = 128 * 64 * 2;           // one swizzled sub-tile: 128 rows of 64 float16
 
 struct Kv8ManyParams {
@@ -178,7 +181,7 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
     int before = up - mine, per_head = 0;
     for (int w = 0; w < KM_THREADS / 32; w++) { if (w < warp) before += scan[w]; per_head += scan[w]; }
     const long long total = (long long)per_head * p.G;
-    const int ctas = (int)min((long long)gridDim.x, total), cta = blockIdx.x;
+    const int ctas = (int)max(1ll, min((long long)gridDim.x, total / KM_MIN_STEPS)), cta = blockIdx.x;
     if (cta >= ctas) return;
     auto start_of = [&](int c) { return total * c / ctas; };
     const long long x_start = start_of(cta), x_end = start_of(cta + 1);

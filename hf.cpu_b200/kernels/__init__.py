@@ -416,7 +416,12 @@ def kv8_head_groups(heads_per_group: int) -> int:
     return next(s for s in range(1, heads_per_group + 1) if heads_per_group <= 16 * s and heads_per_group % s == 0)
 
 
-KV8_MANY = 64               # query rows (tokens times heads on a key/value head) above which a request's portion goes to the prompts' kernel
+# A request's portion goes to the prompts' kernel if it has more query rows (tokens times heads on a key/value head) than KV8_MANY and all such
+# portions of the step together more than KV8_MANY_ROWS.  That kernel's cost is the same for 1 to 256 rows a request, the other's grows
+# with every 16.  Measured in us, few | many, by rows a request: 16 requests of 8,192 tokens, 28 heads of 128 on 4, 35 rows 128 | 114, 63 rows 199 | 117; 14
+# heads of 64 on 2, 35 rows 53 | 66, 63 rows 73 | 66; four requests, 28 heads, 63 rows 66 | 76, 112 rows 92 | 78; one request, 252 rows
+# 61 | 104, 896 rows 162 | 90; four of 1,024 tokens, 112 rows 34 | 45, 252 rows 49 | 52.
+KV8_MANY, KV8_MANY_ROWS = 32, 512
 
 
 def kv8_step_arrays(q_lens, heads_per_group: int):
@@ -428,6 +433,8 @@ def kv8_step_arrays(q_lens, heads_per_group: int):
     first = (np.cumsum(q) - q).astype(np.int32)
     share = kv8_head_groups(heads_per_group)
     long = (q > 1) & (q * heads_per_group > KV8_MANY) & (heads_per_group <= 128)
+    if int(q[long].sum()) * heads_per_group <= KV8_MANY_ROWS:
+        long[:] = False
     out = {}
     for name, of, per in (("few", np.flatnonzero(~long), 1 if share > 1 else max(1, 16 // heads_per_group)),
                           ("many", np.flatnonzero(long), 2 * (128 // max(1, min(heads_per_group, 128))))):

@@ -221,6 +221,12 @@ STEPS = {                                                    # what requests bri
     "portion": ([70], [70]), "behind": ([100, 33], [420, 700]), "mixed": ([1, 90, 1, 3, 130, 1], [500, 90, 1, 260, 300, 64])}
 
 
+@pytest.fixture(autouse=True)
+def prompts_kernel_for_small_steps(monkeypatch):
+    """Lets small portions reach the kernel for prompts, which otherwise waits for rows enough."""
+    monkeypatch.setattr(native(), "KV8_MANY_ROWS", 64)
+
+
 @pytest.mark.parametrize("name", list(STEPS))
 @pytest.mark.parametrize("shape", SHAPES + OTHER, ids=str)
 def test_attention(shape, name):
