@@ -544,3 +544,36 @@ def test_session_generates_on_8_bits(tiny_folders):
     c = sess.generate(prompts[2], n=2, **kw)
     assert c[0].tokens == c[1].tokens
     sess.engine.cache.check()
+
+
+@pytest.mark.parametrize("heads", [(8, 2, 64), (8, 2, 128)])
+def test_alike_layers_made_again_give_the_same_bits(heads, monkeypatch):
+    """A step through recorded launches against the same step layer by layer, on records of layers that differ in nothing else:
+    portions on either kernel, several requests, single tokens."""
+    from hfcpu_b200.config import config_from_dict
+    from hfcpu_b200.engine import Engine, StepEntry
+    from hfcpu_b200.kernels.native import Recording
+    from hfcpu_b200.models import random_model
+    K, (H, G, d) = native(), heads
+    config = config_from_dict(dict(architectures=["Qwen2ForCausalLM"], num_hidden_layers=5, hidden_size=H * d, num_attention_heads=H,
+                                   num_key_value_heads=G, intermediate_size=1024, vocab_size=1000, max_position_embeddings=1024,
+                                   rms_norm_eps=1e-6, rope_theta=1e6, tie_word_embeddings=False))
+    model, made, inner = random_model(config, seed=5, dtype=torch.bfloat16, device=DEV, std=0.08), [], Recording.replay
+
+    def replay(self, tensors):
+        made.append(inner(self, tensors))
+        return made[-1]
+    monkeypatch.setattr(Recording, "replay", replay)
+    got = []
+    for record in (True, False):
+        if not record:
+            monkeypatch.setattr(K, "recorder", lambda: None)
+        engine = Engine(model, block_size=16, max_tokens=2048, max_requests=4, kv_dtype="int8")
+        engine.use_graphs = False
+        engine.add_request("a")
+        engine.add_request("b")
+        got.append(torch.stack([engine.step([StepEntry(r, [(7 * i + n + (r == "b")) % 1000 for i in range(n)], [n - 1]) for r in "ab"]).clone()
+                                for n in (300, 40, 3, 1, 1)]))
+    assert torch.equal(got[0], got[1]) and torch.isfinite(got[0]).all()
+    assert len(made) >= 10 and all(made)
+    K.check_device_errors()
