@@ -451,6 +451,11 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
             const float hscale = (p.head_scales && valid) ? p.head_scales[it.g * r + hl] : 1.f;
             const bool capped = p.softcap > 0.f, finished = capped || p.slopes || p.head_scales;     // (scores are finished in place)
             const float cap_in = capped ? unit * hscale / (p.softcap * log2e) : 0.f, cap2 = p.softcap * log2e;
+            // which of 32 keys from key0 on the row sees, those from `lo` to `pos`, as bits
+            auto seen = [&](int key0) {
+                const int from = min(max(lo - key0, 0), 32), to = min(max(pos + 1 - key0, 0), 32);
+                return (to > 31 ? 0xffffffffu : (1u << to) - 1u) & (from > 31 ? 0u : 0xffffffffu << from);
+            };
             float ref = -INFINITY, l = 0.f;                              // what the exponentials refer to, their sum
             for (int j = 0; j < it.n_kt && ok; j++) {
                 const uint32_t b = (gs + j) & 1, sc_ph = ((gs + j) >> 1) & 1, s_at = sS + b * 64u;
@@ -467,24 +472,34 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                 const float4 there4 = km_load4(s_at + 32u);
                 const bool full = (__float_as_uint(there4.x) & __float_as_uint(there4.y) & __float_as_uint(there4.z) & __float_as_uint(there4.w)) == 0xffffffffu;
                 const bool open = __all_sync(0xffffffffu, !valid || (key0 + KM_KEYS - 1 <= pos && key0 >= lo)) && full && !finished;
-                const float b0 = slope2 * (float)(key0 - pos), by_head = unit * hscale;
+                const float by_head = unit * hscale;
                 // (loops over the quarters of a tile stay loops: eight warps of these run beside four that convert, and unrolled their
                 // instructions do not stay in the caches: 410 us for the portion named above, 358 so)
                 auto load32 = [&](int q, uint32_t (&raw)[32]) { tmem_ld16(tS + 32 * q, raw); tmem_ld16(tS + 32 * q + 16, raw + 16); };
                 auto k_ref = [&](int q) { return km_load1(s_at + 4u * q); };
                 auto v_log = [&](int q) { return km_load1(s_at + 16u + 4u * q); };
-                // 32 finished scores (options, masks) in the exponent's base 2
-                auto finish = [&](int q, uint32_t (&raw)[32]) {
+                // 32 finished scores (options, masks) in the exponent's base 2.  (What a step does not have costs it nothing: a capped step in which
+                // every row sees every key is as long as its special functions, three a score.)
+                auto finish = [&](int q, uint32_t (&raw)[32], uint32_t sees) {
                     const float in = (capped ? cap_in : by_head) * k_ref(q);
-                    const uint32_t there = __float_as_uint(km_load1(s_at + 32u + 4u * q));
+                    if (capped) {
 #pragma unroll
-                    for (int c = 0; c < 32; c++) {
-                        const int key = key0 + 32 * q + c;
-                        const float bias = fmaf(slope2, (float)(32 * q + c), b0), v = __uint_as_float(raw[c]);
-                        const float x = capped ? fmaf(cap2, tanh_fast(v * in), bias) : fmaf(v, in, bias);
-                        raw[c] = valid && key >= lo && key <= pos && (there >> c & 1u) ? __float_as_uint(x) : 0xff800000u;
+                        for (int c = 0; c < 32; c++) raw[c] = __float_as_uint(cap2 * tanh_fast(__uint_as_float(raw[c]) * in));
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 32; c++) raw[c] = __float_as_uint(__uint_as_float(raw[c]) * in);
+                    }
+                    if (p.slopes) {
+                        const float far = (float)(key0 + 32 * q - pos);
+#pragma unroll
+                        for (int c = 0; c < 32; c++) raw[c] = __float_as_uint(fmaf(slope2, far + (float)c, __uint_as_float(raw[c])));
+                    }
+                    if (__any_sync(0xffffffffu, sees != 0xffffffffu)) {
+#pragma unroll
+                        for (int c = 0; c < 32; c++) raw[c] = sees >> c & 1u ? raw[c] : 0xff800000u;
                     }
                 };
+                auto sees_of = [&](int q) { return valid ? seen(key0 + 32 * q) & __float_as_uint(km_load1(s_at + 32u + 4u * q)) : 0u; };
                 float mx = -INFINITY;
                 uint32_t ra[32], rb[32];
                 if (open) {
@@ -517,16 +532,17 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                         km_wait(ra);
                         float top = -INFINITY;
                         if (p.slopes) {
-                            finish(q, ra);
+                            finish(q, ra, sees_of(q));
 #pragma unroll
                             for (int c = 0; c < 32; c++) top = fmaxf(top, __uint_as_float(ra[c]));
                         } else {
-                            const uint32_t there = __float_as_uint(km_load1(s_at + 32u + 4u * q));
+                            const uint32_t sees = sees_of(q);
+                            if (__all_sync(0xffffffffu, sees == 0xffffffffu)) {
 #pragma unroll
-                            for (int c = 0; c < 32; c++) {
-                                const int key = key0 + 32 * q + c;
-                                const bool see = valid && key >= lo && key <= pos && (there >> c & 1u);
-                                top = fmaxf(top, see ? __uint_as_float(ra[c]) * way : -INFINITY);
+                                for (int c = 0; c < 32; c++) top = fmaxf(top, __uint_as_float(ra[c]) * way);
+                            } else {
+#pragma unroll
+                                for (int c = 0; c < 32; c++) top = fmaxf(top, sees >> c & 1u ? __uint_as_float(ra[c]) * way : -INFINITY);
                             }
                             if (top != -INFINITY) top = capped ? cap2 * tanh_fast(top * way * cap_in * k_ref(q)) : top * way * by_head * k_ref(q);
                         }
@@ -588,7 +604,7 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                         __syncwarp();
                         load32(q, ra);
                         km_wait(ra);
-                        finish(q, ra);
+                        finish(q, ra, sees_of(q));
                         __syncwarp();
                         weights(q, ra, true);
                     }
