@@ -198,7 +198,7 @@ class Engine:
         self._static_meta: Dict[int, torch.Tensor] = {}
         self._meta_ring = []            # [host buffer, device buffer, event of its last copy]
         self._meta_next = 0
-        self._places = None
+        self._places: List[torch.Tensor] = []        # (outgrown ones stay alive: captured graphs may point at them)
         self.steps_run = 0
 
     # ---- requests -----------------------------------------------------------------------------
@@ -231,9 +231,9 @@ class Engine:
 
     def places(self, n: int) -> torch.Tensor:
         """0, 1, ... n - 1 (int32): the slots of rows that lie one behind the other."""
-        if self._places is None or self._places.numel() < n:
-            self._places = torch.arange(max(n, 4096), dtype=torch.int32, device=self.device)
-        return self._places[:n]
+        if not self._places or self._places[-1].numel() < n:
+            self._places.append(torch.arange(max(n, 4096), dtype=torch.int32, device=self.device))
+        return self._places[-1][:n]
 
     def read_cache(self, req: Hashable, entry: int = 0):
         """What a request holds in a schedule entry's cache: ``(first position, keys, values)`` with keys and values [tokens, heads, size]

@@ -227,3 +227,18 @@ def test_latent_and_other_mixers_are_refused(emu, arch):
     model = random_model(config_from_dict(importlib.import_module(arch + "_util").WIDE), seed=3, dtype=torch.float32, device="cpu", std=0.05)
     with pytest.raises(UnsupportedError, match="8 bits"):
         Engine(model, block_size=16, max_tokens=512, max_requests=2, ctx_max=128, kv_dtype="int8")
+
+
+def test_places_stay_where_captured_steps_point(emu):
+    """A step with more tokens than any before asks for more places; graphs made earlier go on reading theirs."""
+    import gc
+    engine = Engine(random_model(config_from_dict(TINY["A"]), seed=3, dtype=torch.float32, device="cpu"), block_size=16, max_tokens=64, kv_dtype="int8")
+    small = engine.places(8)
+    address = small.data_ptr()
+    storage = small.untyped_storage()._cdata
+    large = engine.places(5000)
+    del small
+    gc.collect()
+    assert torch.equal(large, torch.arange(5000, dtype=torch.int32))
+    assert any(p.data_ptr() == address and p.untyped_storage()._cdata == storage for p in engine._places)
+    assert torch.equal(engine.places(3), torch.arange(3, dtype=torch.int32))
