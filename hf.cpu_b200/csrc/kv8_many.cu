@@ -24,7 +24,7 @@
 // * work is cut evenly (as in kv8_few.cu): a step is a tile of keys of one double tile and key/value head, CTA c of C walks steps c N / C to
 //   (c + 1) N / C.  What a CTA has of a double tile that others share goes to scratch, and whoever brings its last piece merges them, in
 //   the order of the keys.  (Whole double tiles a CTA: 228 items of 2,048 tokens and 28 heads are two rounds on 148 SMs where 1.5 would do.)
-// Measured: 2,048 tokens behind 6,144, 28 heads of 128 on 4: 316 us, 666 TFLOP/s, 0.41 of the measured bf16 rate; the bfloat16 cache's kernel
+// Measured: 2,048 tokens behind 6,144, 28 heads of 128 on 4: 312 us, 674 TFLOP/s, 0.41 of the measured bf16 rate; the bfloat16 cache's kernel
 // takes 288 us.  Steps without the conversion take 268: its instructions and the softmax's share the issue slots.
 // Barrier waits are bounded (HFB_ERR_WAIT, TMEM freed; tc_ptx.cuh).
 #include <cuda_fp16.h>
@@ -40,8 +40,9 @@ namespace hfb {
 int *error_word();
 
 constexpr int KM_ROWS = 128, KM_KEYS = 128, KM_THREADS = 416, KM_TMEM_COLS = 512;
-// Fewest steps that are worth a CTA of their own: a piece costs its merge 64 KB or 128 KB of reads by one CTA.  Four requests of 1,024 tokens,
-// 28 heads of 128 on 4: 43, 57, 64 us with 3, 6, 10; one of 8,192: 92, 70, 71, where the kernel of few queries is taken anyway.
+// Fewest steps (a tile's start and end counted) that are worth a CTA of their own: a piece costs its merge 64 KB or 128 KB of reads by one CTA.
+// With 3 | 5 | 8, 28 heads of 128 on 4: 64 tokens of each of four requests of 1,024 tokens 43 | 49 | 57 us, a prompt of 500 41 | 51 | 56; 64 tokens
+// behind 8,192 94 | 80 | 77, but those go to the kernel of few queries.
 constexpr int KM_MIN_STEPS = 3;
 constexpr uint32_t KM_SUB = 128 * 64 * 2;           // one swizzled sub-tile: 128 rows of 64 float16
 

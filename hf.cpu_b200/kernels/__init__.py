@@ -416,11 +416,12 @@ def kv8_head_groups(heads_per_group: int) -> int:
     return next(s for s in range(1, heads_per_group + 1) if heads_per_group <= 16 * s and heads_per_group % s == 0)
 
 
-# A request's portion goes to the prompts' kernel if it has more query rows (tokens times heads on a key/value head) than KV8_MANY and all such
-# portions of the step together more than KV8_MANY_ROWS.  That kernel's cost is the same for 1 to 256 rows a request, the other's grows
-# with every 16.  Measured in us, few | many, by rows a request: 16 requests of 8,192 tokens, 28 heads of 128 on 4, 35 rows 128 | 114, 63 rows 199 | 117; 14
-# heads of 64 on 2, 35 rows 53 | 66, 63 rows 73 | 66; four requests, 28 heads, 63 rows 66 | 76, 112 rows 92 | 78; one request, 252 rows
-# 61 | 104, 896 rows 162 | 90; four of 1,024 tokens, 112 rows 34 | 45, 252 rows 49 | 52.
+# A request's portion goes to the prompts' kernel if it has more query rows (tokens times heads on a key/value head) than KV8_MANY and all
+# such portions of the step together more than KV8_MANY_ROWS.  That kernel's cost is the same for 1 to 256 rows a request, the other's
+# grows with every 16.  Measured in us, few | many, by rows a request, 28 heads of 128 on 4 unless named: 16 requests of 8,192
+# tokens, 21 rows 94 | 109, 35 rows 129 | 109, 63 rows 201 | 111 (14 heads of 64 on 2: 35 rows 51 | 59, 63 rows 72 | 61); one such
+# request, 252 rows 61 | 102, 448 rows 92 | 92, 896 rows 162 | 79; four, 112 rows 92 | 70, 168 rows 127 | 78 (14 heads of 64: 39 | 59,
+# 51 | 61); four of 1,024 tokens, 112 rows 34 | 41, 252 rows 49 | 47.
 KV8_MANY, KV8_MANY_ROWS = 32, 512
 
 
