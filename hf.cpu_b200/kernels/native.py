@@ -448,8 +448,9 @@ class NativeBackend:
                 counters = self._kv8_zeros(dev, stream, capturing, 2 * n * G)
                 self._check(self.lib.hfb_kv8_attention_many(
                     *front, seq.data_ptr(), tiles["many.t0"].data_ptr(), tiles["many.nt"].data_ptr(), n, ctas,
-                    self.kv8_many_tile_cost[softcap > 0], settled, bs, cache.shape[0], window, scale, out_at, ctx.buf("kv8_scratch", (need,), torch.uint8).data_ptr(), need, counters.data_ptr(), counters.shape[0], H, G, d,
-                    *options, stream), "kv8_attention_many")
+                    self.kv8_many_tile_cost[softcap > 0], settled, bs, cache.shape[0], window, scale, out_at,
+                    ctx.buf("kv8_scratch", (need,), torch.uint8).data_ptr(), need, counters.data_ptr(), counters.shape[0], H, G, d, *options, stream),
+                    "kv8_attention_many")
             seq = tiles.get("few.seq")
             if seq is not None:
                 share = 1 if r <= 16 else kv8_head_groups(r)
