@@ -357,6 +357,12 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                 }
                 asm volatile("cp.async.commit_group;" ::: "memory");
             };
+            // ... behind a piece's last step nothing, but a group all the same, for the count: the next piece's first copies go to the same
+            // places, and nothing orders two copies to one place but a wait
+            auto fetch_next = [&](bool any, int page, int skip, uint32_t to) {
+                if (any) fetch(page, skip, to);
+                else asm volatile("cp.async.commit_group;" ::: "memory");
+            };
             auto fetched = [&] { asm volatile("cp.async.wait_group 1;" ::: "memory"); __syncwarp(); };       // (all but the last)
             auto scales_of = [&](int page) {
                 if (page < 0) return make_float2(0.f, 0.f);
@@ -390,13 +396,13 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                 fetched();
                 convert(stK, sK + b * HT, __half2half2(k_hi), __half2half2(k_lo), std::true_type());
                 if (lane == 0) mbar_arrive(k_full + 8 * b);
-                fetch(page, 0, stK);                                      // (of step j + 1)
+                fetch_next(j + 1 < it.n_kt, page, 0, stK);                // (of step j + 1)
                 sc = scales_of(page);
                 if (!mbar_wait(v_empty + 8 * b, ph ^ 1, abort_flag, err)) { ok = false; break; }
                 fetched();
                 convert(stV, sV + b * HT, __half2half2(v_hi), __half2half2(v_hi), std::false_type());
                 if (lane == 0) mbar_arrive(v_full + 8 * b);
-                fetch(page, bs * D, stV);
+                fetch_next(j + 1 < it.n_kt, page, bs * D, stV);
                 there = page >= 0;
                 page = page_of(j + 2);
             }

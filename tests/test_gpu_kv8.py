@@ -577,3 +577,21 @@ def test_alike_layers_made_again_give_the_same_bits(heads, monkeypatch):
     assert torch.equal(got[0], got[1]) and torch.isfinite(got[0]).all()
     assert len(made) >= 10 and all(made)
     K.check_device_errors()
+
+
+# ---- the prompts' kernel: what stands between a CTA's pieces -----------------------------------------------------------------
+
+@pytest.mark.parametrize("shape", [(32, 8, 64, 16), (28, 4, 128, 8)], ids=str)
+def test_many_short_pieces_a_cta(shape):
+    """Portions of one or two steps each, many more than there are CTAs: a CTA's places for codes go from one piece to the next without a
+    pause, and a piece's last copies must not land on the next one's first."""
+    H, G, d, bs = shape
+    s = step([33 + i % 5 for i in range(60)], [33 + i % 5 + 100 * (i % 3) for i in range(60)], bs, G, d, seed=d)
+    assert set(n.split(".")[0] for n in native().kv8_step_arrays(s.q_lens, H // G)) == {"many"}
+    cache = pack(s.k, s.ks, s.v, s.vs)
+    q = torch.randn(s.T, H * d, generator=s.g, device=DEV).bfloat16()
+    got = attend(s, q, cache, H)
+    check(s, q, cache, got, H)
+    for _ in range(5):
+        assert torch.equal(got, attend(s, q, cache, H))
+    native().check_device_errors()
