@@ -379,7 +379,7 @@ kv8_few_kernel(Kv8FewParams f, int *err)
             const int skip = (js ^ group) & 1;
             for (int j = skip; j < len; j += 2) {
                 const int kt = kt_first + j, s = (js + j) % STAGES;
-                ok = mbar_wait(full0 + 8 * s, ((js + j) / STAGES) & 1, abort_flag, err) && ok;
+                ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, ((js + j) / STAGES) & 1, abort_flag, err)) && ok;   // (lanes go on together)
                 if (!ok) continue;
                 const uint32_t st = tiles0 + s * stage_bytes, sv = st + v_codes;
                 const uint8_t *sg = gen + (tiles0 - base) + s * stage_bytes;

@@ -126,6 +126,14 @@ __device__ __forceinline__ void km_wait(uint32_t (&v)[32])
 #undef KM_REGS
 }
 
+// A wait of a whole warp: its lanes look for the phase one by one, and go on together.  Lane 0's release behind it may begin the phase
+// after next, in which a lane that still looked would never find the one it looks for; and where a wait runs out for one lane no
+// other may go on to what the warp does as one.
+__device__ __forceinline__ bool km_wait_warp(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *err)
+{
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err));
+}
+
 template <int D>
 __global__ void __launch_bounds__(KM_THREADS, 1)
 kv8_many_kernel(Kv8ManyParams f, int *err)
@@ -385,20 +393,20 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                 const __half k_hi = __float2half_rn(ks), k_lo = __float2half_rn(ks - __half2float(k_hi));
                 const __half v_hi = __float2half_rn(number ? sc.y * __uint_as_float((254u - vf) << 23) : 0.f);
                 const uint32_t present = __ballot_sync(0xffffffffu, there);
-                ok = mbar_wait(sc_empty + 8 * b, ph ^ 1, abort_flag, err);
+                ok = km_wait_warp(sc_empty + 8 * b, ph ^ 1, abort_flag, err);
                 if (!ok) break;
                 if (lane == 0) {
                     asm volatile("st.shared.f32 [%0], %1;\n\tst.shared.f32 [%0 + 16], %2;\n\tst.shared.u32 [%0 + 32], %3;"
                                  ::"r"(at), "f"(__uint_as_float(kf << 23)), "f"((float)vf - 127.f), "r"(present) : "memory");
                     mbar_arrive(sc_full + 8 * b);
                 }
-                if (!mbar_wait(k_empty + 8 * b, ph ^ 1, abort_flag, err)) { ok = false; break; }
+                if (!km_wait_warp(k_empty + 8 * b, ph ^ 1, abort_flag, err)) { ok = false; break; }
                 fetched();
                 convert(stK, sK + b * HT, __half2half2(k_hi), __half2half2(k_lo), std::true_type());
                 if (lane == 0) mbar_arrive(k_full + 8 * b);
                 fetch_next(j + 1 < it.n_kt, page, 0, stK);                // (of step j + 1)
                 sc = scales_of(page);
-                if (!mbar_wait(v_empty + 8 * b, ph ^ 1, abort_flag, err)) { ok = false; break; }
+                if (!km_wait_warp(v_empty + 8 * b, ph ^ 1, abort_flag, err)) { ok = false; break; }
                 fetched();
                 convert(stV, sV + b * HT, __half2half2(v_hi), __half2half2(v_hi), std::false_type());
                 if (lane == 0) mbar_arrive(v_full + 8 * b);
@@ -466,14 +474,14 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
             float ref = -INFINITY, l = 0.f;                              // what the exponentials refer to, their sum
             for (int j = 0; j < it.n_kt && ok; j++) {
                 const uint32_t b = (gs + j) & 1, sc_ph = ((gs + j) >> 1) & 1, s_at = sS + b * 64u;
-                if (!mbar_wait(sc_full + 8 * b, sc_ph, abort_flag, err)) { ok = false; break; }
+                if (!km_wait_warp(sc_full + 8 * b, sc_ph, abort_flag, err)) { ok = false; break; }
                 if (j >= n_mine) {                                       // (the other query tile's step)
                     if (lane == 0) mbar_arrive(sc_empty + 8 * b);
                     continue;
                 }
                 const uint32_t ph = (g_mine + j) & 1;                    // (O holds everything up to the step before once these scores are there)
                 const int key0 = (it.kt_lo + j) * KM_KEYS;
-                if (!mbar_wait(s_full + 8 * i, ph, abort_flag, err)) { ok = false; break; }
+                if (!km_wait_warp(s_full + 8 * i, ph, abort_flag, err)) { ok = false; break; }
                 tc_fence_after();
                 // a step without options in which every row sees every key, as most are (rows beyond the tile's tokens go with those)
                 const float4 there4 = km_load4(s_at + 32u);
@@ -626,7 +634,7 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
             }
             gs += it.n_kt;
             g_mine += n_mine;
-            if (ok && n_mine > 0) ok = mbar_wait(pv_done + 8 * i, (g_mine - 1) & 1, abort_flag, err);
+            if (ok && n_mine > 0) ok = km_wait_warp(pv_done + 8 * i, (g_mine - 1) & 1, abort_flag, err);
             {
                 // (a wait that ran out ends the walk of the query tile's warps together: none may be left at a barrier)
                 int all;

@@ -595,3 +595,16 @@ def test_many_short_pieces_a_cta(shape):
     for _ in range(5):
         assert torch.equal(got, attend(s, q, cache, H))
     native().check_device_errors()
+
+
+def test_second_query_tile_without_tokens():
+    """Portions that the first query tile holds alone: the second one's warps walk through hundreds of steps that are not theirs."""
+    for d in (64, 128):
+        s = step([20] * 6, [20, 5000, 900, 3000, 64, 2000], 16, 2, d, seed=d + 1)
+        assert set(n.split(".")[0] for n in native().kv8_step_arrays(s.q_lens, 4)) == {"many"}
+        cache = pack(s.k, s.ks, s.v, s.vs)
+        q = torch.randn(s.T, 8 * d, generator=s.g, device=DEV).bfloat16()
+        got = attend(s, q, cache, 8)
+        check(s, q, cache, got, 8)
+        assert torch.equal(got, attend(s, q, cache, 8))
+        native().check_device_errors()
