@@ -350,6 +350,7 @@ def _kv8_records(cache, block_size, G, d, what) -> None:
 
 _KV8_RECORDS = {}
 _KV8_TYPES = (torch.float32, torch.bfloat16)
+_KV8_TILES = tuple(tuple(f"{kind}.{part}" for part in ("seq", "t0", "nt")) for kind in ("few", "many"))
 
 
 def _kv8_rows(x, T, n, dtype, what) -> None:
@@ -463,6 +464,13 @@ def paged_attention_kv8(q, cache, meta, ctx, H, G, d, window, scale, out, tiles=
     _kv8_records(cache, meta.block_size, G, d, "paged_attention_kv8")
     _kv8_index(ctx.positions, T, "paged_attention_kv8: positions")
     _kv8_index(ctx.token_seq, T, "paged_attention_kv8: the tokens' requests")
+    for name in _KV8_TILES if tiles else ():
+        seq, t0, nt = (tiles.get(n) for n in name)
+        if seq is t0 is nt is None:
+            continue
+        if not (seq is not None and t0 is not None and nt is not None and seq.dtype is t0.dtype is nt.dtype is torch.int32 and seq.dim() == t0.dim() == nt.dim() == 1
+                and seq.numel() == t0.numel() == nt.numel() and seq.device == t0.device == nt.device == q.device):
+            raise ValueError("paged_attention_kv8: tile lists %s, %s, %s must be int32, of one length, on the queries' device" % name)
     if table.dtype != torch.int32 or table.dim() != 2 or table.shape[1] != meta.max_blocks:
         raise ValueError("paged_attention_kv8: the block table must be int32 [requests, max_blocks]")
     options = ()

@@ -433,7 +433,7 @@ class NativeBackend:
     def paged_attention_kv8(self, q, cache, meta, ctx, H, G, d, window, scale, out, tiles, settled=False, sinks=None, zero_sink=False,
                             slopes=None, head_scales=None, softcap=0.0):
         table, positions, bs = meta.block_table, ctx.positions, meta.block_size
-        dev = self._here((q, cache, table, ctx.token_seq, positions, out, sinks, slopes, head_scales))
+        dev = self._here((q, cache, table, ctx.token_seq, positions, out, sinks, slopes, head_scales, *tiles.values()))
         at = lambda t: 0 if t is None else t.data_ptr()
         options = (at(sinks), 1 if zero_sink else 0, at(slopes), at(head_scales), softcap)
         q_at, out_at, kept = q.data_ptr(), out.data_ptr(), _p(cache)

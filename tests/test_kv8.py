@@ -242,3 +242,19 @@ def test_places_stay_where_captured_steps_point(emu):
     assert torch.equal(large, torch.arange(5000, dtype=torch.int32))
     assert any(p.data_ptr() == address and p.untyped_storage()._cdata == storage for p in engine._places)
     assert torch.equal(engine.places(3), torch.arange(3, dtype=torch.int32))
+
+
+def test_tile_lists_are_looked_at(emu):
+    """Lists of another type, of different lengths or of another device are refused, and a kind of tile without one of its lists."""
+    q, i4 = torch.zeros(4, 128), torch.zeros(4, dtype=torch.int32)
+    meta = SimpleNamespace(block_table=torch.zeros(1, 2, dtype=torch.int32), block_size=8, max_blocks=2)
+    ctx = SimpleNamespace(positions=i4, token_seq=i4, max_q_len=4, max_kv_len=4)
+    args = dict(q=q, cache=kernels.kv8_cache(3, 8, 2, 32, "cpu"), meta=meta, ctx=ctx, H=4, G=2, d=32, window=0, scale=1.0, out=torch.zeros_like(q))
+    for kind in ("few", "many"):
+        good = {f"{kind}.{n}": torch.ones(2, dtype=torch.int32) for n in ("seq", "t0", "nt")}
+        kernels.paged_attention_kv8(**args, tiles=good)
+        for n in good:
+            for bad in (good[n].long(), good[n].float(), good[n][:1], good[n][None], good[n].to("meta"), None):
+                with pytest.raises(ValueError):
+                    kernels.paged_attention_kv8(**args, tiles={**good, n: bad})
+    kernels.paged_attention_kv8(**args, tiles={})
