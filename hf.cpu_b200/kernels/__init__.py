@@ -453,8 +453,8 @@ def paged_attention_kv8(q, cache, meta, ctx, H, G, d, window, scale, out, tiles=
                         slopes=None, head_scales=None, softcap: float = 0.0) -> None:
     """:func:`paged_attention` over a cache in 8 bits, with its masks and options.  ``q`` and ``out`` [T, H * d] are float32 or bfloat16;
     ``tiles``: the device arrays of :func:`kv8_step_arrays` for this step (without them only the plain kernel runs).  ``settled``: all
-    rows before the step's own positions were written before the kernel in front of this one was launched, so that they may be
-    fetched while it still runs."""
+    rows before the step's own positions, and the index arrays, were written before the kernel in front of this one was launched, so that
+    they may be read while it still runs.  Calls, captured ones too, to which ``ctx.buf`` gives the same scratch must follow one another."""
     T = q.shape[0]
     if q.dtype not in _KV8_TYPES or q.dim() != 2 or q.shape[1] != H * d or out.shape != q.shape or out.dtype != q.dtype:
         raise ValueError("paged_attention_kv8: queries and output must be [T, H * d], both float32 or bfloat16")

@@ -445,12 +445,12 @@ class NativeBackend:
             if seq is not None:
                 n, ctas = seq.shape[0], self.sm_count
                 need = self._kv8_scratch(True, ctas, d)
-                counters = self._kv8_zeros(dev, stream, capturing, 2 * n * G)
+                scratch = ctx.buf("kv8_scratch", (need,), torch.uint8).data_ptr()
+                counters = self._kv8_zeros(dev, scratch, capturing, 2 * n * G)
                 self._check(self.lib.hfb_kv8_attention_many(
                     *front, seq.data_ptr(), tiles["many.t0"].data_ptr(), tiles["many.nt"].data_ptr(), n, ctas,
                     self.kv8_many_tile_cost[softcap > 0], settled, bs, cache.shape[0], window, scale, out_at,
-                    ctx.buf("kv8_scratch", (need,), torch.uint8).data_ptr(), need, counters.data_ptr(), counters.shape[0], H, G, d, *options, stream),
-                    "kv8_attention_many")
+                    scratch, need, counters.data_ptr(), counters.shape[0], H, G, d, *options, stream), "kv8_attention_many")
             seq = tiles.get("few.seq")
             if seq is not None:
                 share = 1 if r <= 16 else kv8_head_groups(r)
@@ -460,7 +460,7 @@ class NativeBackend:
                 scratch = ctx.buf("kv8_scratch", (need,), torch.uint8).data_ptr()
                 for i in range(0, seq.shape[0], self._kv8_few_tiles):
                     n = min(self._kv8_few_tiles, seq.shape[0] - i)
-                    counters = self._kv8_zeros(dev, stream, capturing, n * G * share)
+                    counters = self._kv8_zeros(dev, scratch, capturing, n * G * share)
                     self._check(self.lib.hfb_kv8_attention_few(
                         *front, seq.data_ptr() + 4 * i, tiles["few.t0"].data_ptr() + 4 * i, tiles["few.nt"].data_ptr() + 4 * i, n, tile_tokens, ctas,
                         self.kv8_min_steps, self.kv8_tile_cost, settled, bs, cache.shape[0], window, scale, out_at, scratch, need, counters.data_ptr(),
@@ -478,22 +478,17 @@ class NativeBackend:
             need = self._kv8_needs[many, ctas, d] = ask(c_int(ctas), c_int(d))
         return need
 
-    def _kv8_zeros(self, dev, stream, capturing, n):
-        """``n`` counters that are zero and that no launch uses which may run beside the one they are for: one set a stream, and for
-        a launch that is being captured a set of its own, since its graph may be replayed beside anything."""
-        if capturing:
-            pool = self._kv8_counters.get(dev)
-            if pool is None or pool[1] + n > pool[0].numel():
+    def _kv8_zeros(self, dev, scratch, capturing, n):
+        """``n`` counters that are zero, for a launch that merges through the scratch at this address.  Launches with the same scratch
+        follow one another, eager and captured ones alike, and each leaves its counters zero: so they have the same counters too."""
+        held = self._kv8_counters.get((dev, scratch))
+        if held is None or held[-1].shape[0] < n:
+            if capturing:
                 return torch.zeros(n, dtype=torch.int32, device=dev)              # (a part of the graph then)
-            pool[1] += n
-            return pool[0][pool[1] - n:pool[1]]
-        have = self._kv8_counters.get((dev, stream))
-        if have is None or have.shape[0] < n:
-            if dev not in self._kv8_counters:
-                self._kv8_counters[dev] = [torch.zeros(1 << 20, dtype=torch.int32, device=dev), 0]
-                torch.cuda.current_stream().synchronize()                         # (other streams' captures take from it)
-            have = self._kv8_counters[dev, stream] = torch.zeros(max(n, 4096), dtype=torch.int32, device=dev)
-        return have
+            # (outgrown ones stay: captured launches may point at them)
+            held = self._kv8_counters.setdefault((dev, scratch), [])
+            held.append(torch.zeros(max(2 * n, 4096), dtype=torch.int32, device=dev))
+        return held[-1]
 
     def swiglu(self, gu, out, interleaved):
         self._on_gpu(gu, out)

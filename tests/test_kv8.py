@@ -258,3 +258,20 @@ def test_tile_lists_are_looked_at(emu):
                 with pytest.raises(ValueError):
                     kernels.paged_attention_kv8(**args, tiles={**good, n: bad})
     kernels.paged_attention_kv8(**args, tiles={})
+
+
+def test_captured_launches_share_counters_with_their_scratch():
+    """However many steps are captured, none of their launches comes to counters of its own (zeroed by a node of the graph), and
+    outgrown counters stay where captured launches point."""
+    from hfcpu_b200.kernels import native
+    b = native.NativeBackend.__new__(native.NativeBackend)
+    b._kv8_counters = {}
+    first = b._kv8_zeros("cpu", 1000, False, 256)
+    assert first.numel() >= 256 and not first.any()
+    at = first.data_ptr()
+    assert all(b._kv8_zeros("cpu", 1000, capturing, 256).data_ptr() == at for capturing in (True, False) for _ in range(8192))
+    # other scratch, which may be in use at the same time: other counters; and more counters than there were
+    other, more = b._kv8_zeros("cpu", 2000, False, 256), b._kv8_zeros("cpu", 1000, False, 100000)
+    assert len({at, other.data_ptr(), more.data_ptr()}) == 3 and more.numel() >= 100000 and not more.any()
+    assert any(c is first for c in b._kv8_counters["cpu", 1000])
+    assert b._kv8_zeros("cpu", 3000, True, 8).numel() == 8 and ("cpu", 3000) not in b._kv8_counters
