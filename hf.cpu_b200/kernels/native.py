@@ -490,6 +490,18 @@ class NativeBackend:
             held.append(torch.zeros(max(2 * n, 4096), dtype=torch.int32, device=dev))
         return held[-1]
 
+    def _kv8_clear(self):
+        """All counters to zero again: a launch that gave up on a wait may have left any of them behind, and whatever stream or graph
+        uses them next would take a tile for finished before its pieces are there."""
+        held = [c for of_scratch in self._kv8_counters.values() for c in of_scratch]
+        devices = {c.device for c in held}
+        for d in devices:
+            torch.cuda.synchronize(d)                     # (launches on any stream have ended)
+        for c in held:
+            c.zero_()
+        for d in devices:
+            torch.cuda.synchronize(d)                     # (... and none begins before)
+
     def swiglu(self, gu, out, interleaved):
         self._on_gpu(gu, out)
         T, F = out.shape
@@ -1026,6 +1038,8 @@ class NativeBackend:
         self._check(self.lib.hfb_error_word_take(ctypes.byref(w), self._stream()), "error word")
         if w.value and self._counters is not None:
             self._counters.zero_()             # a kernel that gave up may have left tile counts behind
+        if w.value:
+            self._kv8_clear()
         return w.value
 
 

@@ -608,3 +608,44 @@ def test_second_query_tile_without_tokens():
         check(s, q, cache, got, 8)
         assert torch.equal(got, attend(s, q, cache, 8))
         native().check_device_errors()
+
+
+def test_attention_is_right_again_behind_a_launch_that_gave_up(monkeypatch):
+    """Counts that a launch left behind (put there from the host) are gone once its error has been taken: eager and captured launches."""
+    import ctypes
+    K = native()
+    b = K.backend()
+    s = step([1, 90, 1], [3000, 2000, 1500], 16, 2, 64, seed=12)
+    cache = pack(s.k, s.ks, s.v, s.vs)
+    q, buf = torch.randn(s.T, 8 * 64, generator=s.g, device=DEV).bfloat16(), context()
+    plan = {n: torch.from_numpy(a).to(DEV) for n, a in K.kv8_step_arrays(s.q_lens, 4).items()}
+    assert len(plan) == 6
+    right, out = attend(s, q, cache, 8, buf=buf, plan=plan), torch.zeros_like(q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        attend(s, q, cache, 8, buf=buf, plan=plan, out=out)
+    for c in (c for of_scratch in b._kv8_counters.values() for c in of_scratch):
+        c.fill_(1)
+    torch.cuda.synchronize()
+    take = b.lib.hfb_error_word_take
+
+    class Lib:
+        def __getattr__(self, name):
+            return getattr(lib, name)
+
+        @staticmethod
+        def hfb_error_word_take(at, stream):
+            rc = take(at, stream)
+            ctypes.cast(at, ctypes.POINTER(ctypes.c_int32))[0] = 4
+            return rc
+    lib = b.lib
+    b.lib = Lib()
+    try:
+        with pytest.raises(K.DeviceFault):
+            K.check_device_errors()
+    finally:
+        b.lib = lib
+    graph.replay()
+    assert torch.equal(out, right) and torch.equal(attend(s, q, cache, 8, buf=buf, plan=plan), right)
+    check(s, q, cache, right, 8)
+    K.check_device_errors()

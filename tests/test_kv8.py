@@ -275,3 +275,27 @@ def test_captured_launches_share_counters_with_their_scratch():
     assert len({at, other.data_ptr(), more.data_ptr()}) == 3 and more.numel() >= 100000 and not more.any()
     assert any(c is first for c in b._kv8_counters["cpu", 1000])
     assert b._kv8_zeros("cpu", 3000, True, 8).numel() == 8 and ("cpu", 3000) not in b._kv8_counters
+
+
+def test_counters_are_cleared_behind_a_launch_that_gave_up(monkeypatch):
+    """A nonzero error word clears whatever counters there are, not the other kernels' alone."""
+    import ctypes
+    from hfcpu_b200.kernels import native
+    b = native.NativeBackend.__new__(native.NativeBackend)
+    word = [0]
+
+    class Lib:
+        @staticmethod
+        def hfb_error_word_take(at, stream):
+            ctypes.cast(at, ctypes.POINTER(ctypes.c_int32))[0] = word[0]
+            return 0
+    b.lib, b._counters, b.launches = Lib, torch.ones(4, dtype=torch.int32), 0
+    b._stream = lambda: None
+    synced = []
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda d=None: synced.append(d))
+    held = [torch.ones(n, dtype=torch.int32) for n in (8, 5, 3)]
+    b._kv8_counters = {(0, 17): held[:2], (0, 18): held[2:]}
+    assert b.error_word() == 0 and all(bool(x.all()) for x in held)
+    word[0] = 8
+    assert b.error_word() == 8 and not any(bool(x.any()) for x in held) and not b._counters.any()
+    assert synced
