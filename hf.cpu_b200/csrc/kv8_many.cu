@@ -219,7 +219,7 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
 
     // A piece: steps off .. off + n_kt of one double tile and head; n_kt0, n_kt1: how many of them the two query tiles take part in.
     // Every role walks the same ones.
-    struct Item { int g, seq, t0, nt0, nt1, pos_last, lo_first, kt_lo, n_kt0, n_kt1, n_kt, tile, all; long long first; bool begins; };
+    struct Item { int g, seq, t0, nt0, nt1, pos_last, lo_first, kt_lo, n_kt0, n_kt1, n_kt, tile, all; long long first; };
     struct Walk { long long x; int tile, before; };
     auto item_of = [&](Walk &w, Item &it) -> bool {
         for (;;) {
@@ -235,7 +235,7 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
             const int off = (int)(begin - it.first);
             it.n_kt = (int)max(0ll, w.x - begin);
             if (it.n_kt == 0) continue;
-            it.tile = w.tile; it.all = tl.n_kt; it.begins = off == 0;
+            it.tile = w.tile; it.all = tl.n_kt;
             it.seq = tl.seq; it.t0 = tl.t0; it.pos_last = tl.pos_last; it.lo_first = tl.lo_first; it.kt_lo = tl.kt_lo + off;
             it.nt0 = min(tl.nt, f.per); it.nt1 = tl.nt - it.nt0;         // tokens of the two query tiles
             it.n_kt0 = max(0, min(it.n_kt, tl.n_kt0 - off));
@@ -644,17 +644,21 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
             }
             if (!ok || nt_mine <= 0) continue;
             tc_fence_after();
-            if (it.begins && (p.sinks || p.zero_sink)) {
-                // the sink: one more term of the sum, in the scale of the row's reference
-                const float sk = p.sinks ? (valid ? p.sinks[it.g * r + hl] : 0.f) * log2e : 0.f;
-                if (ref == -INFINITY && l == 0.f) ref = sk;
-                l += exp2f(sk - (ref == -INFINITY ? 0.f : ref));
-            }
+            // the sink is one more term of the whole sum, and joins it where that is made: what one piece's exponentials refer to may lie hundreds
+            // below it (with slopes a tile's oldest keys do), out of float32's range
+            const bool sink = p.sinks || p.zero_sink;
+            const float sk = p.sinks && valid ? p.sinks[it.g * r + hl] * log2e : 0.f;
             // the pieces of this double tile and head: of CTAs c_first .. c_first + pieces - 1, each its first but for the first one's last
             const int c_first = (int)(((it.first + 1) * ctas - 1) / total), pieces = (int)(((it.first + it.all) * ctas - 1) / total) - c_first + 1;
             uint4 *dst = (uint4 *)((__nv_bfloat16 *)p.out + th);
             if (pieces == 1) {
-                const float inv = l == 0.f ? 0.f : 1.0f / l;
+                float scaled = 1.f;                                      // what the outputs and their sum are brought down by for the sink
+                if (sink) {
+                    const float top = fmaxf(ref, sk);
+                    scaled = exp2f(ref - top);
+                    l = fmaf(l, scaled, exp2f(sk - top));
+                }
+                const float inv = l == 0.f ? 0.f : scaled / l;
 #pragma unroll 1
                 for (int c = 0; c < D / 16; c += 4) {                    // four reads of 16 columns under way together
                     uint32_t ov[64];
@@ -708,8 +712,9 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
             asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
             if (!*(volatile int *)flag || !valid) continue;              // (the flag is written again behind two barriers)
             __threadfence();
-            float top = -INFINITY, sum = 0.f;
+            float top = sink ? sk : -INFINITY, sum = 0.f;
             for (int c = 0; c < pieces; c++) top = fmaxf(top, __ldcg((const float2 *)f.part_ml + place_of(c_first + c) * 128 + row).x);
+            if (sink) sum = exp2f(sk - top);
             for (int c = 0; c < pieces; c++) {
                 const float2 ml = __ldcg((const float2 *)f.part_ml + place_of(c_first + c) * 128 + row);
                 sum += ml.y * (ml.x == -INFINITY ? 1.f : exp2f(ml.x - top));           // (zero, or no number)

@@ -649,3 +649,27 @@ def test_attention_is_right_again_behind_a_launch_that_gave_up(monkeypatch):
     assert torch.equal(out, right) and torch.equal(attend(s, q, cache, 8, buf=buf, plan=plan), right)
     check(s, q, cache, right, 8)
     K.check_device_errors()
+
+
+@pytest.mark.parametrize("sink", ["learned", "zero"])
+@pytest.mark.parametrize("slope", [0.0, 0.01, 0.02, 0.05, 0.2])
+@pytest.mark.parametrize("shape", [(14, 2, 64, 16), (28, 4, 128, 16)], ids=str)
+def test_sinks_beside_keys_far_below_them(shape, slope, sink):
+    """Thousands of keys, many pieces a tile: with a bias linear in the distance the oldest keys' scores lie hundreds or thousands below the
+    sink, and without one a sink may stand far above (or below) every score."""
+    H, G, d, bs = shape
+    K = native()
+    s = step([40, 300, 96], [8040, 8300, 700], bs, G, d, seed=H)
+    assert set(n.split(".")[0] for n in K.kv8_step_arrays(s.q_lens, H // G)) == {"many"}
+    cache = pack(s.k, s.ks, s.v, s.vs)
+    q = (torch.randn(s.T, H * d, generator=s.g, device=DEV) * 2).bfloat16()
+    o = dict(zero_sink=True) if sink == "zero" else dict(sinks=torch.randn(H, device=DEV, generator=gen(2)))
+    if slope:
+        o["slopes"] = torch.full((H,), slope, device=DEV) * torch.linspace(0.5, 1, H, device=DEV)
+    for far in (0.0, 120.0, -120.0) if sink == "learned" else (0.0,):
+        if sink == "learned":
+            o["sinks"] = torch.randn(H, device=DEV, generator=gen(2)) + far
+        got = attend(s, q, cache, H, **o)
+        assert torch.isfinite(got).all()
+        check(s, q, cache, got, H, **o)
+    K.check_device_errors()
