@@ -9,6 +9,10 @@
 //   a sum of two float16) or, with its scale, twice (values); half a step is 2^-11 of the number, an eighth of what bfloat16 keys and
 //   values lose.  (Scales applied to scores and weights in float32 by the softmax's threads: two reads of shared memory and
 //   two multiplications for every four scores, 3 % of the time.)
+// * 32 keys whose scales lie further apart than 2^11, and values beyond 2^45 or 2^-45, have a power of two each.  A row's weights then go by the
+//   largest score and reference among the keys that it sees, its sum by the scores alone, an exponential each: what a row does not see, or
+//   gives no weight, takes no bits from what it does.  Steps of such keys take several times as long (km_apart); all others pay 2 % of the
+//   time for looking (309 and 315 us for the portion below).
 // * each of these warps asks for its keys' codes of the next tile as soon as it has converted the last ones, and both operands have two
 //   places, so that the conversion runs a tile ahead of the products.
 // * a row whose key or value is no number makes its scores so and leaves its values zero: a weight of zero stays zero in the sums of the
@@ -16,7 +20,7 @@
 // * queries are multiplied by the power of two that brings a row's largest number to 2^14..2^15 (kv8_few.cu).
 // * a row's exponentials refer to R = (largest score + log2 of its value reference) - 10: a weight 2^(s - R) reference is at most 2^14
 //   before R is raised, and is rounded once to float16.  Both sums carry the factor, which cancels.  R is raised, and the sums so far
-//   rescaled (the output in TMEM), only when it has been outgrown by 2^4.  (Values below 2^-90 are zeros.)
+//   rescaled (the output in TMEM), only when it has been outgrown by 2^4.
 // * a row belongs to one thread, which reads its scores from TMEM twice, 32 at a time, for the maximum and for the weights.  The weights
 //   go back to TMEM in the scores' place, as the second product's left operand; O lives in TMEM too.  One query tile's softmax runs
 //   beside the other's products: its own next scores follow its outputs in the tensor core's order, which is all that keeps them off
@@ -49,11 +53,11 @@ constexpr uint32_t KM_SUB = 128 * 64 * 2;           // one swizzled sub-tile: 12
 struct Kv8ManyParams {
     Kv8Params a;
     int per, n_tiles, tile_cost, settled;            // tokens per query tile, double tiles in all, steps that a tile's start and end are reckoned as
-    float *part_o, *part_ml;                         // pieces of double tiles: [CTAs, 2, 2, D / 4, 128, 4] and [CTAs, 2, 2, 128, 2]
+    float *part_o, *part_ml;                         // pieces of double tiles: [CTAs, 2, 2, D / 4, 128, 4] and [CTAs, 2, 2, 128, 4]
     int *counters;                                   // ... one per (double tile, head, query tile), zero between launches
 };
 
-template <int D> constexpr uint32_t km_smem() { return 6 * (D / 64) * KM_SUB + 2 * KM_KEYS * D + 128 + 256; }
+template <int D> constexpr uint32_t km_smem() { return 6 * (D / 64) * KM_SUB + 2 * KM_KEYS * D + 128 + 256 + 4 * KM_KEYS; }
 
 __device__ __forceinline__ uint32_t km_off(int row, int c16)
 {
@@ -126,6 +130,58 @@ __device__ __forceinline__ void km_wait(uint32_t (&v)[32])
 #undef KM_REGS
 }
 
+// Exponent field of the power of two above a scale; of none (zero), that of one.
+__device__ __forceinline__ uint32_t km_above(float scale) { return scale > 0.f ? min((__float_as_uint(scale) >> 23) + 1u, 253u) : 127u; }
+// 32 keys share their references unless one of their scales is below the largest one's by more than a factor of 2^KM_APART: up to there
+// no number code * scale, down to the code 1, leaves float16's normal range, and a key's second float16 is good to 2^-13.
+// ... and unless the values' reference is beyond 2^KM_RANGE or its inverse: within, a score's exponential relative to the largest weight, whatever
+// the quarters of a row's keys are scaled by, stays in float32 as long as it counts (down to 2^-46 of the largest).
+constexpr uint32_t KM_APART = 11, KM_RANGE = 45;
+
+// The steps whose keys have references of their own, one for all of the row's 128 scores: the largest score, and the largest with its value's
+// reference; or (WEIGHTS) the weights into their place, and the sum of the exponentials, each relative to the largest so far.  For what
+// models don't do: it may be slow, and stays out of the way of the other steps' registers and instructions.
+struct KmRow {
+    uint32_t tmem, exponents, present;               // where the scores, the keys' exponents and the bits of the keys there are (0: no row) lie
+    float by, cap, slope;
+    int key0, pos, lo;
+};
+template <bool WEIGHTS> __device__ __noinline__ float2 km_apart(KmRow r, float minus, float l_minus)
+{
+    float2 out = WEIGHTS ? make_float2(0.f, 0.f) : make_float2(-INFINITY, -INFINITY);
+#pragma unroll 1
+    for (int n = 0; n < 16; n++) {                   // eight scores a time
+        uint32_t raw[8], ex[4], pk[4], there;
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(ex[0]), "=r"(ex[1]), "=r"(ex[2]), "=r"(ex[3]) : "r"(r.exponents + 16u * n));
+        there = r.present ? (__float_as_uint(km_load1(r.present + 4u * (n >> 2))) | __float_as_uint(km_load1(r.present + 16u + 4u * (n >> 2)))) >> (8 * (n & 3)) : 0u;
+        __syncwarp();
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=r"(raw[0]), "=r"(raw[1]), "=r"(raw[2]), "=r"(raw[3]), "=r"(raw[4]), "=r"(raw[5]), "=r"(raw[6]), "=r"(raw[7]) : "r"(r.tmem + 8 * n));
+        tmem_wait_ld();
+        float before = 0.f;
+#pragma unroll
+        for (int c = 0; c < 8; c++) {
+            const int key = r.key0 + 8 * n + c;
+            const uint32_t e = ex[c >> 1] >> (16 * (c & 1));
+            float x = __uint_as_float(raw[c]) * r.by * __uint_as_float((e & 255u) << 23);
+            const float log = (float)(e >> 8 & 255u) - 127.f;
+            if (r.cap > 0.f) x = r.cap * tanh_fast(x);
+            x = fmaf(r.slope, (float)(key - r.pos), x);
+            if (!(there >> c & 1u) || key < r.lo || key > r.pos) x = -INFINITY;
+            if (!WEIGHTS) { out.x = fmaxf(out.x, x); out.y = fmaxf(out.y, x + log); continue; }
+            const float w = km_ex2(x + (log + minus));
+            out.x += km_ex2(x + l_minus);
+            if (c & 1) pk[c / 2] = km_pack(before, w);
+            before = w;
+        }
+        if (WEIGHTS) {
+            __syncwarp();
+            asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(r.tmem + 4 * n), "r"(pk[0]), "r"(pk[1]), "r"(pk[2]), "r"(pk[3]) : "memory");
+        }
+    }
+    return out;
+}
+
 // A wait of a whole warp: its lanes look for the phase one by one, and go on together.  Lane 0's release behind it may begin the phase
 // after next, in which a lane that still looked would never find the one it looks for; and where a wait runs out for one lane no
 // other may go on to what the warp does as one.
@@ -145,8 +201,9 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
     constexpr uint32_t HT = (D / 64) * KM_SUB;       // a [128 x D] float16 operand: Q, K or V
     const uint32_t sQ = base, sK = base + 2 * HT, sV = base + 4 * HT;         // (keys and values: two each)
     const uint32_t stK = base + 6 * HT, stV = stK + KM_KEYS * D;         // codes of the next keys and values
-    const uint32_t sS = stV + KM_KEYS * D;           // [2][16]: per quarter of a tile the keys' reference, log2 of the values', the keys there are
-    const uint32_t bars = sS + 128;
+    // [2][16]: per quarter of a tile the keys' reference, log2 of the values', the keys there are, or in the next four those of a quarter "apart"
+    const uint32_t sS = stV + KM_KEYS * D;
+    const uint32_t bars = sS + 128, sE = bars + 256; // sE [2][128]: exponents of a key's references (key, value), a byte each
     const uint32_t q_ready = bars, s_full = bars + 16, p_ready = bars + 32, pv_done = bars + 48;                          // + 8 * query tile
     const uint32_t k_full = bars + 144, k_empty = bars + 160, v_full = bars + 176, v_empty = bars + 192;                  // + 8 * place
     const uint32_t sc_full = bars + 208, sc_empty = bars + 64;                                                            // + 8 * buffer
@@ -386,18 +443,26 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
             for (int j = 0; j < it.n_kt && ok; j++) {
                 const uint32_t g = gs + j, b = g & 1, ph = (g >> 1) & 1, at = sS + b * 64u + 4u * (warp - 8);
                 // the references: powers of two above the largest scales (maxima pass by what is no number)
-                const uint32_t kf = min((__float_as_uint(warp_max(fmaxf(sc.x, 0.f))) >> 23) + 1u, 253u);
-                const uint32_t vf = max(min((__float_as_uint(warp_max(fmaxf(sc.y, 0.f))) >> 23) + 1u, 253u), 37u);           // 2^-90
+                const float k_scale = fmaxf(sc.x, 0.f), v_scale = fmaxf(sc.y, 0.f);
+                uint32_t kf = km_above(warp_max(k_scale)), vf = km_above(warp_max(v_scale));
                 const bool number = sc.x == sc.x && sc.y == sc.y;
+                // ... for all 32 keys, unless they are so far apart that float16 would lose the smaller ones, or so large or small that a row's weights
+                // and exponentials could not go by one reference: then every key has its own
+                const bool apart = __any_sync(0xffffffffu, there && number && (km_above(k_scale) + KM_APART < kf || km_above(v_scale) + KM_APART < vf)) ||
+                                   vf + KM_RANGE < 127u || vf > 127u + KM_RANGE;
+                const uint32_t k_ref = kf, v_ref = vf;
+                if (apart && there && number) { kf = km_above(k_scale); vf = km_above(v_scale); }
                 const float ks = number ? sc.x * __uint_as_float((254u - kf) << 23) : __uint_as_float(0x7fc00000u);
                 const __half k_hi = __float2half_rn(ks), k_lo = __float2half_rn(ks - __half2float(k_hi));
                 const __half v_hi = __float2half_rn(number ? sc.y * __uint_as_float((254u - vf) << 23) : 0.f);
                 const uint32_t present = __ballot_sync(0xffffffffu, there);
                 ok = km_wait_warp(sc_empty + 8 * b, ph ^ 1, abort_flag, err);
                 if (!ok) break;
+                asm volatile("st.shared.u16 [%0], %1;" ::"r"(sE + 2u * (b * KM_KEYS + row)), "h"((unsigned short)(kf | vf << 8)) : "memory");
+                __syncwarp();
                 if (lane == 0) {
-                    asm volatile("st.shared.f32 [%0], %1;\n\tst.shared.f32 [%0 + 16], %2;\n\tst.shared.u32 [%0 + 32], %3;"
-                                 ::"r"(at), "f"(__uint_as_float(kf << 23)), "f"((float)vf - 127.f), "r"(present) : "memory");
+                    asm volatile("st.shared.f32 [%0], %1;\n\tst.shared.f32 [%0 + 16], %2;\n\tst.shared.u32 [%0 + 32], %3;\n\tst.shared.u32 [%0 + 48], %4;"
+                                 ::"r"(at), "f"(__uint_as_float(k_ref << 23)), "f"((float)v_ref - 127.f), "r"(apart ? 0u : present), "r"(apart ? present : 0u) : "memory");
                     mbar_arrive(sc_full + 8 * b);
                 }
                 if (!km_wait_warp(k_empty + 8 * b, ph ^ 1, abort_flag, err)) { ok = false; break; }
@@ -472,6 +537,9 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                 return (to > 31 ? 0xffffffffu : (1u << to) - 1u) & (from > 31 ? 0u : 0xffffffffu << from);
             };
             float ref = -INFINITY, l = 0.f;                              // what the exponentials refer to, their sum
+            // `two`: weights and sum have references of their own, the sum l_ref
+            bool two = false;
+            float l_ref = -INFINITY;
             for (int j = 0; j < it.n_kt && ok; j++) {
                 const uint32_t b = (gs + j) & 1, sc_ph = ((gs + j) >> 1) & 1, s_at = sS + b * 64u;
                 if (!km_wait_warp(sc_full + 8 * b, sc_ph, abort_flag, err)) { ok = false; break; }
@@ -486,7 +554,12 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                 // a step without options in which every row sees every key, as most are (rows beyond the tile's tokens go with those)
                 const float4 there4 = km_load4(s_at + 32u);
                 const bool full = (__float_as_uint(there4.x) & __float_as_uint(there4.y) & __float_as_uint(there4.z) & __float_as_uint(there4.w)) == 0xffffffffu;
-                const bool open = __all_sync(0xffffffffu, !valid || (key0 + KM_KEYS - 1 <= pos && key0 >= lo)) && full && !finished;
+                const bool open = __all_sync(0xffffffffu, !valid || (key0 + KM_KEYS - 1 <= pos && key0 >= lo)) && full && !finished && !two;
+                bool apart = two;                                        // (keys with references of their own are not among `there4`)
+                if (!open) {
+                    const float4 own = km_load4(s_at + 48u);
+                    apart = apart || (__float_as_uint(own.x) | __float_as_uint(own.y) | __float_as_uint(own.z) | __float_as_uint(own.w)) != 0u;
+                }
                 const float by_head = unit * hscale;
                 // (loops over the quarters of a tile stay loops: eight warps of these run beside four that convert, and unrolled their
                 // instructions do not stay in the caches: 410 us for the portion named above, 358 so)
@@ -514,10 +587,16 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                         for (int c = 0; c < 32; c++) raw[c] = sees >> c & 1u ? raw[c] : 0xff800000u;
                     }
                 };
+                auto row_of = [&] {
+                    return KmRow{tS, sE + 2u * b * KM_KEYS, valid ? s_at + 32u : 0u, capped ? cap_in : by_head, capped ? cap2 : 0.f, slope2, key0, pos, lo};
+                };
                 auto sees_of = [&](int q) { return valid ? seen(key0 + 32 * q) & __float_as_uint(km_load1(s_at + 32u + 4u * q)) : 0u; };
-                float mx = -INFINITY;
+                float mx = -INFINITY, ms = -INFINITY;                    // the row's largest weight (`apart`: and score), in the exponent's base 2
                 uint32_t ra[32], rb[32];
-                if (open) {
+                if (apart) {
+                    const float2 most = km_apart<false>(row_of(), 0.f, 0.f);
+                    ms = most.x; mx = most.y;
+                } else if (open) {
                     // (the next 32 are on their way while these are worked on)
                     auto largest = [&](int q, const uint32_t (&raw)[32]) {
                         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -566,6 +645,7 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                 }
                 mx -= 10.f;
                 // raise the reference only when it has been outgrown by 2^4 (or there was none yet)
+                const float before = ref;
                 float corr = 1.f;
                 if (mx > ref + 4.f || (ref == -INFINITY && mx > -INFINITY)) {
                     corr = ref == -INFINITY ? 0.f : km_ex2(ref - mx);
@@ -585,7 +665,7 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                 const float minus = ref == -INFINITY ? 0.f : -ref;
                 const f32pair one2 = pair_of(1.f, 1.f);
                 float step_sum = 0.f;
-                // weights 2^(score + log2 of the values' reference - R), over scores that have been read; the sum goes without the reference
+                // weights 2^(score + log2 of the values' reference - R), over scores that have been read; the sum goes without that reference
                 auto weights = [&](int q, const uint32_t (&raw)[32], bool scaled) {
                     const float factor = scaled ? 1.f : unit * k_ref(q), log = v_log(q);
                     const f32pair a2 = pair_of(factor, factor), m2 = pair_of(log + minus, log + minus);
@@ -603,7 +683,25 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                     step_sum = fmaf((s0.x + s0.y) + (s1.x + s1.y), __uint_as_float((uint32_t)(127.f - log) << 23), step_sum);
                 };
                 __syncwarp();
-                if (open) {
+                if (apart) {
+                    // the sum's own reference: that of the weights until here, then kept such that the sum is near one
+                    auto near_one = [&] {
+                        const int e = l > 0.f && l < 1e38f ? (int)(__float_as_uint(l) >> 23) - 127 : 0;
+                        l *= __uint_as_float((uint32_t)(127 - e) << 23);
+                        l_ref += (float)e;
+                    };
+                    if (!two) { l_ref = before; near_one(); }
+                    if (ms > l_ref + 4.f || (l_ref == -INFINITY && ms > -INFINITY)) {
+                        if (l_ref != -INFINITY) l *= km_ex2(l_ref - ms);
+                        l_ref = ms;
+                    }
+                    l += km_apart<true>(row_of(), minus, l_ref == -INFINITY ? 0.f : -l_ref).x;
+                    near_one();
+                    // one reference does again where the two are as near each other, in every row of the warp, as steps of one reference bring them
+                    const float gap = ref == -INFINITY ? 0.f : l_ref - ref;
+                    two = !__all_sync(0xffffffffu, gap > 10.f - KM_RANGE && gap < KM_RANGE);
+                    if (!two) l *= km_ex2(gap);
+                } else if (open) {
 #pragma unroll 1
                     for (int q = 0; q < 4; q += 2) {
                         load32(q + 1, rb);
@@ -626,7 +724,7 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(sc_empty + 8 * b);
-                l = fmaf(l, corr, step_sum);
+                if (!apart) l = fmaf(l, corr, step_sum);
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 tc_fence_before();
                 __syncwarp();
@@ -647,18 +745,15 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
             // the sink is one more term of the whole sum, and joins it where that is made: what one piece's exponentials refer to may lie hundreds
             // below it (with slopes a tile's oldest keys do), out of float32's range
             const bool sink = p.sinks || p.zero_sink;
+            if (!two) l_ref = ref;
             const float sk = p.sinks && valid ? p.sinks[it.g * r + hl] * log2e : 0.f;
             // the pieces of this double tile and head: of CTAs c_first .. c_first + pieces - 1, each its first but for the first one's last
             const int c_first = (int)(((it.first + 1) * ctas - 1) / total), pieces = (int)(((it.first + it.all) * ctas - 1) / total) - c_first + 1;
             uint4 *dst = (uint4 *)((__nv_bfloat16 *)p.out + th);
             if (pieces == 1) {
-                float scaled = 1.f;                                      // what the outputs and their sum are brought down by for the sink
-                if (sink) {
-                    const float top = fmaxf(ref, sk);
-                    scaled = exp2f(ref - top);
-                    l = fmaf(l, scaled, exp2f(sk - top));
-                }
-                const float inv = l == 0.f ? 0.f : scaled / l;
+                const float top = sink ? fmaxf(l_ref, sk) : l_ref;
+                if (sink) l = fmaf(l, exp2f(l_ref - top), exp2f(sk - top));
+                const float inv = l == 0.f ? 0.f : (ref == -INFINITY ? 1.f : exp2f(ref - top)) / l;
 #pragma unroll 1
                 for (int c = 0; c < D / 16; c += 4) {                    // four reads of 16 columns under way together
                     uint32_t ov[64];
@@ -698,7 +793,7 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                 } else {
                     for (int c = 0; c < D / 4; c++) po[c * 128] = make_float4(0.f, 0.f, 0.f, 0.f);
                 }
-                ((float2 *)f.part_ml)[place_of(cta) * 128 + row] = make_float2(ref, l);
+                ((float4 *)f.part_ml)[place_of(cta) * 128 + row] = make_float4(ref, l_ref, l, 0.f);
             }
             int *flag = (int *)(gen + (bars - base) + 232 + 4 * i);
             asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
@@ -713,11 +808,12 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
             if (!*(volatile int *)flag || !valid) continue;              // (the flag is written again behind two barriers)
             __threadfence();
             float top = sink ? sk : -INFINITY, sum = 0.f;
-            for (int c = 0; c < pieces; c++) top = fmaxf(top, __ldcg((const float2 *)f.part_ml + place_of(c_first + c) * 128 + row).x);
+            auto sums_of = [&](int c) { return __ldcg((const float4 *)f.part_ml + place_of(c_first + c) * 128 + row); };
+            for (int c = 0; c < pieces; c++) top = fmaxf(top, sums_of(c).y);
             if (sink) sum = exp2f(sk - top);
             for (int c = 0; c < pieces; c++) {
-                const float2 ml = __ldcg((const float2 *)f.part_ml + place_of(c_first + c) * 128 + row);
-                sum += ml.y * (ml.x == -INFINITY ? 1.f : exp2f(ml.x - top));           // (zero, or no number)
+                const float4 m = sums_of(c);
+                sum += m.z * (m.y == -INFINITY ? 1.f : exp2f(m.y - top));              // (zero, or no number)
             }
             const float inv = sum == 0.f ? 0.f : 1.0f / sum;
 #pragma unroll 1
@@ -727,8 +823,7 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                 for (int u = 0; u < 8; u++) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
                 for (int k = 0; k < pieces; k++) {
                     const size_t at = place_of(c_first + k);
-                    const float2 ml = __ldcg((const float2 *)f.part_ml + at * 128 + row);
-                    const float e = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
+                    const float own = sums_of(k).x, e = own == -INFINITY ? 0.f : exp2f(own - top) * inv;
                     const float4 *po = (const float4 *)f.part_o + (at * (D / 4) + c) * 128 + row;
 #pragma unroll
                     for (int u = 0; u < 8; u++) {
@@ -738,8 +833,8 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                 }
 #pragma unroll
                 for (int u = 0; u < 8; u += 2) {
-                    __nv_bfloat162 h[4] = {__floats2bfloat162_rn(acc[u].x * inv, acc[u].y * inv), __floats2bfloat162_rn(acc[u].z * inv, acc[u].w * inv),
-                                           __floats2bfloat162_rn(acc[u + 1].x * inv, acc[u + 1].y * inv), __floats2bfloat162_rn(acc[u + 1].z * inv, acc[u + 1].w * inv)};
+                    __nv_bfloat162 h[4] = {__floats2bfloat162_rn(acc[u].x, acc[u].y), __floats2bfloat162_rn(acc[u].z, acc[u].w),
+                                           __floats2bfloat162_rn(acc[u + 1].x, acc[u + 1].y), __floats2bfloat162_rn(acc[u + 1].z, acc[u + 1].w)};
                     dst[(c + u) / 2] = *(uint4 *)h;
                 }
             }
@@ -774,7 +869,7 @@ static int launch_kv8_many(const Kv8ManyParams &f, int grid, cudaStream_t st)
 
 using namespace hfb;
 
-extern "C" size_t hfb_kv8_attention_many_scratch(int ctas, int d) { return (size_t)ctas * 4 * 128 * (d + 2) * sizeof(float); }
+extern "C" size_t hfb_kv8_attention_many_scratch(int ctas, int d) { return (size_t)ctas * 4 * 128 * (d + 4) * sizeof(float); }
 
 extern "C" int hfb_kv8_attention_many(const void *q, const void *cache, const int32_t *block_table, int max_blocks, const int32_t *positions,
                                       const int32_t *tile_seq, const int32_t *tile_t0, const int32_t *tile_nt, int n_tiles, int ctas, int tile_cost, int settled, int block_size,

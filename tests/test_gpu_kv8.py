@@ -673,3 +673,93 @@ def test_sinks_beside_keys_far_below_them(shape, slope, sink):
         assert torch.isfinite(got).all()
         check(s, q, cache, got, H, **o)
     K.check_device_errors()
+
+
+# ---- scales far apart --------------------------------------------------------------------------------------------------------
+# Nothing that a row does not see may take part in how its numbers are rounded by more than a step, and no value is too small beside its
+# neighbours.  Tolerance: the output's rounding 2^-8; a weight's rounding 2^-11, a value's scale's and the value's own, 2^-11 each, of
+# sum p |v|; the scores' e as above, with a key's own rounding in the prompts' kernel: 2^-11 of sum |q k|, which the sum |q| 255 scale that e
+# is taken of exceeds twofold at least, so 2^-12 of it at most; 4 e.  And float16's smallest step, 2^-24: a weight times its value's
+# reference (a power of two, at most twice the value's scale) is held as 2^10 times its share of the largest such product among the keys
+# that the row sees, so that each of n keys is off by 127 2^-25 2^-10 2 times the largest p scale of the row.  The row of values that has
+# it has a code of 127: 127 p scale is at most the largest sum p |v| of the row.  2^-34 n of that, and nothing of what the row does not
+# see.  (The first run came without this last term: numbers of 1e-10 beside ones of 1e12 in the same output row were zeros.)
+
+def check_apart(s, q, got, H, rows=None, mask=0, scale=None, cache=None, size_of_scores=None, least=0.0):
+    """``rows``: tokens that are looked at; ``size_of_scores``: sum |q| 255 scale to reckon with instead of that of all keys seen."""
+    scale = 1 / math.sqrt(s.d) if scale is None else scale
+    rows = torch.arange(s.T, device=DEV) if rows is None else rows
+    ref, size, worst, _ = attention(q[rows], cache, s.table, s.seq[rows], s.positions[rows], s.bs, H, s.G, s.d, mask, scale)
+    worst = worst if size_of_scores is None else size_of_scores
+    e = (2.0 ** -16 + 2.0 ** -20 + (2.0 ** -12 if size_of_scores is None else 0)) * worst
+    got = got[rows].double().view(ref.shape)
+    assert torch.isfinite(got).all()
+    tol = 2.0 ** -8 * ref.abs() + (3 * 2.0 ** -11 + 4 * min(e, 0.02)) * size + 2.0 ** -34 * max(s.kv_lens) * size.amax(-1, keepdim=True)
+    off = (got - ref).abs()
+    assert float(ref.abs().max()) >= least and (off <= tol + 1e-37).all(), float((off / (tol + 1e-37)).max())
+
+
+APART = [(14, 2, 64, 16), (28, 4, 128, 16), (8, 2, 80, 16)]
+APART_STEPS = {"portion": ([70, 90], [70, 800])}
+
+
+@pytest.mark.parametrize("name", list(APART_STEPS))
+@pytest.mark.parametrize("shape", APART, ids=str)
+def test_later_tokens_change_nothing_before_them(shape, name):
+    """The last tokens of each request bring values, or keys, up to 2^60 times as large as the others."""
+    H, G, d, bs = shape
+    for by in (2.0 ** 14, 2.0 ** 24, 2.0 ** 40, 2.0 ** 60):
+        for of in ("values", "keys"):
+            s = step(*APART_STEPS[name], bs, G, d, seed=d)
+            q = torch.randn(s.T, H * d, generator=s.g, device=DEV).bfloat16()
+            before, at = [], 0
+            for i, (n_q, n) in enumerate(zip(s.q_lens, s.kv_lens)):
+                late = 0 if n_q == 1 else n_q // 2
+                for p in range(n - late, n):
+                    (s.vs if of == "values" else s.ks)[s.table[i, p // bs], p % bs] *= by
+                before += range(at, at + n_q - late)
+                at += n_q
+            cache = pack(s.k, s.ks, s.v, s.vs)
+            check_apart(s, q, attend(s, q, cache, H), H, rows=torch.tensor(before, device=DEV), cache=cache)
+
+
+@pytest.mark.parametrize("name", list(APART_STEPS))
+@pytest.mark.parametrize("shape", APART, ids=str)
+def test_values_of_any_size(shape, name):
+    """All values small or large; sizes from 2^-40 to 2^40 side by side; large ones that weigh next to nothing."""
+    H, G, d, bs = shape
+    for by in (2.0 ** -115, 2.0 ** -95, 2.0 ** 80):
+        s = step(*APART_STEPS[name], bs, G, d, seed=d)
+        q = torch.randn(s.T, H * d, generator=s.g, device=DEV).bfloat16()
+        s.vs *= by
+        cache = pack(s.k, s.ks, s.v, s.vs)
+        check_apart(s, q, attend(s, q, cache, H), H, cache=cache, least=by)
+    s = step(*APART_STEPS[name], bs, G, d, seed=d)
+    s.vs *= 2.0 ** torch.randint(-40, 41, s.vs.shape, generator=s.g, device=DEV)
+    cache = pack(s.k, s.ks, s.v, s.vs)
+    check_apart(s, q, attend(s, q, cache, H), H, cache=cache)
+    # every ninth key's score lies about 40 below the others' in the base 2, and its value is 2^30 or 2^-30 as large
+    for by in (2.0 ** 30, 2.0 ** -30):
+        s = step(*APART_STEPS[name], bs, G, d, seed=d)
+        q = (torch.randn(s.T, H * d, generator=s.g, device=DEV) * 0.3 + 0.5).bfloat16()
+        s.k[:, ::9], s.ks[:, ::9] = -100, 28 / (100 * 0.5 * math.sqrt(d))
+        s.vs[:, ::9] *= by
+        cache = pack(s.k, s.ks, s.v, s.vs)
+        check_apart(s, q, attend(s, q, cache, H), H, cache=cache)
+
+
+@pytest.mark.parametrize("name", list(APART_STEPS))
+@pytest.mark.parametrize("shape", APART, ids=str)
+def test_keys_beside_one_that_is_far_larger(shape, name):
+    """A key of each tile 2^22 times as large as the others, whose scores are as far below theirs: it has no weight, and the others have
+    theirs."""
+    H, G, d, bs = shape
+    s = step(*APART_STEPS[name], bs, G, d, seed=d)
+    q = (torch.randn(s.T, H * d, generator=s.g, device=DEV) * 0.3 + 1).bfloat16()
+    plain = pack(s.k, s.ks, s.v, s.vs)
+    _, _, worst, _ = attention(q, plain, s.table, s.seq, s.positions, bs, H, G, d, 0, 1 / math.sqrt(d))
+    for i, n in enumerate(s.kv_lens):
+        for p in range(3, n, 33):
+            s.k[s.table[i, p // bs], p % bs], s.ks[s.table[i, p // bs], p % bs] = -100, 2.0 ** 22 * 0.02
+    cache = pack(s.k, s.ks, s.v, s.vs)
+    check_apart(s, q, attend(s, q, cache, H), H, cache=cache, size_of_scores=worst)
