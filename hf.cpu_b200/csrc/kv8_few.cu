@@ -21,6 +21,9 @@
 //   references are raised, and the sums so far rescaled, only when a score exceeds its by more than 2^4 or a scale by more than a
 //   factor of two: the product is 2^15 at most, and is rounded once to float16 (11 bits; weights down to 2^-24 of the largest at
 //   full precision, 2^-34 at all).  (Raised whenever a maximum grows, one of eight columns' did in more than half of the steps.)
+// * The scales' reference is all columns', whatever each of them sees.  Where a scale lies more than 2^12 below it, the step's second product
+//   is made up to four times, for weights of 2^-24 of each other: down to 2^-91 of the largest they keep their 11 bits, beside keys that
+//   their token does not see or gives no weight.
 //
 // Measured (28 heads of 128 on 4): 64 requests of up to 8,192 tokens 70 us, 0.61 of the measured bandwidth (the bfloat16 cache's kernel, which
 // reads twice the bytes, 113 us); eight of up to 32,768 tokens 43 us, 0.49 (65).  About 15 us of each are the start of a launch, its
@@ -42,6 +45,7 @@ namespace hfb {
 int *error_word();
 
 constexpr int KF_MAX_TILES = 2048;
+constexpr float KF_APART = 0.000244140625f;          // 2^-12: value scales up to here below the reference go into the weights all at once
 
 struct Kv8FewParams {
     Kv8Params a;
@@ -422,22 +426,27 @@ kv8_few_kernel(Kv8FewParams f, int *err)
 #pragma unroll
                         for (int u = 0; u < 2; u++) {
                             const int k = kbase + 16 * h + 8 * u + row8;
-                            if (kt * ABN + k > pos_last || kt * ABN + k < lo_first || !(mask >> (k / bs) & 1u)) ks[h][u] = vs[h][u] = 0.f;
+                            if (kt * ABN + k > pos_last || kt * ABN + k < lo_first || !(mask >> (k / bs) & 1u)) { ks[h][u] = 0.f; vs[h][u] = vm; }
                         }
                 }
                 const float vs_top = fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[KH - 1][0], vs[KH - 1][1]));
-                if (__any_sync(0xffffffffu, vs_top > 2.f * vm)) {
-                    float v = fmaxf(vm, vs_top);
-                    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
-                    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
-                    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-                    const float shrink = vm / v;
+                const float vs_low = fminf(fminf(vs[0][0], vs[0][1]), fminf(vs[KH - 1][0], vs[KH - 1][1]));
+                bool apart = false;
+                if (__any_sync(0xffffffffu, vs_top > 2.f * vm || vs_low < KF_APART * vm)) {
+                    if (__any_sync(0xffffffffu, vs_top > 2.f * vm)) {
+                        float v = fmaxf(vm, vs_top);
+                        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+                        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+                        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+                        const float shrink = vm / v;
 #pragma unroll
-                    for (int c = 0; c < CH; c++)
+                        for (int c = 0; c < CH; c++)
 #pragma unroll
-                        for (int n = 0; n < NT; n++) { o[c][n][0] *= shrink; o[c][n][1] *= shrink; o[c][n][2] *= shrink; o[c][n][3] *= shrink; }
-                    vm = v;
-                    rv = 1.0f / v;
+                            for (int n = 0; n < NT; n++) { o[c][n][0] *= shrink; o[c][n][1] *= shrink; o[c][n][2] *= shrink; o[c][n][3] *= shrink; }
+                        vm = v;
+                        rv = 1.0f / v;
+                    }
+                    apart = __any_sync(0xffffffffu, vs_low < KF_APART * vm);
                 }
 #pragma unroll
                 for (int h = 0; h < KH; h++)
@@ -494,39 +503,73 @@ kv8_few_kernel(Kv8FewParams f, int *err)
                             m[n][i] = v;
                         }
                 }
-                uint32_t pf[KH][NT][2];
 #pragma unroll
                 for (int h = 0; h < KH; h++) {
                     const float vn0 = vs[h][0] * rv * 1024.f, vn1 = vs[h][1] * rv * 1024.f;
 #pragma unroll
                     for (int n = 0; n < NT; n++) {
-                        float w[4];
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             const int i = e & 1;
+                            const bool none = edge && sc[h][n][e] == -INFINITY;
                             const float q = fast_exp2(sc[h][n][e] - (m[n][i] == -INFINITY ? 0.f : m[n][i]));
                             l[n][i] += q;
-                            w[e] = q * (e < 2 ? vn0 : vn1);
-                            if (edge && sc[h][n][e] == -INFINITY) w[e] = 0.f;    // (a value that is no number, for a row that does not see it)
+                            sc[h][n][e] = q * (e < 2 ? vn0 : vn1);
+                            if (none) sc[h][n][e] = 0.f;                  // (a value that is no number, for a row that does not see it)
                         }
-                        pf[h][n][0] = transpose8(pack_f16(w[0], w[1]));
-                        pf[h][n][1] = transpose8(pack_f16(w[2], w[3]));
                     }
                 }
+                // the weights in float16: all at once, or those down to 2^-24 of the largest there can be, the next 2^-24 with the sums so far (and
+                // themselves) 2^24 times as large, and so on
+                int times = 0;
+#pragma unroll 1
+                for (;;) {
+                    uint32_t pf[KH][NT][2];
+                    bool more = false;
 #pragma unroll
-                for (int h = 0; h < KH; h++)
-#pragma unroll
-                    for (int c = 0; c < CH / 2; c++) {
-                        uint32_t w0, w1, w2, w3;
-                        ldsm_x4_t(sv + piece[h][c], w0, w1, w2, w3);
-                        const uint32_t a0 = codes_f16(w0, 0x4240), a1 = codes_f16(w0, 0x4341), a2 = codes_f16(w1, 0x4240), a3 = codes_f16(w1, 0x4341);
-                        const uint32_t b0 = codes_f16(w2, 0x4240), b1 = codes_f16(w2, 0x4341), b2 = codes_f16(w3, 0x4240), b3 = codes_f16(w3, 0x4341);
+                    for (int h = 0; h < KH; h++)
 #pragma unroll
                         for (int n = 0; n < NT; n++) {
-                            mma_f16(o[2 * c][n], a0, a1, a2, a3, pf[h][n][0], pf[h][n][1]);
-                            mma_f16(o[2 * c + 1][n], b0, b1, b2, b3, pf[h][n][0], pf[h][n][1]);
+                            if (apart) {
+                                float w[4];
+#pragma unroll
+                                for (int e = 0; e < 4; e++) {
+                                    const bool small = sc[h][n][e] < 0.001953125f;           // 2^-9
+                                    w[e] = small ? 0.f : sc[h][n][e];
+                                    sc[h][n][e] = small ? sc[h][n][e] * 16777216.f : 0.f;
+                                    more |= sc[h][n][e] != 0.f;
+                                }
+                                pf[h][n][0] = transpose8(pack_f16(w[0], w[1]));
+                                pf[h][n][1] = transpose8(pack_f16(w[2], w[3]));
+                            } else {
+                                pf[h][n][0] = transpose8(pack_f16(sc[h][n][0], sc[h][n][1]));
+                                pf[h][n][1] = transpose8(pack_f16(sc[h][n][2], sc[h][n][3]));
+                            }
                         }
-                    }
+#pragma unroll
+                    for (int h = 0; h < KH; h++)
+#pragma unroll
+                        for (int c = 0; c < CH / 2; c++) {
+                            uint32_t w0, w1, w2, w3;
+                            ldsm_x4_t(sv + piece[h][c], w0, w1, w2, w3);
+                            const uint32_t a0 = codes_f16(w0, 0x4240), a1 = codes_f16(w0, 0x4341), a2 = codes_f16(w1, 0x4240), a3 = codes_f16(w1, 0x4341);
+                            const uint32_t b0 = codes_f16(w2, 0x4240), b1 = codes_f16(w2, 0x4341), b2 = codes_f16(w3, 0x4240), b3 = codes_f16(w3, 0x4341);
+#pragma unroll
+                            for (int n = 0; n < NT; n++) {
+                                mma_f16(o[2 * c][n], a0, a1, a2, a3, pf[h][n][0], pf[h][n][1]);
+                                mma_f16(o[2 * c + 1][n], b0, b1, b2, b3, pf[h][n][0], pf[h][n][1]);
+                            }
+                        }
+                    if (!apart) break;
+                    more = __any_sync(0xffffffffu, more) && times < 3;
+                    const float by = more ? 16777216.f : __uint_as_float((uint32_t)(127 - 24 * times) << 23);
+#pragma unroll
+                    for (int c = 0; c < CH; c++)
+#pragma unroll
+                        for (int n = 0; n < NT; n++) { o[c][n][0] *= by; o[c][n][1] *= by; o[c][n][2] *= by; o[c][n][3] *= by; }
+                    if (!more) break;
+                    times++;
+                }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(empty0 + 8 * s);
             }

@@ -700,7 +700,7 @@ def check_apart(s, q, got, H, rows=None, mask=0, scale=None, cache=None, size_of
 
 
 APART = [(14, 2, 64, 16), (28, 4, 128, 16), (8, 2, 80, 16)]
-APART_STEPS = {"portion": ([70, 90], [70, 800])}
+APART_STEPS = {"portion": ([70, 90], [70, 800]), "few": ([5, 3, 16, 1], [5, 300, 90, 200])}
 
 
 @pytest.mark.parametrize("name", list(APART_STEPS))
