@@ -94,6 +94,15 @@ class LayerCache:
         return (self.k, self.v) if self.kv8 is None else (self.kv8,)
 
 
+def eight_bits_refusal(spec: CacheSpec, block_size: int) -> Optional[str]:
+    """Why a cache in 8 bits does not hold what a layer caches; None if it does."""
+    if not spec.values_in_keys and spec.value_dim == spec.head_dim and kernels.kv8_takes(spec.head_dim, block_size):
+        return None
+    what = "values inside its keys" if spec.values_in_keys else f"heads of {spec.head_dim} and {spec.value_dim} in pages of {block_size} tokens"
+    return (f"caches {what}: a cache in 8 bits holds keys and values of one size, a multiple of 16 up to {kernels.MAX_HEAD_DIM}, in pages of up to "
+            f"{kernels.KV8_BLOCK} tokens")
+
+
 class CacheGroup:
     """Schedule entries with the same needs share page geometry, a pool and block tables."""
 
@@ -105,10 +114,9 @@ class CacheGroup:
         shape = (len(self.entries), num_pages, block_size, spec.num_kv_heads)
         self.records = None
         if eight_bits:
-            if spec.values_in_keys or spec.value_dim != spec.head_dim or not kernels.kv8_takes(spec.head_dim, block_size):
-                raise UnsupportedError(f"a cache in 8 bits holds keys and values of one size, a multiple of 16 up to {kernels.MAX_HEAD_DIM}, in pages of "
-                                       f"up to {kernels.KV8_BLOCK} tokens; this model has layers with "
-                                       + ("values inside their keys" if spec.values_in_keys else f"heads of {spec.head_dim} and {spec.value_dim}"))
+            reason = eight_bits_refusal(spec, block_size)
+            if reason:
+                raise UnsupportedError(f"schedule entry {self.entries[0]} {reason}")
             self.storage = self.keys = self.values = None
             self.records = kernels.kv8_cache(len(self.entries) * num_pages, block_size, spec.num_kv_heads, spec.head_dim, device).view(
                 len(self.entries), num_pages, spec.num_kv_heads, -1)

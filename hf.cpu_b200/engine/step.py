@@ -18,7 +18,7 @@ import torch
 
 from .. import kernels
 from ..config.base import UnsupportedError
-from ..cache import KVCacheManager, OutOfPages, StateSlots
+from ..cache import KVCacheManager, OutOfPages, StateSlots, eight_bits_refusal
 from ..models import EMBEDDING_STATE, Model, block_state_key
 
 
@@ -175,8 +175,10 @@ class Engine:
         if self.eight_bits:
             for e in plan.schedule:
                 mixer = model.layers[e.layer].mixer
-                if mixer.cache_spec() is not None and not mixer.caches_eight_bits:
-                    raise UnsupportedError(f"layer {e.layer} ({type(mixer).__name__}) does not run on a cache in 8 bits")
+                spec = mixer.cache_spec()
+                reason = None if spec is None else "does not run on a cache in 8 bits" if not mixer.caches_eight_bits else eight_bits_refusal(spec, self.block_size)
+                if reason:
+                    raise UnsupportedError(f"layer {e.layer} ({type(mixer).__name__}) {reason}")
         # index arrays the mixers want built per step (tile lists of their kernels and the like): one owner per key,
         # so that layers with the same needs share one set
         self._array_owners: Dict[Hashable, object] = {}

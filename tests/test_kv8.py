@@ -299,3 +299,16 @@ def test_counters_are_cleared_behind_a_launch_that_gave_up(monkeypatch):
     word[0] = 8
     assert b.error_word() == 8 and not any(bool(x.any()) for x in held) and not b._counters.any()
     assert synced
+
+
+@pytest.mark.parametrize("change,what", [(dict(d=24, dv=24), "heads of 24 and 24"), (dict(values_are_keys=True), "values inside its keys"), (dict(dv=48), "heads of 32 and 48"),
+                                         (dict(caches_eight_bits=False), "does not run")])
+def test_refusals_name_the_layer(emu, change, what):
+    """A model with a layer that 8 bits do not serve, behind others that they do."""
+    model = random_model(config_from_dict(TINY["A"]), seed=3, dtype=torch.float32, device="cpu", std=0.05)
+    mixer = model.layers[1].mixer
+    mixer.d, mixer.dv = 32, 32
+    for name, value in change.items():
+        setattr(mixer, name, value)
+    with pytest.raises(UnsupportedError, match=rf"layer 1 \(PagedAttention\) .*{what}"):
+        Engine(model, block_size=8, max_tokens=64, kv_dtype="int8")
