@@ -354,7 +354,7 @@ _KV8_TILES = tuple(tuple(f"{kind}.{part}" for part in ("seq", "t0", "nt")) for k
 
 
 def _kv8_rows(x, T, n, dtype, what) -> None:
-    if x.dim() != 2 or x.shape[0] != T or x.shape[1] != n or x.dtype != dtype or x.stride(1) != 1 or x.stride(0) < n:
+    if x.dim() != 2 or x.shape[0] != T or x.shape[1] != n or x.dtype != dtype or x.stride(1) != 1 or (x.stride(0) < n and T > 1):
         raise ValueError(f"{what} must be rows [{T}, {n}] of one type")
 
 

@@ -312,3 +312,19 @@ def test_refusals_name_the_layer(emu, change, what):
         setattr(mixer, name, value)
     with pytest.raises(UnsupportedError, match=rf"layer 1 \(PagedAttention\) .*{what}"):
         Engine(model, block_size=8, max_tokens=64, kv_dtype="int8")
+
+
+def test_a_single_row_may_say_what_it_likes_of_the_next(emu):
+    """One row's stride to the next one means nothing: any number is taken, as torch makes them."""
+    row = torch.randn(1, 256)
+    odd = torch.as_strided(row.clone(), (1, 256), (1, 1))
+    assert odd.stride(0) == 1
+    caches = []
+    for x in (row, odd):
+        a = _args(T=1, dtype=torch.float32)
+        kernels.rope_kv8_write(**{**a, "qkv": x})
+        kernels.kv8_write(x[:, 128:192], x[:, 192:], a["slots"] + 9, a["cache"], 2, 32, 8)
+        caches.append(a["cache"])
+    assert torch.equal(*caches) and caches[0].any()
+    with pytest.raises(ValueError):
+        kernels.rope_kv8_write(**{**_args(T=2, dtype=torch.float32), "qkv": torch.as_strided(torch.zeros(512), (2, 256), (1, 1))})
