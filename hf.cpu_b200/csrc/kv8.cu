@@ -214,8 +214,7 @@ kv8_write_kernel(Kv8WriteParams p, int *err)
 
 // ---- read ----------------------------------------------------------------------------------------------------------------
 // The rows of some pages as the values that they stand for, [N, block, G, d] keys and values.  A thread makes 16 bytes of the output at a
-// time, neighbouring threads neighbouring ones.  A block takes as many records
-// at once as its threads have pieces for, and four times that many before it stores any: a thread has the same pieces of each.
+// time, neighbouring threads neighbouring ones.
 __device__ __forceinline__ void kv8_store(float *dst, const float (&v)[4]) { *(float4 *)dst = make_float4(v[0], v[1], v[2], v[3]); }
 __device__ __forceinline__ void kv8_store(__nv_bfloat16 *dst, const float (&v)[8])
 {
@@ -309,6 +308,7 @@ kv8_read_bulk_kernel(const uint8_t *cache, long long num_pages, const int32_t *p
     __syncthreads();
 }
 
+// Larger records (more pieces than threads, then): plain loads, of four records before any is stored.
 template <typename T>
 __global__ void __launch_bounds__(KV8_READ_THREADS)
 kv8_read_kernel(const uint8_t *cache, long long num_pages, const int32_t *pages, const int32_t *used, T *k_out, T *v_out, int records,
@@ -316,21 +316,19 @@ kv8_read_kernel(const uint8_t *cache, long long num_pages, const int32_t *pages,
 {
     pdl_sync();
     constexpr int PER = 16 / sizeof(T);                          // codes of a piece: 8 or 4
-    const int row_pieces = d / PER, pieces = 2 * block_size * row_pieces, at_once = max(1, KV8_READ_THREADS / pieces);
-    const int mine = threadIdx.x / pieces;                       // of the records at once (more pieces than threads: always 0)
-    if (mine >= at_once) return;
-    for (int i = threadIdx.x % pieces; i < pieces; i += KV8_READ_THREADS) {
+    const int row_pieces = d / PER, pieces = 2 * block_size * row_pieces;
+    for (int i = threadIdx.x; i < pieces; i += KV8_READ_THREADS) {
         const int kv = i / (pieces / 2), in_kv = i % (pieces / 2), row = in_kv / row_pieces, c = in_kv % row_pieces * PER;
         const size_t from = (size_t)(kv ? block_size * d : 0) + row * d + kv8_piece(row, c >> 4, d) * 16 + (c & 15);
         const size_t scale_from = (size_t)2 * block_size * d + 4 * (kv * block_size + row);
         T *out = (kv ? v_out : k_out) + (size_t)row * G * d + c;
-        for (int r0 = blockIdx.x * at_once + mine; r0 < records; r0 += gridDim.x * at_once * KV8_READ_AHEAD) {
+        for (int r0 = blockIdx.x; r0 < records; r0 += gridDim.x * KV8_READ_AHEAD) {
             uint32_t codes[KV8_READ_AHEAD][PER / 4];
             float scale[KV8_READ_AHEAD];
             int n[KV8_READ_AHEAD], g[KV8_READ_AHEAD];
 #pragma unroll
             for (int u = 0; u < KV8_READ_AHEAD; u++) {
-                const int r = r0 + u * gridDim.x * at_once;
+                const int r = r0 + u * gridDim.x;
                 n[u] = r < records ? r / G : -1;
                 g[u] = r - n[u] * G;
 #pragma unroll
@@ -546,7 +544,7 @@ extern "C" int hfb_kv8_read(const void *cache, int64_t num_pages, const int32_t 
         return fail(HFB_EINVAL, "kv8_read: bad arguments (G=%d)", G);
     if (!kv8_sizes(block_size, d)) return fail(HFB_ENOTSUP, "kv8_read: head size %d or page of %d tokens (multiples of 16 up to 256, 1..1024)", d, block_size);
     if (((uintptr_t)cache | (uintptr_t)k_out | (uintptr_t)v_out) & 15) return fail(HFB_EINVAL, "kv8_read: arrays must be 16-byte aligned");
-    const int pieces = 2 * block_size * (d / (out_dt == HFB_F32 ? 4 : 8)), at_once = pieces < KV8_READ_THREADS ? KV8_READ_THREADS / pieces : 1;
+    const int pieces = 2 * block_size * (d / (out_dt == HFB_F32 ? 4 : 8));
     if (N * G >= (1ll << 31) - (1 << 24)) return fail(HFB_ENOTSUP, "kv8_read: %lld pages of %d heads", (long long)N, G);
     const int record = kv8_record_bytes(block_size, d);
     if (record <= 24 * 1024) {
@@ -569,8 +567,7 @@ extern "C" int hfb_kv8_read(const void *cache, int64_t num_pages, const int32_t 
                                       error_word());
         return check_pdl_launch(g_launch_err, "kv8_read");
     }
-    const long long blocks = (N * G + at_once - 1) / at_once;
-    const int grid = (int)(blocks < 148 * 8 ? blocks : 148 * 8);          // (as many as are resident)
+    const int grid = (int)(N * G < 148 * 8 ? N * G : 148 * 8);            // (as many as are resident)
     if (out_dt == HFB_F32)
         g_launch_err = launch_pdl(kv8_read_kernel<float>, dim3(grid), dim3(KV8_READ_THREADS), 0, (cudaStream_t)s, (const uint8_t *)cache, (long long)num_pages,
                                   pages, used, (float *)k_out, (float *)v_out, (int)(N * G), block_size, G, d, record, error_word());
