@@ -104,16 +104,16 @@ __device__ __forceinline__ void mma_f16(float *c, uint32_t a0, uint32_t a1, uint
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// D: head size; NT: columns (token, head) of a tile in eights; STAGES: tiles of 64 keys in flight; OPTS: a cap or slopes; KH: sixteens of
-// keys a warp and step.  Two groups of 4 / KH computing warps take the tiles in turn.
-template <int D, int NT, int STAGES, bool OPTS, int KH, int CTAS>
-__global__ void __launch_bounds__(32 * (8 / KH + 1), CTAS)
+// D: head size; NT: columns (token, head) of a tile in eights; STAGES: tiles of 64 keys in flight; OPTS: a cap or slopes.  Two groups of four
+// computing warps take the tiles in turn, a warp has 16 keys of each.
+template <int D, int NT, int STAGES, bool OPTS, int CTAS>
+__global__ void __launch_bounds__(32 * 9, CTAS)
 kv8_few_kernel(Kv8FewParams f, int *err)
 {
     const Kv8Params &p = f.a;
     // (a stage belongs to one of the two groups of warps: one that took turns on it could find the phase before its own complete)
     static_assert(STAGES % 2 == 0, "the groups of warps have stages of their own");
-    constexpr int WARPS = 8 / KH, GROUP = WARPS / 2, THREADS = 32 * (WARPS + 1);
+    constexpr int WARPS = 8, GROUP = WARPS / 2, THREADS = 32 * (WARPS + 1);
     constexpr int COLS = 8 * NT, CH = D / 16, OROW = D + 4;  // (rows of the merge buffer in different banks)
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 127u) & ~127u;
@@ -290,22 +290,19 @@ kv8_few_kernel(Kv8FewParams f, int *err)
         const float log2e = 1.4426950408889634f, cap2 = p.softcap * log2e;
         const bool capped = p.softcap > 0.f;
         const int c4 = lane & 3, row8 = lane >> 2;
-        const int kbase = (warp % GROUP) * 16 * KH, group = warp / GROUP;
+        const int kbase = (warp % GROUP) * 16, group = warp / GROUP;
         // ldmatrix: lanes 0..7 and 8..15 name the rows of two eights of keys, the upper lanes the same rows one piece further; this lane
-        // holds the scores of the keys `row8` and `row8 + 8` of each sixteen
+        // holds the scores of the keys `row8` and `row8 + 8` of the warp's sixteen
         const int turn = D == 128 ? lane & 7 : (lane & 7) >> 1;
-        uint32_t piece[KH][CH / 2], s_at[KH][2];
+        uint32_t piece[CH / 2], s_at[2];
+        const int kk = kbase + (lane & 7) + ((lane >> 3) & 1) * 8;
 #pragma unroll
-        for (int h = 0; h < KH; h++) {
-            const int kk = kbase + 16 * h + (lane & 7) + ((lane >> 3) & 1) * 8;
+        for (int c = 0; c < CH / 2; c++)
+            piece[c] = (uint32_t)(kk / bs) * p.record + (uint32_t)(kk % bs) * D + (uint32_t)((2 * c + (lane >> 4)) ^ turn) * 16u;
 #pragma unroll
-            for (int c = 0; c < CH / 2; c++)
-                piece[h][c] = (uint32_t)(kk / bs) * p.record + (uint32_t)(kk % bs) * D + (uint32_t)((2 * c + (lane >> 4)) ^ turn) * 16u;
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int k = kbase + 16 * h + 8 * u + row8;
-                s_at[h][u] = (uint32_t)(k / bs) * p.record + 2u * bs * D + 4u * (k % bs);
-            }
+        for (int u = 0; u < 2; u++) {
+            const int k = kbase + 8 * u + row8;
+            s_at[u] = (uint32_t)(k / bs) * p.record + 2u * bs * D + 4u * (k % bs);
         }
         const uint32_t v_codes = (uint32_t)bs * D, v_scales = 4u * bs;
         const uint32_t all_pages = (1u << pages) - 1u;
@@ -389,48 +386,42 @@ kv8_few_kernel(Kv8FewParams f, int *err)
                 const uint8_t *sg = gen + (tiles0 - base) + s * stage_bytes;
                 const uint32_t mask = page_mask[s];
                 // (two sums a score, of the even and the odd pieces of a row: a chain of products half as long)
-                float sc[KH][NT][4], sd[KH][NT][4];
+                float sc[NT][4], sd[NT][4];
 #pragma unroll
-                for (int c = 0; c < CH / 2; c++)
+                for (int c = 0; c < CH / 2; c++) {
+                    uint32_t w0, w1, w2, w3;
+                    ldsm_x4(st + piece[c], w0, w1, w2, w3);
+                    const uint32_t a0 = bytes_f16(w0, 0x4140), a1 = bytes_f16(w1, 0x4140), a2 = bytes_f16(w0, 0x4342), a3 = bytes_f16(w1, 0x4342);
+                    const uint32_t b0 = bytes_f16(w2, 0x4140), b1 = bytes_f16(w3, 0x4140), b2 = bytes_f16(w2, 0x4342), b3 = bytes_f16(w3, 0x4342);
 #pragma unroll
-                    for (int h = 0; h < KH; h++) {
-                        uint32_t w0, w1, w2, w3;
-                        ldsm_x4(st + piece[h][c], w0, w1, w2, w3);
-                        const uint32_t a0 = bytes_f16(w0, 0x4140), a1 = bytes_f16(w1, 0x4140), a2 = bytes_f16(w0, 0x4342), a3 = bytes_f16(w1, 0x4342);
-                        const uint32_t b0 = bytes_f16(w2, 0x4140), b1 = bytes_f16(w3, 0x4140), b2 = bytes_f16(w2, 0x4342), b3 = bytes_f16(w3, 0x4342);
-#pragma unroll
-                        for (int n = 0; n < NT; n++) {
-                            if (c == 0) {
-                                mma_f16_first(sc[h][n], a0, a1, a2, a3, qf[0][n][0], qf[0][n][1]);
-                                mma_f16_first(sd[h][n], b0, b1, b2, b3, qf[1][n][0], qf[1][n][1]);
-                            } else {
-                                mma_f16(sc[h][n], a0, a1, a2, a3, qf[2 * c][n][0], qf[2 * c][n][1]);
-                                mma_f16(sd[h][n], b0, b1, b2, b3, qf[2 * c + 1][n][0], qf[2 * c + 1][n][1]);
-                            }
+                    for (int n = 0; n < NT; n++) {
+                        if (c == 0) {
+                            mma_f16_first(sc[n], a0, a1, a2, a3, qf[0][n][0], qf[0][n][1]);
+                            mma_f16_first(sd[n], b0, b1, b2, b3, qf[1][n][0], qf[1][n][1]);
+                        } else {
+                            mma_f16(sc[n], a0, a1, a2, a3, qf[2 * c][n][0], qf[2 * c][n][1]);
+                            mma_f16(sd[n], b0, b1, b2, b3, qf[2 * c + 1][n][0], qf[2 * c + 1][n][1]);
                         }
                     }
-                float ks[KH][2], vs[KH][2];
+                }
+                float ks[2], vs[2];
 #pragma unroll
-                for (int h = 0; h < KH; h++)
-#pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        ks[h][u] = *(const float *)(sg + s_at[h][u]);
-                        vs[h][u] = *(const float *)(sg + s_at[h][u] + v_scales);
-                    }
+                for (int u = 0; u < 2; u++) {
+                    ks[u] = *(const float *)(sg + s_at[u]);
+                    vs[u] = *(const float *)(sg + s_at[u] + v_scales);
+                }
                 // a tile wholly inside every row's range, with all of its pages, needs no mask
                 const bool edge = kt * ABN + ABN - 1 > pos_first || kt * ABN < lo_last || mask != all_pages;
                 if (edge) {
                     // (rows behind the request's last, those that every token's mask has passed and missing pages hold anything)
 #pragma unroll
-                    for (int h = 0; h < KH; h++)
-#pragma unroll
-                        for (int u = 0; u < 2; u++) {
-                            const int k = kbase + 16 * h + 8 * u + row8;
-                            if (kt * ABN + k > pos_last || kt * ABN + k < lo_first || !(mask >> (k / bs) & 1u)) { ks[h][u] = 0.f; vs[h][u] = vm; }
-                        }
+                    for (int u = 0; u < 2; u++) {
+                        const int k = kbase + 8 * u + row8;
+                        if (kt * ABN + k > pos_last || kt * ABN + k < lo_first || !(mask >> (k / bs) & 1u)) { ks[u] = 0.f; vs[u] = vm; }
+                    }
                 }
-                const float vs_top = fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[KH - 1][0], vs[KH - 1][1]));
-                const float vs_low = fminf(fminf(vs[0][0], vs[0][1]), fminf(vs[KH - 1][0], vs[KH - 1][1]));
+                const float vs_top = fmaxf(vs[0], vs[1]);
+                const float vs_low = fminf(vs[0], vs[1]);
                 bool apart = false;
                 if (__any_sync(0xffffffffu, vs_top > 2.f * vm || vs_low < KF_APART * vm)) {
                     if (__any_sync(0xffffffffu, vs_top > 2.f * vm)) {
@@ -449,33 +440,27 @@ kv8_few_kernel(Kv8FewParams f, int *err)
                     apart = __any_sync(0xffffffffu, vs_low < KF_APART * vm);
                 }
 #pragma unroll
-                for (int h = 0; h < KH; h++)
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sc[n][e] = fmaf(sc[n][e] + sd[n][e], fac[n][e & 1], off[n][e & 1]) * ks[e >> 1];
+                if (OPTS) {
 #pragma unroll
                     for (int n = 0; n < NT; n++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) sc[h][n][e] = fmaf(sc[h][n][e] + sd[h][n][e], fac[n][e & 1], off[n][e & 1]) * ks[h][e >> 1];
-                if (OPTS) {
-#pragma unroll
-                    for (int h = 0; h < KH; h++)
-#pragma unroll
-                        for (int n = 0; n < NT; n++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                const int key = kt * ABN + kbase + 16 * h + 8 * (e >> 1) + row8;
-                                if (capped) sc[h][n][e] = cap2 * tanh_fast(sc[h][n][e]);
-                                sc[h][n][e] = fmaf(slope[n][e & 1], (float)(key - pos[n][e & 1]), sc[h][n][e]);
-                            }
+                        for (int e = 0; e < 4; e++) {
+                            const int key = kt * ABN + kbase + 8 * (e >> 1) + row8;
+                            if (capped) sc[n][e] = cap2 * tanh_fast(sc[n][e]);
+                            sc[n][e] = fmaf(slope[n][e & 1], (float)(key - pos[n][e & 1]), sc[n][e]);
+                        }
                 }
                 if (edge) {
 #pragma unroll
-                    for (int h = 0; h < KH; h++)
+                    for (int n = 0; n < NT; n++)
 #pragma unroll
-                        for (int n = 0; n < NT; n++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                const int k = kbase + 16 * h + 8 * (e >> 1) + row8, key = kt * ABN + k;
-                                if (key > pos[n][e & 1] || key < lo[n][e & 1] || !(mask >> (k / bs) & 1u)) sc[h][n][e] = -INFINITY;
-                            }
+                        for (int e = 0; e < 4; e++) {
+                            const int k = kbase + 8 * (e >> 1) + row8, key = kt * ABN + k;
+                            if (key > pos[n][e & 1] || key < lo[n][e & 1] || !(mask >> (k / bs) & 1u)) sc[n][e] = -INFINITY;
+                        }
                 }
                 float top[NT][2];
                 bool grew = false;
@@ -483,7 +468,7 @@ kv8_few_kernel(Kv8FewParams f, int *err)
                 for (int n = 0; n < NT; n++)
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
-                        top[n][i] = fmaxf(fmaxf(sc[0][n][i], sc[0][n][2 + i]), fmaxf(sc[KH - 1][n][i], sc[KH - 1][n][2 + i]));
+                        top[n][i] = fmaxf(sc[n][i], sc[n][2 + i]);
                         grew |= top[n][i] > m[n][i] + 4.f;
                     }
                 if (__any_sync(0xffffffffu, grew)) {
@@ -503,20 +488,17 @@ kv8_few_kernel(Kv8FewParams f, int *err)
                             m[n][i] = v;
                         }
                 }
+                const float vn0 = vs[0] * rv * 1024.f, vn1 = vs[1] * rv * 1024.f;
 #pragma unroll
-                for (int h = 0; h < KH; h++) {
-                    const float vn0 = vs[h][0] * rv * 1024.f, vn1 = vs[h][1] * rv * 1024.f;
+                for (int n = 0; n < NT; n++) {
 #pragma unroll
-                    for (int n = 0; n < NT; n++) {
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const int i = e & 1;
-                            const bool none = edge && sc[h][n][e] == -INFINITY;
-                            const float q = fast_exp2(sc[h][n][e] - (m[n][i] == -INFINITY ? 0.f : m[n][i]));
-                            l[n][i] += q;
-                            sc[h][n][e] = q * (e < 2 ? vn0 : vn1);
-                            if (none) sc[h][n][e] = 0.f;                  // (a value that is no number, for a row that does not see it)
-                        }
+                    for (int e = 0; e < 4; e++) {
+                        const int i = e & 1;
+                        const bool none = edge && sc[n][e] == -INFINITY;
+                        const float q = fast_exp2(sc[n][e] - (m[n][i] == -INFINITY ? 0.f : m[n][i]));
+                        l[n][i] += q;
+                        sc[n][e] = q * (e < 2 ? vn0 : vn1);
+                        if (none) sc[n][e] = 0.f;                            // (a value that is no number, for a row that does not see it)
                     }
                 }
                 // the weights in float16: all at once, or those down to 2^-24 of the largest there can be, the next 2^-24 with the sums so far (and
@@ -524,42 +506,38 @@ kv8_few_kernel(Kv8FewParams f, int *err)
                 int times = 0;
 #pragma unroll 1
                 for (;;) {
-                    uint32_t pf[KH][NT][2];
+                    uint32_t pf[NT][2];
                     bool more = false;
 #pragma unroll
-                    for (int h = 0; h < KH; h++)
+                    for (int n = 0; n < NT; n++) {
+                        if (apart) {
+                            float w[4];
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const bool small = sc[n][e] < 0.001953125f;           // 2^-9
+                                w[e] = small ? 0.f : sc[n][e];
+                                sc[n][e] = small ? sc[n][e] * 16777216.f : 0.f;
+                                more |= sc[n][e] != 0.f;
+                            }
+                            pf[n][0] = transpose8(pack_f16(w[0], w[1]));
+                            pf[n][1] = transpose8(pack_f16(w[2], w[3]));
+                        } else {
+                            pf[n][0] = transpose8(pack_f16(sc[n][0], sc[n][1]));
+                            pf[n][1] = transpose8(pack_f16(sc[n][2], sc[n][3]));
+                        }
+                    }
+#pragma unroll
+                    for (int c = 0; c < CH / 2; c++) {
+                        uint32_t w0, w1, w2, w3;
+                        ldsm_x4_t(sv + piece[c], w0, w1, w2, w3);
+                        const uint32_t a0 = codes_f16(w0, 0x4240), a1 = codes_f16(w0, 0x4341), a2 = codes_f16(w1, 0x4240), a3 = codes_f16(w1, 0x4341);
+                        const uint32_t b0 = codes_f16(w2, 0x4240), b1 = codes_f16(w2, 0x4341), b2 = codes_f16(w3, 0x4240), b3 = codes_f16(w3, 0x4341);
 #pragma unroll
                         for (int n = 0; n < NT; n++) {
-                            if (apart) {
-                                float w[4];
-#pragma unroll
-                                for (int e = 0; e < 4; e++) {
-                                    const bool small = sc[h][n][e] < 0.001953125f;           // 2^-9
-                                    w[e] = small ? 0.f : sc[h][n][e];
-                                    sc[h][n][e] = small ? sc[h][n][e] * 16777216.f : 0.f;
-                                    more |= sc[h][n][e] != 0.f;
-                                }
-                                pf[h][n][0] = transpose8(pack_f16(w[0], w[1]));
-                                pf[h][n][1] = transpose8(pack_f16(w[2], w[3]));
-                            } else {
-                                pf[h][n][0] = transpose8(pack_f16(sc[h][n][0], sc[h][n][1]));
-                                pf[h][n][1] = transpose8(pack_f16(sc[h][n][2], sc[h][n][3]));
-                            }
+                            mma_f16(o[2 * c][n], a0, a1, a2, a3, pf[n][0], pf[n][1]);
+                            mma_f16(o[2 * c + 1][n], b0, b1, b2, b3, pf[n][0], pf[n][1]);
                         }
-#pragma unroll
-                    for (int h = 0; h < KH; h++)
-#pragma unroll
-                        for (int c = 0; c < CH / 2; c++) {
-                            uint32_t w0, w1, w2, w3;
-                            ldsm_x4_t(sv + piece[h][c], w0, w1, w2, w3);
-                            const uint32_t a0 = codes_f16(w0, 0x4240), a1 = codes_f16(w0, 0x4341), a2 = codes_f16(w1, 0x4240), a3 = codes_f16(w1, 0x4341);
-                            const uint32_t b0 = codes_f16(w2, 0x4240), b1 = codes_f16(w2, 0x4341), b2 = codes_f16(w3, 0x4240), b3 = codes_f16(w3, 0x4341);
-#pragma unroll
-                            for (int n = 0; n < NT; n++) {
-                                mma_f16(o[2 * c][n], a0, a1, a2, a3, pf[h][n][0], pf[h][n][1]);
-                                mma_f16(o[2 * c + 1][n], b0, b1, b2, b3, pf[h][n][0], pf[h][n][1]);
-                            }
-                        }
+                    }
                     if (!apart) break;
                     more = __any_sync(0xffffffffu, more) && times < 3;
                     const float by = more ? 16777216.f : __uint_as_float((uint32_t)(127 - 24 * times) << 23);
@@ -689,28 +667,28 @@ kv8_few_kernel(Kv8FewParams f, int *err)
     __syncthreads();
 }
 
-template <int D, int NT, int STAGES, int KH, int CTAS, bool OPTS>
+template <int D, int NT, int STAGES, int CTAS, bool OPTS>
 static int launch_kv8_few_opts(const Kv8FewParams &f, int ctas, cudaStream_t st)
 {
-    constexpr int fixed = 128 + 256 + 2 * (128 + 8 * NT * D * 2) + 8 / KH * (8 * NT * (D + 6) + 1) * 4 + 128;
+    constexpr int fixed = 128 + 256 + 2 * (128 + 8 * NT * D * 2) + 8 * (8 * NT * (D + 6) + 1) * 4 + 128;
     constexpr int most = fixed + 4 * (KF_MAX_TILES + 1) + STAGES * ABN * (2 * D + 8);
     const int smem = fixed + 4 * (f.n_tiles + 1) + STAGES * (ABN / f.a.block_size) * f.a.record;
-    const auto kernel = kv8_few_kernel<D, NT, STAGES, OPTS, KH, CTAS>;
+    const auto kernel = kv8_few_kernel<D, NT, STAGES, OPTS, CTAS>;
     static bool configured[64] = {false};                     // (the opt-in is a property of the function on one device)
     if (!configured[current_device()]) {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
         if (e != cudaSuccess) return fail(HFB_ECUDA, "kv8_attention_few: cannot opt in to %d bytes of shared memory: %s", most, cudaGetErrorString(e));
         configured[current_device()] = true;
     }
-    g_launch_err = launch_pdl(kernel, dim3(ctas), dim3(32 * (8 / KH + 1)), smem, st, f, error_word());
+    g_launch_err = launch_pdl(kernel, dim3(ctas), dim3(32 * 9), smem, st, f, error_word());
     return check_pdl_launch(g_launch_err, "kv8_attention_few");
 }
 
-template <int D, int NT, int STAGES, int KH, int CTAS>
+template <int D, int NT, int STAGES, int CTAS>
 static int launch_kv8_few(const Kv8FewParams &f, int ctas, cudaStream_t st)
 {
-    return f.a.slopes || f.a.softcap > 0.f ? launch_kv8_few_opts<D, NT, STAGES, KH, CTAS, true>(f, ctas, st)
-                                           : launch_kv8_few_opts<D, NT, STAGES, KH, CTAS, false>(f, ctas, st);
+    return f.a.slopes || f.a.softcap > 0.f ? launch_kv8_few_opts<D, NT, STAGES, CTAS, true>(f, ctas, st)
+                                           : launch_kv8_few_opts<D, NT, STAGES, CTAS, false>(f, ctas, st);
 }
 
 }  // namespace hfb
@@ -750,6 +728,6 @@ extern "C" int hfb_kv8_attention_few(const void *q, const void *cache, const int
     f.part_o = (float *)scratch; f.part_ml = (float *)scratch + (size_t)ctas * 2 * 16 * d;
     f.counters = counters; f.n_tiles = n_tiles; f.min_steps = min_steps; f.tile_cost = tile_cost; f.kv_share = share; f.settled = settled;
     cudaStream_t st = (cudaStream_t)s;
-    if (d == 128) return cols <= 8 ? launch_kv8_few<128, 1, 4, 1, 2>(f, ctas, st) : launch_kv8_few<128, 2, 4, 1, 1>(f, ctas, st);
-    return cols <= 8 ? launch_kv8_few<64, 1, 4, 1, 2>(f, ctas, st) : launch_kv8_few<64, 2, 4, 1, 2>(f, ctas, st);
+    if (d == 128) return cols <= 8 ? launch_kv8_few<128, 1, 4, 2>(f, ctas, st) : launch_kv8_few<128, 2, 4, 1>(f, ctas, st);
+    return cols <= 8 ? launch_kv8_few<64, 1, 4, 2>(f, ctas, st) : launch_kv8_few<64, 2, 4, 2>(f, ctas, st);
 }
