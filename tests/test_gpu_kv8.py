@@ -763,3 +763,101 @@ def test_keys_beside_one_that_is_far_larger(shape, name):
             s.k[s.table[i, p // bs], p % bs], s.ks[s.table[i, p // bs], p % bs] = -100, 2.0 ** 22 * 0.02
     cache = pack(s.k, s.ks, s.v, s.vs)
     check_apart(s, q, attend(s, q, cache, H), H, cache=cache, size_of_scores=worst)
+
+
+# ---- what users get without these tests' smaller threshold; other architectures ------------------------------------------------
+
+@pytest.mark.parametrize("mask", [0, 50, -100])
+@pytest.mark.parametrize("shape", [(14, 2, 64, 16), (28, 4, 128, 16), (32, 8, 128, 16), (40, 2, 128, 8)], ids=str)
+def test_steps_below_the_prompts_kernels_threshold(shape, mask, monkeypatch):
+    """The choice as it is: steps of up to 512 rows go to the kernel of few queries, several tiles a request, and larger ones to both."""
+    H, G, d, bs = shape
+    K = native()
+    monkeypatch.setattr(K, "KV8_MANY_ROWS", 512)
+    for q_lens, kv_lens, kinds in (([9, 1, 14], [309, 200, 14], {"few"}), ([25], [700], {"few"}), ([1, 130, 2], [900, 130, 400], {"few", "many"})):
+        s = step(q_lens, kv_lens, bs, G, d, seed=d + len(q_lens))
+        assert {n.split(".")[0] for n in K.kv8_step_arrays(s.q_lens, H // G)} == kinds
+        cache = pack(s.k, s.ks, s.v, s.vs)
+        q = torch.randn(s.T, H * d, generator=s.g, device=DEV).bfloat16()
+        o = dict(sinks=torch.randn(H, device=DEV, generator=gen(2)), slopes=torch.full((H,), 0.05, device=DEV)) if mask >= 0 else {}
+        got = attend(s, q, cache, H, mask=mask, **o)
+        check(s, q, cache, got, H, mask=mask, **o)
+        assert torch.equal(got, attend(s, q, cache, H, mask=mask, settled=True, **o))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("arch", ["manapel", "tupalorn"])
+def test_other_architectures_on_8_bits(arch, dtype, monkeypatch):
+    """Layers with tails of their own (head norms, a norm over the row), windows, caches that later layers read: logits against the
+    stand-in backend's, with the tolerances of the engine's test above; prompts on either kernel, graphs and eager steps."""
+    import importlib
+    from hfcpu_b200.config import config_from_dict
+    from hfcpu_b200.engine import Engine, StepEntry
+    from hfcpu_b200.models import Model
+    from hfcpu_b200.weights.random_init import RandomSource
+    K = native()
+    monkeypatch.setattr(K, "KV8_MANY_ROWS", 512)
+    cfg = config_from_dict(importlib.import_module(arch + "_util").WIDE)
+    cpu = torch.device("cpu")
+    source = RandomSource(Model(cfg, torch.float32, cpu).tensor_specs(), 5, torch.float32, cpu, std=0.05)
+    weights = {t.name: source[t.name].to(DT[dtype]) for t in Model(cfg, torch.float32, cpu).tensor_specs()}
+    ids = [int(x) for x in torch.randint(0, 1000, (400,), generator=torch.Generator().manual_seed(1))]
+
+    def run(kv, dt, device, cuts):
+        model = Model(cfg, dt, torch.device(device)).bind({n: w.to(device) for n, w in weights.items()})
+        engine, out = Engine(model, block_size=16, max_tokens=2048, max_requests=2, kv_dtype=kv), []
+        for r, cut in enumerate(cuts):
+            engine.add_request(r)
+            at = 0
+            for n in cut:
+                got = engine.step([StepEntry(r, ids[at:at + n], [n - 1])])
+                at += n
+            out.append(torch.cat([got.clone()] + [engine.step([StepEntry(r, [5 + i], [0])]).clone() for i in range(5)]).float().cpu())
+            engine.finish_request(r)
+        return out
+    real = K.backend()
+    try:
+        K.set_backend(EmuKv8())
+        plain, emu = (run(kv, torch.float32, "cpu", [[300]])[0] for kv in ("auto", "int8"))
+    finally:
+        K.set_backend(real)
+    own = float((run("auto", DT[dtype], DEV, [[300]])[0] - plain).abs().max())
+    far = float((emu - plain).abs().max())
+    assert far > 0
+    for got in run("int8", DT[dtype], DEV, [[300], [200, 90, 10], [3, 40, 257]]):
+        assert torch.isfinite(got).all()
+        assert float((got - emu).abs().max()) <= (0.25 * far + 1e-4 if dtype == "float32" else far + 2 * own)
+    K.check_device_errors()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_two_streams_and_a_graph_at_once(d):
+    """Calls that run beside each other, each with scratch of its own: two streams' eager launches and a graph's replays, of tiles that many
+    CTAs share."""
+    K, H = native(), 8
+    s = step([1, 100, 1, 1], [9000, 4000, 30, 5000], 16, 2, d, seed=d)
+    cache = pack(s.k, s.ks, s.v, s.vs)
+    plan = {n: torch.from_numpy(a).to(DEV) for n, a in K.kv8_step_arrays(s.q_lens, H // 2).items()}
+    assert len(plan) == 6
+    qs = [torch.randn(s.T, H * d, generator=s.g, device=DEV).bfloat16() for _ in range(3)]
+    right = [attend(s, q, cache, H, plan=plan) for q in qs]
+    check(s, qs[0], cache, right[0], H)
+    bufs, outs, streams = [context() for _ in qs], [torch.zeros_like(q) for q in qs], [torch.cuda.Stream() for _ in qs]
+    attend(s, qs[2], cache, H, plan=plan, buf=bufs[2])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        attend(s, qs[2], cache, H, plan=plan, buf=bufs[2], out=outs[2])
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for o in outs:
+            o.zero_()
+        for i, stream in enumerate(streams):
+            stream.wait_stream(torch.cuda.current_stream())
+        for _ in range(3):
+            for i, stream in enumerate(streams):
+                with torch.cuda.stream(stream):
+                    graph.replay() if i == 2 else attend(s, qs[i], cache, H, plan=plan, buf=bufs[i], out=outs[i])
+        for stream in streams:
+            torch.cuda.current_stream().wait_stream(stream)
+        assert all(torch.equal(a, b) for a, b in zip(outs, right))
+    K.check_device_errors()
