@@ -25,8 +25,8 @@
 //   is made up to four times, for weights of 2^-24 of each other: down to 2^-91 of the largest they keep their 11 bits, beside keys that
 //   their token does not see or gives no weight.
 //
-// Measured (28 heads of 128 on 4): 64 requests of up to 8,192 tokens 70 us, 0.61 of the measured bandwidth (the bfloat16 cache's kernel, which
-// reads twice the bytes, 113 us); eight of up to 32,768 tokens 43 us, 0.49 (65).  About 15 us of each are the start of a launch, its
+// Measured (28 heads of 128 on 4): 64 requests of up to 8,192 tokens 70 us, 0.60 of the measured bandwidth (the bfloat16 cache's kernel, which
+// reads twice the bytes, 108 us); eight of up to 32,768 tokens 43 us, 0.49 (59).  About 15 us of each are the start of a launch, its
 // first copies and its merges, which a launch that follows another one on the stream hides in part.
 //
 // Work is cut evenly: all steps (64 keys of one tile and key/value head) stand in one row, a tile's behind `tile_cost` empty ones

@@ -11,8 +11,8 @@
 //   two multiplications for every four scores, 3 % of the time.)
 // * 32 keys whose scales lie further apart than 2^11, and values beyond 2^45 or 2^-45, have a power of two each.  A row's weights then go by the
 //   largest score and reference among the keys that it sees, its sum by the scores alone, an exponential each: what a row does not see, or
-//   gives no weight, takes no bits from what it does.  Steps of such keys take several times as long (km_apart); all others pay 2 % of the
-//   time for looking (309 and 315 us for the portion below).
+//   gives no weight, takes no bits from what it does.  Steps of such keys take four times as long (km_apart: 1,325 us if all of the portion
+//   below are); all others pay 2 % of the time for looking (309 and 315 us).
 // * each of these warps asks for its keys' codes of the next tile as soon as it has converted the last ones, and both operands have two
 //   places, so that the conversion runs a tile ahead of the products.
 // * a row whose key or value is no number makes its scores so and leaves its values zero: a weight of zero stays zero in the sums of the
@@ -28,8 +28,9 @@
 // * work is cut evenly (as in kv8_few.cu): a step is a tile of keys of one double tile and key/value head, CTA c of C walks steps c N / C to
 //   (c + 1) N / C.  What a CTA has of a double tile that others share goes to scratch, and whoever brings its last piece merges them, in
 //   the order of the keys.  (Whole double tiles a CTA: 228 items of 2,048 tokens and 28 heads are two rounds on 148 SMs where 1.5 would do.)
-// Measured: 2,048 tokens behind 6,144, 28 heads of 128 on 4: 312 us, 674 TFLOP/s, 0.41 of the measured bf16 rate; the bfloat16 cache's kernel
-// takes 288 us.  Steps without the conversion take 268: its instructions and the softmax's share the issue slots.
+// Measured: 2,048 tokens behind 6,144, 28 heads of 128 on 4: 315 us, 668 TFLOP/s, 0.41 of the measured bf16 rate; the bfloat16 cache's kernel
+// takes 270 us (both a pass among others; alone 330 and 289).  Latency bounds it: half of the issue slots stay empty and the tensor pipe is
+// active a third of the time, with 13 warps an SM (128 registers a thread) waiting for TMEM reads and for each other's results.
 // Barrier waits are bounded (HFB_ERR_WAIT, TMEM freed; tc_ptx.cuh).
 #include <cuda_fp16.h>
 
@@ -447,8 +448,10 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                 uint32_t kf = km_above(warp_max(k_scale)), vf = km_above(warp_max(v_scale));
                 const bool number = sc.x == sc.x && sc.y == sc.y;
                 // ... for all 32 keys, unless they are so far apart that float16 would lose the smaller ones, or so large or small that a row's weights
-                // and exponentials could not go by one reference: then every key has its own
-                const bool apart = __any_sync(0xffffffffu, there && number && (km_above(k_scale) + KM_APART < kf || km_above(v_scale) + KM_APART < vf)) ||
+                // and exponentials could not go by one reference: then every key has its own.  (Rows of zeros, which have the least scale there is, don't
+                // count, nor do those with them whose largest number is below 1.5e-36.)
+                auto far_below = [&](float scale, uint32_t f) { return scale > 1.17549435e-38f && km_above(scale) + KM_APART < f; };
+                const bool apart = __any_sync(0xffffffffu, there && number && (far_below(k_scale, kf) || far_below(v_scale, vf))) ||
                                    vf + KM_RANGE < 127u || vf > 127u + KM_RANGE;
                 const uint32_t k_ref = kf, v_ref = vf;
                 if (apart && there && number) { kf = km_above(k_scale); vf = km_above(v_scale); }
@@ -562,7 +565,7 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
                 }
                 const float by_head = unit * hscale;
                 // (loops over the quarters of a tile stay loops: eight warps of these run beside four that convert, and unrolled their
-                // instructions do not stay in the caches: 410 us for the portion named above, 358 so)
+                // instructions do not stay in the caches: when that was tried, 410 us for the portion named above against 358)
                 auto load32 = [&](int q, uint32_t (&raw)[32]) { tmem_ld16(tS + 32 * q, raw); tmem_ld16(tS + 32 * q + 16, raw + 16); };
                 auto k_ref = [&](int q) { return km_load1(s_at + 4u * q); };
                 auto v_log = [&](int q) { return km_load1(s_at + 16u + 4u * q); };

@@ -153,7 +153,7 @@ class NativeBackend:
         # attention of few queries over the 8-bit cache: CTAs per SM by (heads of 128, more than 8 places a tile), fewest steps of a CTA
         self.kv8_ctas_per_sm, self.kv8_min_steps = {(False, False): 2, (False, True): 2, (True, False): 2, (True, True): 1}, 1
         self.kv8_tile_cost = 6                    # ... and what a tile's start and end are reckoned as, in steps
-        # the same of prompt portions, whose steps are long: without a cap of the scores, and with one, whose steps are twice as long.  us with
+        # the same of prompt portions, whose steps are long: without a cap of the scores, and with one, whose steps are twice as long.  us, alone, with
         # 1 | 3 | 6, heads of 128 on 4: 2,048 tokens alone 123 | 94 | 100, 16 times 100 behind up to 8,192 266 | 188 | 193, a portion of 2,048
         # behind 6,144 332 | 328 | 330; with a cap, 3 times 333 tokens, 16 heads of 64: 49 | 55 | 66
         self.kv8_many_tile_cost = 3, 1
