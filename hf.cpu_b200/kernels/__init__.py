@@ -389,7 +389,8 @@ def rope_kv8_write(qkv, cos_sin, n_rot, positions, slots, q_out, cache, H, G, d,
 
 
 def kv8_write(k, v, slots, cache, G, d, block_size) -> None:
-    """Keys and values [T, G * d] as they are into a cache in 8 bits (for layers whose own tails have made them)."""
+    """Keys and values [T, G * d] as they are into a cache in 8 bits (for layers whose own tails have made them, and rounded them to the run's
+    type already)."""
     T = k.shape[0]
     if k.dtype not in _KV8_TYPES:
         raise ValueError("kv8_write: rows are float32 or bfloat16")
@@ -428,7 +429,7 @@ KV8_MANY, KV8_MANY_ROWS = 32, 512
 
 def kv8_step_arrays(q_lens, heads_per_group: int):
     """Tile lists of a step's tokens for :func:`paged_attention_kv8`, as named int32 arrays: a tile is ``nt`` consecutive tokens of request
-    ``seq`` from token ``t0`` of the step on.  "few": up to 16 (token, head) places of requests that bring few tokens; "many": two tiles
+    ``seq``, at consecutive positions, from token ``t0`` of the step on.  "few": up to 16 (token, head) places of requests that bring few tokens; "many": two tiles
     of 128 rows of those that bring more."""
     import numpy as np
     q = np.asarray(q_lens, dtype=np.int32)
