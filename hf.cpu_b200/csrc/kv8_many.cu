@@ -847,6 +847,9 @@ kv8_many_kernel(Kv8ManyParams f, int *err)
     // ---- teardown -------------------------------------------------------------------------------------------------------------------
     tc_fence_before();
     __syncthreads();
+    if (*abort_flag != 0 && threadIdx.x == 0)                            // a wait ran out: products still in flight end before their operands go away
+        for (int i = 0; i < 2000; i++) __nanosleep(1000);
+    __syncthreads();
     if (warp == 12) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(KM_TMEM_COLS) : "memory");
